@@ -342,6 +342,149 @@ int va_linear_bf16(va_ctx* ctx, const void* a, const void* w_t, const float* bia
                    const float* scale, const float* residual, float* out, int64_t m, int n, int k,
                    void* stream);
 
+/* ------------------------------------------------------------- streaming attention
+ * Operators for windows that grow view by view and for several requests in one call
+ * (no counterpart in the reference, which runs one request's fixed window): rotary
+ * positions over several axes, attention with score terms and masks over packed
+ * documents, and a quantised key/value cache with the attention that reads it.
+ * All data pointers are device pointers on the context's device; every call runs on
+ * `stream` of that device (whichever device is current), launches kernels only,
+ * allocates nothing and can be captured into a CUDA graph.  No call keeps state
+ * between calls, so calls on different streams do not disturb each other.  Inference
+ * only: there are no backward passes. */
+#define VA_BF16 0
+#define VA_F16 1
+#define VA_F32 2
+
+/* A token-major tensor of heads: element (token, head, c) of `data` is at token *
+ * token_stride + head * head_stride + c (strides in elements, the head's channels
+ * contiguous), so q, k and v may be views of one packed projection. */
+typedef struct va_heads {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+  int32_t heads;
+  int32_t dtype; /* VA_BF16, VA_F16 or VA_F32 */
+} va_heads;
+
+/* Rotary positions over 1 to 4 axes (for example time, height, width).  Axis a turns
+ * section[a] channels of every head (even; the sum at most head_dim; channels past the
+ * sum are copied).
+ *   VA_ROPE_PER_AXIS: section a is a rotary block of its own, pair i of it turned by
+ *     position[a] * base^(-2 i / section[a]) (two axes of 32 channels of 64: the
+ *     layer path's 2-D RoPE);
+ *   VA_ROPE_SHARED: one block of S = sum of the sections; pair i is turned by
+ *     position[a(i)] * base^(-2 i / S), a(i) the section whose half holds pair i
+ *     (section 0 the first section[0] / 2 pairs, and so on).
+ * pairing 0: pair i of a block of B channels is (i, i + B/2); 1: (2i, 2i + 1). */
+#define VA_ROPE_PER_AXIS 0
+#define VA_ROPE_SHARED 1
+typedef struct va_rope_axes {
+  int32_t axes;
+  int32_t section[4];
+  int32_t layout;
+  int32_t pairing;
+  float base;
+} va_rope_axes;
+/* q_out = rotated q and, with k non-NULL, k_out = rotated k, in one launch.
+ * positions int32 [rows, axes] on the device (any value; angles are reduced in 64
+ * bits).  head_dim even, 2..256.  BF16, F16 or F32, the same type throughout.
+ * An output may be its input (same data and strides) and must not overlap it
+ * otherwise.  rows 0: nothing to do. */
+int va_rope_axes_device(va_ctx* ctx, const va_rope_axes* rope, int64_t rows, int head_dim,
+                        const int32_t* positions, const va_heads* q, const va_heads* q_out,
+                        const va_heads* k, const va_heads* k_out, void* stream);
+
+/* Score terms and mask of one attention.  Row i of a document with Lq query rows and
+ * Lk keys stands at key position p = i + Lk - Lq (its last row at the last key); with
+ * f(x) = floor(x / frame), frame = tokens per frame (1: single tokens):
+ *   score(i, j) = cap * tanh(scale * q.k / cap) - slope[head] * |f(p) - f(j)|
+ *   visible(i, j) = not causal, or f(j) <= f(p), or j < prefix[document]
+ * score_cap 0: no cap; scale 0: 1/sqrt(64).  A row that sees no key gives zeros.
+ * Query head h reads key head h / (heads / kv_heads). */
+typedef struct va_attn_terms {
+  int32_t heads;    /* 1..128 */
+  int32_t kv_heads; /* divides heads */
+  int32_t causal;
+  int32_t frame;    /* >= 1 */
+  float scale;
+  float score_cap;
+} va_attn_terms;
+
+/* Masked attention over packed documents, head_dim 64: document b's queries are rows
+ * [q_offsets[b], q_offsets[b+1]) and its keys rows [k_offsets[b], k_offsets[b+1]); no
+ * document sees another's keys.  The plan holds the work list of one such layout on
+ * the context's device.  All arrays are host arrays, read during the call:
+ * q_offsets, k_offsets [documents + 1] ascending from >= 0, below 2^31 rows, at most
+ * 2^24 keys per document; prefix [documents] >= 0 or NULL; slopes [heads] finite or
+ * NULL.  Create allocates device memory (not during a capture); a plan serves any
+ * number of calls, also at once, and is destroyed when none is running, and before
+ * its context. */
+typedef struct va_attn_plan va_attn_plan;
+int va_attn_plan_create(va_ctx* ctx, const va_attn_terms* terms, int documents, const int64_t* q_offsets,
+                        const int64_t* k_offsets, const int64_t* prefix, const float* slopes,
+                        va_attn_plan** out);
+void va_attn_plan_destroy(va_attn_plan* plan);
+/* The launch a plan of these shapes makes on a GPU of `sms` multiprocessors, computed
+ * on the host (no GPU needed).  plan[5]: query tiles (all key heads), CTAs per tile
+ * (each takes a range of its keys), query tokens per tile, 128-key tiles of all query
+ * tiles together, CTAs of the launch.  The checks are those of va_attn_plan_create. */
+int va_attn_plan_shape(const va_attn_terms* terms, int documents, const int64_t* q_offsets,
+                       const int64_t* k_offsets, const int64_t* prefix, int sms, int64_t* plan);
+/* q, out: [.., heads]; k, v: [.., kv_heads]; all BF16 or all F16; data 16-byte
+ * aligned, strides multiples of 8 elements, heads not overlapping.  Only rows of the
+ * plan's documents are read or written, but a document's own key and value rows must be
+ * finite: a NaN or infinity in one may reach rows that do not see it.  out may be q. */
+int va_masked_attention_device(va_ctx* ctx, const va_attn_plan* plan, const va_heads* q, const va_heads* k,
+                               const va_heads* v, const va_heads* out, void* stream);
+
+/* Quantised key/value cache of `documents` sequences, in buffers the caller owns:
+ * codes [documents][kv_heads][capacity][64] bytes (16-byte aligned), scales
+ * [documents][kv_heads][capacity] F32 (16-byte aligned).  One scale per token and head:
+ *   VA_KV_INT8: scale = amax / 127 (at least 2^-126), code = x / scale rounded half to even;
+ *   VA_KV_E4M3: scale = the smallest power of two (at least 2^-126) with amax <= 448 *
+ *     scale, code = e4m3(x / scale), so that the division is exact.
+ * A head with a NaN or an infinity is stored with scale NaN and reads as NaN. */
+#define VA_KV_INT8 0
+#define VA_KV_E4M3 1
+typedef struct va_kv_cache {
+  int32_t documents;
+  int32_t kv_heads;
+  int64_t capacity; /* tokens per document, below 2^31 */
+  int32_t format;
+  int32_t reserved; /* 0 */
+  void* k_codes;
+  void* v_codes;
+  float* k_scales;
+  float* v_scales;
+} va_kv_cache;
+/* Appends: rows [offsets[b], offsets[b+1]) of k and v become tokens [lens[b] - n,
+ * lens[b]) of document b, n = offsets[b+1] - offsets[b]; lens = tokens held after the
+ * call.  offsets int32 [documents + 1] and lens int32 [documents] are device arrays,
+ * read when the kernel runs (a captured call follows their contents).  rows = rows of
+ * k and v; rows outside every document are not read.  A document with lens[b] - n < 0, lens[b] >
+ * capacity, or offsets out of [0, rows] or descending is skipped and reported by
+ * va_check_device (VA_ERR_DEVICE).  k, v [rows, kv_heads] of one type. */
+int va_kv_cache_write_device(va_ctx* ctx, const va_kv_cache* cache, int64_t rows, const int32_t* offsets,
+                             const int32_t* lens, const va_heads* k, const va_heads* v, void* stream);
+/* Reads back: rows [offsets[b], offsets[b+1]) of k and v receive tokens first[b].. of
+ * document b (first NULL: 0) as code * scale, limited to the type's largest finite
+ * value; other rows are left as they were.  Bad offsets or token ranges outside
+ * [0, capacity): as above. */
+int va_kv_cache_read_device(va_ctx* ctx, const va_kv_cache* cache, int64_t rows, const int32_t* offsets,
+                            const int32_t* first, const va_heads* k, const va_heads* v, void* stream);
+/* Attention of a few new tokens per document over the cache (terms as above): rows
+ * [offsets[b], offsets[b+1]) of q are the last tokens of the lens[b] held, normally
+ * just written.  prefix int32 [documents] and slopes F32 [heads] on the device, or
+ * NULL.  max_tokens: the most rows a document usually has (sizes the launch; more rows
+ * are served too, more slowly).  q, out [rows, heads] BF16 or F16, 16-byte aligned,
+ * strides multiples of 8 elements.  Bad offsets, or lens outside [0, capacity]: as
+ * above, and the document's rows of out are left as they were.  For many new tokens
+ * read the cache back and run va_masked_attention_device. */
+int va_cache_attention_device(va_ctx* ctx, const va_kv_cache* cache, const va_attn_terms* terms, int64_t rows,
+                              const int32_t* offsets, const int32_t* lens, int max_tokens, const int32_t* prefix,
+                              const float* slopes, const va_heads* q, const va_heads* out, void* stream);
+
 /* Host-side view scheduling (backbone.rs:133-224, engine.rs:198-205). */
 /* select_reference_view_saddle: cls [views, embed] F32 -> reference view index. */
 int va_select_reference_view_saddle(const float* cls, int views, int embed, int* out_index);

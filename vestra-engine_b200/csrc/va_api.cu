@@ -879,13 +879,26 @@ int read_device_error(va_ctx* c) {
     // An aborted split-tail CTA may have left an arrival counter behind.
     cudaMemset(c->part_count, 0, static_cast<size_t>(va::flash_part_slots(c->sms)) * sizeof(int));
     char buf[128];
-    std::snprintf(buf, sizeof(buf), "device error word %d (a bounded wait timed out)", h);
+    std::snprintf(buf, sizeof(buf), "device error word %d (%s)", h,
+                  h == va::kDevBadLengths ? "offsets or lengths of a cache call out of range"
+                                          : "a bounded wait timed out");
     return fail(c, VA_ERR_DEVICE, buf);
   }
   return VA_OK;
 }
 
 }  // namespace
+
+namespace va {
+CtxCore ctx_core(const va_ctx* c) { return CtxCore{c->device, c->sms, c->err}; }
+int ctx_fail(va_ctx* c, int code, const char* msg) {
+  try {
+    return fail(c, code, msg);
+  } catch (...) {
+    return code;
+  }
+}
+}  // namespace va
 
 extern "C" {
 

@@ -10,8 +10,19 @@
 #include <stdint.h>
 
 struct va_gguf;
+struct va_ctx;
 
 namespace va {
+
+// What the streaming operators (va_stream.cu) need of a context.
+struct CtxCore {
+  int device;
+  int sms;
+  int* err;  // device error word
+};
+CtxCore ctx_core(const va_ctx* c);
+// Records msg as the context's last error and returns code.
+int ctx_fail(va_ctx* c, int code, const char* msg);
 
 // ---- QKV projection (K1): X[rows,E] bf16 x Wqkv^T -> Q,K,V token-major bf16 ----
 constexpr int kMaxRanks = 8;
@@ -192,6 +203,11 @@ bool encode_tma_3d_f32_strided(CUtensorMap* map, const void* base, uint64_t d0, 
                                uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes,
                                uint32_t b0, uint32_t b1, uint32_t b2);
 
+// Two-byte elements [d2][d1][64] with explicit byte strides of dims 1 and 2, box
+// 64 x b1 x b2, SWIZZLE_128B (bf16 or f16: TMA only copies and zero-fills).
+bool encode_tma_heads(CUtensorMap* map, const void* base, uint64_t d1, uint64_t d2, uint64_t stride1_bytes,
+                      uint64_t stride2_bytes, uint32_t b1, uint32_t b2);
+
 // Launchers return cudaSuccess or the launch error; kernels report device-side
 // failures through *err (see DevError in va_ptx.cuh).
 cudaError_t launch_qkv_gemm(const __nv_bfloat16* x, const __nv_bfloat16* w_qkv_t, int rows,
@@ -285,5 +301,77 @@ class GgufStager {
   size_t cap_ = 0;
   int slot_ = 0;
 };
+
+// ---- streaming attention (va_rope_axes.cu, va_kv_cache.cu, va_masked.cu) ----
+// One [rows][heads][channels] operand: element strides.
+struct HeadsRef {
+  void* data;
+  int64_t token_stride, head_stride;
+  int heads;
+};
+enum ElemType { kBf16 = 0, kF16 = 1, kF32 = 2 };
+
+constexpr int kRopeMaxPairs = 128;
+struct RopeAxesArgs {
+  double turns[kRopeMaxPairs];        // turns per unit of position, by pair
+  uint8_t first[kRopeMaxPairs];       // channel of the pair's first element
+  uint8_t second[kRopeMaxPairs];      // and of its second
+  uint8_t axis[kRopeMaxPairs];
+  int pairs, axes, head_dim, rotated;  // rotated = sum of the sections
+  int pairing;
+  int min_half;                       // gcd of the halves of all blocks and sections
+  int64_t rows;
+  const int32_t* positions;
+  HeadsRef in[2], out[2];             // q and k; heads 0: absent
+};
+cudaError_t launch_rope_axes(const RopeAxesArgs& a, int dtype, cudaStream_t st);
+
+struct KvCacheRef {
+  int documents, kv_heads, e4m3;
+  int64_t capacity;
+  uint8_t* codes[2];  // K, V
+  float* scales[2];
+};
+cudaError_t launch_kv_write(const KvCacheRef& c, int dtype, int64_t rows, const int32_t* offsets,
+                            const int32_t* lens, const HeadsRef& k, const HeadsRef& v, int* err,
+                            cudaStream_t st);
+cudaError_t launch_kv_read(const KvCacheRef& c, int dtype, int64_t rows, const int32_t* offsets,
+                           const int32_t* first, const HeadsRef& k, const HeadsRef& v, int* err,
+                           cudaStream_t st);
+
+// Score terms of the masked and the cache attention.
+struct AttnTerms {
+  int heads, kv_heads, causal, frame;
+  float scale_log2;  // scale * log2(e)
+  float cap_in;      // 2 * log2(e) * scale / cap: ex2(cap_in * q.k) = e^(2 scale q.k / cap); 0: no cap
+  float cap_out;     // cap * log2(e)
+};
+cudaError_t launch_cache_attention(const KvCacheRef& c, const AttnTerms& t, int dtype, int64_t rows,
+                                   const int32_t* offsets, const int32_t* lens, int max_tokens,
+                                   const int32_t* prefix, const float* slopes, const HeadsRef& q,
+                                   const HeadsRef& out, int sms, int* err, cudaStream_t st);
+
+// One query tile of a document (masked attention): all its key heads share the item.
+struct MaskedItem {
+  int q_row;    // first query row (tile)
+  int tokens;   // query tokens of the tile
+  int k_row;    // first key row of the document
+  int keys;     // keys the tile's last row sees (0: the rows are empty)
+  int first;    // key position of the tile's first token (may be negative)
+  int doc_keys; // keys of the document
+  int prefix;
+};
+struct MaskedArgs {
+  AttnTerms t;
+  int group, tile_tokens, items, splits;
+  const MaskedItem* item;
+  const float* slopes;      // [heads] device, times log2(e); nullptr: no bias
+  const float* frame_of;    // [keys + padding] F32 frame index of a key position (bias only)
+  HeadsRef out;
+};
+cudaError_t launch_masked(const HeadsRef& q, const HeadsRef& k, const HeadsRef& v, int64_t q_rows, int64_t k_rows,
+                          const MaskedArgs& a, int dtype, int* err, cudaStream_t st);
+// CTAs per query tile for tiles of these key counts (descending) on `sms` SMs.
+int masked_splits(const int* key_tiles, int64_t items, int kv_heads, int sms);
 
 }  // namespace va

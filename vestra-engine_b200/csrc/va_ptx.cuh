@@ -25,6 +25,7 @@ enum DevError : int {
   kDevTimeoutConsumer = 3,  // softmax / epilogue gave up waiting for the accumulator
   kDevBadShape = 4,         // a kernel saw a shape its host checks should have rejected
   kDevTimeoutPeer = 5,      // the K'/V exchange barrier gave up waiting for a peer GPU
+  kDevBadLengths = 6,       // offsets or lengths of a cache call were out of range
 };
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s per wait

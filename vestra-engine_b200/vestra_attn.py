@@ -54,7 +54,13 @@ EXPORTED = [
     "va_gguf_meta_arr_f32", "va_gguf_meta_arr_str", "va_gguf_tensor_count", "va_gguf_tensor_name",
     "va_gguf_tensor_info", "va_gguf_tensor_check", "va_gguf_tensor_device", "va_gguf_tensor_f32",
     "va_gguf_model_config", "va_load_model_gguf",
+    "va_rope_axes_device", "va_attn_plan_create", "va_attn_plan_destroy", "va_attn_plan_shape",
+    "va_masked_attention_device", "va_kv_cache_write_device", "va_kv_cache_read_device", "va_cache_attention_device",
 ]
+# Element types of the streaming-attention operators, rope layouts and cache formats.
+VA_BF16, VA_F16, VA_F32 = 0, 1, 2
+ROPE_LAYOUTS = {"per_axis": 0, "shared": 1}
+KV_INT8, KV_E4M3 = 0, 1
 
 
 class VestraError(RuntimeError):
@@ -97,6 +103,30 @@ class VaModelConfig(ctypes.Structure):
 _lib = None
 _vp = ctypes.c_void_p
 _f32p = ctypes.POINTER(ctypes.c_float)
+
+class VaHeads(ctypes.Structure):
+    """va_heads: a token-major [rows, heads, channels] operand with element strides."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class VaRopeAxes(ctypes.Structure):
+    _fields_ = [("axes", ctypes.c_int32), ("section", ctypes.c_int32 * 4), ("layout", ctypes.c_int32),
+                ("pairing", ctypes.c_int32), ("base", ctypes.c_float)]
+
+
+class VaAttnTerms(ctypes.Structure):
+    _fields_ = [("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("frame", ctypes.c_int32), ("scale", ctypes.c_float), ("score_cap", ctypes.c_float)]
+
+
+class VaKvCache(ctypes.Structure):
+    _fields_ = [("documents", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("capacity", ctypes.c_int64),
+                ("format", ctypes.c_int32), ("reserved", ctypes.c_int32), ("k_codes", ctypes.c_void_p),
+                ("v_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p)]
+
+
 _i32p = ctypes.POINTER(ctypes.c_int)
 
 
@@ -187,6 +217,16 @@ def load_library(path: str = LIB_PATH):
         "va_gguf_tensor_f32": ([_vp, ctypes.c_char_p, c_int, _vp, i64], c_int),
         "va_gguf_model_config": ([_vp, ctypes.POINTER(VaModelConfig)], c_int),
         "va_load_model_gguf": ([_vp, _vp, ctypes.POINTER(i64)], c_int),
+        "va_rope_axes_device": ([_vp, ctypes.POINTER(VaRopeAxes), i64, c_int, _vp, _vp, _vp, _vp, _vp, _vp], c_int),
+        "va_attn_plan_create": ([_vp, ctypes.POINTER(VaAttnTerms), c_int, _vp, _vp, _vp, _vp, ctypes.POINTER(_vp)],
+                                c_int),
+        "va_attn_plan_destroy": ([_vp], None),
+        "va_attn_plan_shape": ([ctypes.POINTER(VaAttnTerms), c_int, _vp, _vp, _vp, c_int, _vp], c_int),
+        "va_masked_attention_device": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp], c_int),
+        "va_kv_cache_write_device": ([_vp, ctypes.POINTER(VaKvCache), i64, _vp, _vp, _vp, _vp, _vp], c_int),
+        "va_kv_cache_read_device": ([_vp, ctypes.POINTER(VaKvCache), i64, _vp, _vp, _vp, _vp, _vp], c_int),
+        "va_cache_attention_device": ([_vp, ctypes.POINTER(VaKvCache), ctypes.POINTER(VaAttnTerms), i64, _vp, _vp,
+                                       c_int, _vp, _vp, _vp, _vp, _vp], c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -213,6 +253,41 @@ def _ptr(x):
 
 def _f32(a):
     return None if a is None else np.ascontiguousarray(a, dtype=np.float32)
+
+
+_HEADS_DTYPES = {"torch.bfloat16": VA_BF16, "torch.float16": VA_F16, "torch.float32": VA_F32}
+
+
+def _on_device(x, device, what):
+    d = getattr(x, "device", None)
+    if d is None or d.type != "cuda" or d.index != device:
+        raise VestraError(VA_ERR_INVALID, f"{what} must be a tensor on CUDA device {device}")
+
+
+def _heads(x, device, what, channels=None):
+    """va_heads of a [rows, heads, channels] torch tensor; any token and head strides."""
+    _on_device(x, device, what)
+    if x.dim() != 3 or str(x.dtype) not in _HEADS_DTYPES or (channels is not None and x.shape[2] != channels):
+        raise VestraError(VA_ERR_INVALID, f"{what} must be [rows, heads, {channels or 'channels'}] bf16, f16 or f32")
+    rows, heads, d = x.shape
+    ts, hs, cs = x.stride()
+    if cs != 1:
+        raise VestraError(VA_ERR_INVALID, f"{what} needs contiguous channels")
+    if heads == 1:
+        hs = d
+    if rows <= 1:  # never stepped over
+        ts = heads * max(hs, d) if hs >= 0 else 0
+    return VaHeads(x.data_ptr(), ts, hs, heads, _HEADS_DTYPES[str(x.dtype)])
+
+
+def _device_array(x, device, what, dtype, count):
+    """Address of a contiguous device tensor of one dtype and element count (None passes)."""
+    if x is None:
+        return None
+    _on_device(x, device, what)
+    if str(x.dtype) != dtype or not x.is_contiguous() or x.numel() != count:
+        raise VestraError(VA_ERR_INVALID, f"{what} must be a contiguous {dtype} tensor of {count} elements")
+    return x.data_ptr()
 
 
 def default_config(**overrides) -> VaConfig:
@@ -270,6 +345,7 @@ class Context:
     def __init__(self, cfg: VaConfig, device: int = 0):
         self.lib = load_library()
         self.cfg = cfg
+        self.device = device
         h = _vp()
         rc = self.lib.va_create(ctypes.byref(cfg), device, ctypes.byref(h))
         if rc != VA_OK:
@@ -460,6 +536,66 @@ class Context:
                                                    _ptr(qb), _ptr(kg), _ptr(kb), qk_norm_eps, _ptr(pos), freq,
                                                    _ptr(out), stream))
 
+    def rope_axes(self, rope: "RopeAxes", positions, q, q_out, k=None, k_out=None, stream=0):
+        """Rotates q (and k) [rows, heads, head_dim] by positions int32 [rows, axes] (device);
+        an output may be its input."""
+        rows, d = q.shape[0], q.shape[-1]
+        t = [None if x is None else _heads(x, self.device, name, d)
+             for x, name in ((q, "q"), (q_out, "q_out"), (k, "k"), (k_out, "k_out"))]
+        for x in (q_out, k, k_out):
+            if x is not None and x.shape[0] != rows:
+                raise VestraError(VA_ERR_INVALID, "q, k and their outputs must have the same rows")
+        pos = _device_array(positions, self.device, "positions", "torch.int32", rows * rope.c.axes)
+        self.check(self.lib.va_rope_axes_device(self.h, ctypes.byref(rope.c), rows, d, pos, *map(_byref, t), stream))
+
+    def masked_attention(self, plan: "AttentionPlan", q, k, v, out, stream=0):
+        """out = attention of the plan's documents: q, out [rows, heads, 64], k, v [rows,
+        kv_heads, 64], bf16 or f16 on the device.  Rows of no document are left alone."""
+        t = [_heads(x, self.device, name, 64) for x, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out"))]
+        if min(q.shape[0], out.shape[0]) < plan.q_rows or min(k.shape[0], v.shape[0]) < plan.k_rows:
+            raise VestraError(VA_ERR_INVALID, "the plan's documents reach past the tensors' rows")
+        if not plan.h:
+            raise VestraError(VA_ERR_STATE, "the attention plan is closed")
+        self.check(self.lib.va_masked_attention_device(self.h, plan.h, *map(_byref, t), stream))
+
+    def kv_cache_write(self, cache: "KvCache", k, v, offsets, lens, stream=0):
+        """Appends rows offsets[b]..offsets[b+1] of k and v [rows, kv_heads, 64] as the last of
+        document b's lens[b] tokens (offsets int32 [documents + 1], lens int32 [documents], device)."""
+        self._cache_rows(self.lib.va_kv_cache_write_device, cache, k, v, offsets, lens, "lens", stream)
+
+    def kv_cache_read(self, cache: "KvCache", offsets, k_out, v_out, first=None, stream=0):
+        """Rows offsets[b]..offsets[b+1] of the outputs receive document b's tokens from
+        first[b] (default 0) on; other rows are left alone."""
+        self._cache_rows(self.lib.va_kv_cache_read_device, cache, k_out, v_out, offsets, first, "first", stream)
+
+    def _cache_rows(self, fn, cache, k, v, offsets, edge, name, stream):
+        cache.check_device(self.device)
+        kh, vh = _heads(k, self.device, "k", 64), _heads(v, self.device, "v", 64)
+        if k.shape[0] != v.shape[0]:
+            raise VestraError(VA_ERR_INVALID, "k and v must have the same rows")
+        n = cache.c.documents
+        self.check(fn(self.h, ctypes.byref(cache.c), k.shape[0],
+                      _device_array(offsets, self.device, "offsets", "torch.int32", n + 1),
+                      _device_array(edge, self.device, name, "torch.int32", n), _byref(kh), _byref(vh), stream))
+
+    def cache_attention(self, cache: "KvCache", q, out, offsets, lens, max_tokens, causal=True, frame=1, prefix=None,
+                        slopes=None, score_cap=0.0, scale=0.0, stream=0):
+        """Attention of the last offsets[b+1] - offsets[b] of document b's lens[b] tokens over
+        the cache: q, out [rows, heads, 64]; offsets, lens, prefix int32 and slopes f32 on the
+        device, read when the kernel runs."""
+        cache.check_device(self.device)
+        qh, oh = _heads(q, self.device, "q", 64), _heads(out, self.device, "out", 64)
+        if q.shape != out.shape:
+            raise VestraError(VA_ERR_INVALID, "q and out must have the same shape")
+        n, heads = cache.c.documents, q.shape[1]
+        terms = VaAttnTerms(heads, cache.c.kv_heads, int(bool(causal)), frame, scale, score_cap)
+        self.check(self.lib.va_cache_attention_device(
+            self.h, ctypes.byref(cache.c), ctypes.byref(terms), q.shape[0],
+            _device_array(offsets, self.device, "offsets", "torch.int32", n + 1),
+            _device_array(lens, self.device, "lens", "torch.int32", n), max_tokens,
+            _device_array(prefix, self.device, "prefix", "torch.int32", n),
+            _device_array(slopes, self.device, "slopes", "torch.float32", heads), _byref(qh), _byref(oh), stream))
+
     def check_device(self):
         self.check(self.lib.va_check_device(self.h))
 
@@ -537,6 +673,95 @@ class Context:
 
     def last_error(self) -> str:
         return self.lib.va_last_error(self.h).decode()
+
+
+def _byref(x):
+    return None if x is None else ctypes.byref(x)
+
+
+class RopeAxes:
+    """va_rope_axes: channels turned by each position axis (for example (16, 24, 24) for
+    time, height, width), frequency base, layout "per_axis" or "shared", pairing 0 (i, i + half)
+    or 1 (2i, 2i + 1)."""
+
+    def __init__(self, sections, base=100.0, layout="per_axis", pairing=0):
+        sections = [int(s) for s in sections]
+        if not 1 <= len(sections) <= 4 or layout not in ROPE_LAYOUTS:
+            raise VestraError(VA_ERR_INVALID, "rope needs 1 to 4 sections and layout 'per_axis' or 'shared'")
+        self.c = VaRopeAxes(len(sections), (ctypes.c_int32 * 4)(*sections), ROPE_LAYOUTS[layout], pairing, base)
+
+
+def _plan_arrays(q_offsets, k_offsets, prefix):
+    qo = np.ascontiguousarray(q_offsets, dtype=np.int64)
+    ko = np.ascontiguousarray(k_offsets, dtype=np.int64)
+    pre = None if prefix is None else np.ascontiguousarray(prefix, dtype=np.int64)
+    if qo.ndim != 1 or ko.shape != qo.shape or qo.size < 2 or (pre is not None and pre.shape != (qo.size - 1,)):
+        raise VestraError(VA_ERR_INVALID, "offsets need documents + 1 entries each, prefix one per document")
+    return qo, ko, pre
+
+
+class AttentionPlan:
+    """va_attn_plan: the documents of one masked-attention layout (host offsets) on the
+    context's device; serves any number of calls.  Keeps the context alive."""
+
+    def __init__(self, ctx: "Context", heads, kv_heads, q_offsets, k_offsets, causal=False, frame=1, prefix=None,
+                 slopes=None, score_cap=0.0, scale=0.0):
+        self.h = None
+        self.ctx = ctx
+        qo, ko, pre = _plan_arrays(q_offsets, k_offsets, prefix)
+        sl = _f32(slopes)
+        if sl is not None and sl.shape != (heads,):
+            raise VestraError(VA_ERR_INVALID, "slopes need one entry per head")
+        self.q_rows, self.k_rows = int(qo[-1]), int(ko[-1])
+        terms = VaAttnTerms(heads, kv_heads, int(bool(causal)), frame, scale, score_cap)
+        h = _vp()
+        ctx.check(ctx.lib.va_attn_plan_create(ctx.h, ctypes.byref(terms), qo.size - 1, _ptr(qo), _ptr(ko), _ptr(pre),
+                                              _ptr(sl), ctypes.byref(h)))
+        self.h = h
+
+    def close(self):
+        if self.h:
+            self.ctx.lib.va_attn_plan_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def attention_plan_shape(heads, kv_heads, q_offsets, k_offsets, causal=False, frame=1, prefix=None, sms=148) -> dict:
+    """The launch an AttentionPlan of this layout makes (va_attn_plan_shape; needs no GPU)."""
+    qo, ko, pre = _plan_arrays(q_offsets, k_offsets, prefix)
+    terms = VaAttnTerms(heads, kv_heads, int(bool(causal)), frame, 0.0, 0.0)
+    out = (ctypes.c_int64 * 5)()
+    rc = load_library().va_attn_plan_shape(ctypes.byref(terms), qo.size - 1, _ptr(qo), _ptr(ko), _ptr(pre), sms, out)
+    if rc != VA_OK:
+        raise VestraError(rc, "va_attn_plan_shape rejected the layout")
+    return dict(zip(("tiles", "splits", "tile_tokens", "key_tiles", "ctas"), out))
+
+
+class KvCache:
+    """va_kv_cache over caller-owned torch tensors: codes [documents, kv_heads, capacity, 64]
+    (int8 or float8_e4m3fn decides the format), scales f32 [documents, kv_heads, capacity]."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales):
+        fmt = {"torch.int8": KV_INT8, "torch.float8_e4m3fn": KV_E4M3}.get(str(k_codes.dtype))
+        if fmt is None or k_codes.dim() != 4 or k_codes.shape[3] != 64:
+            raise VestraError(VA_ERR_INVALID, "codes must be [documents, kv_heads, capacity, 64] int8 or float8_e4m3fn")
+        docs, heads, capacity, _ = k_codes.shape
+        for x, shape, dtype in ((k_codes, k_codes.shape, k_codes.dtype), (v_codes, k_codes.shape, k_codes.dtype),
+                                (k_scales, k_codes.shape[:3], None), (v_scales, k_codes.shape[:3], None)):
+            if tuple(x.shape) != tuple(shape) or not x.is_contiguous() or x.device != k_codes.device or \
+                    (x.dtype != dtype if dtype is not None else str(x.dtype) != "torch.float32"):
+                raise VestraError(VA_ERR_INVALID, "cache codes and scales must be contiguous, of matching shapes, "
+                                                  "scales float32, on one device")
+        self.tensors = (k_codes, v_codes, k_scales, v_scales)  # kept alive
+        self.c = VaKvCache(docs, heads, capacity, fmt, 0, *[x.data_ptr() for x in self.tensors])
+
+    def check_device(self, device):
+        _on_device(self.tensors[0], device, "the cache")
 
 
 class _FromGguf:
