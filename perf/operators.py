@@ -306,8 +306,11 @@ def _pairs(sections, layout, pairing):
 def _run_rope(st):
     case = st["case"]
     if own:
-        st["ctx"].rope_axes(st["rope"], st["positions"], st["q"], st["q_out"], st["k"], st["k_out"], stream=_stream())
-        return st["q_out"], st["k_out"]
+        # F32 operands turn in place, as in the plain form (where .float() is no copy).
+        in_place = case["dtype"] == "f32"
+        q_out, k_out = (st["q"], st["k"]) if in_place else (st["q_out"], st["k_out"])
+        st["ctx"].rope_axes(st["rope"], st["positions"], st["q"], q_out, st["k"], k_out, stream=_stream())
+        return q_out, k_out
     first, second, axis, power = _pairs(_ints(case["sections"]), case["layout"], case["pairing"])
     freq = torch.tensor([case["base"] ** -p for p in power], device="cuda", dtype=torch.float64)
     angle = st["positions"].double()[:, axis] * freq  # far positions: 64 bits
