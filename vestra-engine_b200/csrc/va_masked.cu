@@ -9,13 +9,16 @@
 //
 // CTA = one tile of 128 query rows of one key head: tile_tokens tokens x the `group` query
 // heads that share the key head (one 3-D TMA box), so shared key heads read K and V once
-// and a single token still fills as many rows as it has heads.  8 warps, two CTAs per SM
+// and a single token still fills as many rows as it has heads.  10 warps, two CTAs per SM
 // (TMEM 256 columns and at most 100 KB of shared memory each), so that one CTA's
 // exponentials cover the other's waits:
 //   warp 0    TMA producer: Q, then K_j (3 stages) and V_j (2 stages)
 //   warp 1    TMEM owner and UMMA issuer; in a document's last tile it first zeroes the V rows
 //             past the document (a masked probability is 0, but 0 x NaN is not)
-//   warps 4-7 softmax, one query row per thread
+//   warps 2-9 softmax: two warps share a TMEM lane quadrant (16-lane loads), four threads a
+//             row, 32 columns of two rows per thread, so that 16 warps per SM overlap their
+//             loads, maxima and MUFU work (one row per thread on four warps spilled and ran at
+//             half the rate)
 // TMEM: S [0, 128) F32, P [128, 192) packed 16-bit pairs, O [192, 256) F32.  The chain per
 // key tile is QK(j+2) | softmax(j) | PV(j) as in the layer path's one-tile kernel.
 //
@@ -28,6 +31,7 @@
 
 #include "va_internal.h"
 #include "va_ptx.cuh"
+#include "va_tmem16.cuh"
 
 namespace va {
 
@@ -35,7 +39,9 @@ namespace {
 
 constexpr int kTile = 128;
 constexpr int kHeadDim = 64;
-constexpr int kThreads = 256;
+constexpr int kThreads = 320;
+constexpr int kFirstSoftmaxWarp = 2;
+constexpr int kSoftmaxThreads = 256;
 constexpr int kKStages = 3;
 constexpr int kVStages = 2;
 constexpr uint32_t kTileBytes = kTile * kHeadDim * 2;
@@ -241,17 +247,74 @@ __device__ __forceinline__ void run_mma(const Ctl& c, const Geom& g, uint32_t tm
   __syncwarp();
 }
 
-__device__ __forceinline__ void store_row16(uint8_t* dst, const float* o, float inv, bool f16) {
-  uint4* d = reinterpret_cast<uint4*>(dst);
+// Maxima of the thread's two rows over its 32 columns each (3-input maxima, two chains a row).
+__device__ __forceinline__ void row_maxima(const float* s, float* mx) {
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    uint32_t w[4];
+  for (int i = 0; i < 2; ++i) {
+    const float* v = s + 2 * i;  // pairs v[4k], v[4k + 1]
+    float a = max3f(v[0], v[1], v[4]), b = max3f(v[5], v[8], v[9]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float lo = o[8 * c + 2 * i] * inv, hi = o[8 * c + 2 * i + 1] * inv;
-      w[i] = f16 ? f16x2_from_f32(lo, hi) : pack_bf16x2(lo, hi);
+    for (int k = 3; k < 15; k += 2) {
+      a = max3f(a, v[4 * k], v[4 * k + 1]);
+      b = max3f(b, v[4 * k + 4], v[4 * k + 5]);
     }
-    d[c] = make_uint4(w[0], w[1], w[2], w[3]);
+    mx[i] = max3f(a, b, fmaxf(v[60], v[61]));
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16x2_of(uint64_t p) {
+  float lo, hi;
+  f32x2_unpack(p, lo, hi);
+  return pack_bf16x2(lo, hi);
+}
+
+// (lo, hi) F32 in [0, 65488) -> f16x2, round half up.  cvt.rn.f16x2.f32 runs on the MUFU's pipe at a
+// quarter of its rate (measured: that pipe 90 % busy, 289 us for four packed documents against
+// 82 GFLOP); this runs on the FMA and integer pipes: times 2^-112 the F32 bits hold
+// the f16 exponent (subnormals included) and mantissa in bits 13..28; 8 u + 2^15 brings
+// them to the upper half, rounded.
+__device__ __forceinline__ uint32_t pack_f16x2_bits(uint64_t p) {
+  const float k = 1.925929944387236e-34f;  // 2^-112
+  float lo, hi;
+  f32x2_unpack(f32x2_mul(p, f32x2_pack(k, k)), lo, hi);
+  const uint32_t a = __float_as_uint(lo) * 8u + 0x8000u, b = __float_as_uint(hi) * 8u + 0x8000u;
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// s <- cap log2(e) tanh(scale s / cap).  While every |s| of the warp's part of the tile is at most
+// cap_range (a score of 0.6 cap, at most 77) by an odd polynomial on the FMA pipe: tanh(z) =
+// z P(z^2), P cubic, fitted here (reweighted least squares on Chebyshev nodes of z^2 in [0, 0.36],
+// relative error below 2.2e-6, so a capped score is within 1.7e-4).  Else, and where hidden keys
+// may hold anything, cap log2(e) (1 - 2 / (1 + e^(2z))): two MUFU operations a score.
+__device__ __forceinline__ void cap_scores(float* s, const AttnTerms& t, bool partial) {
+  bool wide = partial;
+  if (!partial) {
+    float mx[2], mn[2] = {s[0], s[2]};
+    row_maxima(s, mx);
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) asm("min.f32 %0, %0, %1, %2;" : "+f"(mn[i]) : "f"(s[4 * k + 2 * i]), "f"(s[4 * k + 2 * i + 1]));
+    // a NaN fails no comparison: the polynomial hands it on as well
+    wide = fmaxf(fmaxf(mx[0], mx[1]), -fminf(mn[0], mn[1])) > t.cap_range;
+  }
+  if (__any_sync(0xffffffffu, wide)) {
+#pragma unroll
+    for (int q = 0; q < 64; ++q) s[q] = t.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(s[q] * t.cap_in)));
+  } else {
+    const uint64_t k0 = f32x2_pack(t.cap_poly[0], t.cap_poly[0]), k1 = f32x2_pack(t.cap_poly[1], t.cap_poly[1]);
+    const uint64_t k2 = f32x2_pack(t.cap_poly[2], t.cap_poly[2]), k3 = f32x2_pack(t.cap_poly[3], t.cap_poly[3]);
+#pragma unroll
+    for (int q = 0; q < 32; ++q) {
+      const uint64_t v = f32x2_pack(s[2 * q], s[2 * q + 1]);
+      const uint64_t u = f32x2_mul(v, v);
+      uint64_t p = f32x2_fma(k3, u, k2);
+      p = f32x2_fma(p, u, k1);
+      p = f32x2_fma(p, u, k0);
+      f32x2_unpack(f32x2_mul(p, v), s[2 * q], s[2 * q + 1]);
+    }
   }
 }
 
@@ -284,8 +347,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(c.v_empty(s), 1);
     }
     mbar_init(c.s_full(), 1);
-    mbar_init(c.s_free(), 128);
-    mbar_init(c.p_full(), 128);
+    mbar_init(c.s_free(), kSoftmaxThreads);
+    mbar_init(c.p_full(), kSoftmaxThreads);
     mbar_init(c.pv_done(), 1);
     mbar_init(c.o_final(), 1);
     for (int i = 1; i < 7; ++i) *c.misc(i) = 0;
@@ -306,11 +369,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem = *c.tmem_slot();
   volatile int* abort_flag = c.abort_flag();
 
-  if (warp < 4) {
+  if (warp < kFirstSoftmaxWarp) {
     if (warp == 0) {
       if (lane == 0) run_producer(c, g, a, &map_q, &map_k, &map_v, err);
       __syncwarp();
-    } else if (warp == 1) {
+    } else {
       run_mma<kF16>(c, g, tmem, err);
     }
     if (a.splits > 1) {
@@ -319,28 +382,36 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else {
     const int quad = warp & 3;
-    const int r = quad * 32 + lane;  // row of the tile
-    const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
+    const int lane_base = quad * 32 + ((warp - kFirstSoftmaxWarp) >> 2) * 16;
+    const uint32_t lane_off = static_cast<uint32_t>(lane_base) << 16;
     const uint32_t tS = tmem + lane_off + kColS, tP = tmem + lane_off + kColP, tO = tmem + lane_off + kColO;
-    const int tok = r / a.group;
-    const int head = g.kvh * a.group + (r - tok * a.group);
-    const bool live = r < g.rows;
-    const bool warp_live = quad * 32 < g.rows;
-    const int pos = g.it.first + tok;  // key position of the row
-    // floor(pos / frame), also below zero
-    const int frame = pos >= 0 ? pos / a.t.frame : -1 - (-1 - pos) / a.t.frame;
-    int limit = g.it.doc_keys;
-    if (a.t.causal) {
-      const int64_t e = (static_cast<int64_t>(frame) + 1) * a.t.frame;
-      limit = static_cast<int>(max(static_cast<int64_t>(0),
-                                   min(static_cast<int64_t>(limit), max(e, static_cast<int64_t>(g.it.prefix)))));
+    const int c0 = 2 * (lane & 3);  // first of the thread's column pair in every 8 columns
+    const bool warp_live = lane_base < g.rows;
+    // The thread's two rows of the tile.
+    int limit[2], row[2];
+    float slope[2], fpos[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      row[i] = lane_base + (lane >> 2) + 8 * i;
+      const int tok = row[i] / a.group;
+      const int head = g.kvh * a.group + (row[i] - tok * a.group);
+      const bool live = row[i] < g.rows;
+      const int pos = g.it.first + tok;  // key position of the row
+      // floor(pos / frame), also below zero
+      const int frame = pos >= 0 ? pos / a.t.frame : -1 - (-1 - pos) / a.t.frame;
+      limit[i] = g.it.doc_keys;
+      if (a.t.causal) {
+        const int64_t e = (static_cast<int64_t>(frame) + 1) * a.t.frame;
+        limit[i] = static_cast<int>(max(static_cast<int64_t>(0),
+                                        min(static_cast<int64_t>(limit[i]), max(e, static_cast<int64_t>(g.it.prefix)))));
+      }
+      if (!live) limit[i] = 0;
+      slope[i] = kBias ? a.slopes[live ? head : 0] : 0.0f;
+      fpos[i] = static_cast<float>(frame);
     }
-    if (!live) limit = 0;
-    const float slope = kBias ? a.slopes[live ? head : 0] : 0.0f;
-    const float fpos = static_cast<float>(frame);
     const float sl2 = a.t.scale_log2;
-    float m = -INFINITY;  // running maximum, log2 domain, may lag by kGrow
-    float l = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY};  // running maxima, log2 domain, may lag by kGrow
+    float l[2] = {0.0f, 0.0f};            // partial sums over the thread's columns
     bool ok = true;
     for (int j = 0; j < g.n; ++j) {
       ok = mbar_wait(c.s_full(), j & 1, abort_flag, err, kDevTimeoutConsumer);
@@ -359,67 +430,74 @@ __global__ void __launch_bounds__(kThreads, 2)
         continue;
       }
       tc_fence_after();
-      float s[128];
-#pragma unroll
-      for (int q = 0; q < 128; q += 32) tmem_ld32(tS + q, s + q);
+      float s[64];  // block k: s[4k], s[4k+1] row 0, columns 8k + c0, +1; s[4k+2], s[4k+3] row 1
+      tmem_ld_16x256b_x16(tS, s);
       tc_fence_before();
       mbar_arrive(c.s_free());  // QK of the next tile may overwrite S
       const int k0 = (g.t0 + j) * kTile;
-      const int lim = limit - k0;
-      if constexpr (kCap) {
-        // cap log2(e) tanh(z) = cap log2(e) (1 - 2 / (1 + e^(2z)))
-#pragma unroll
-        for (int q = 0; q < 128; ++q)
-          s[q] = a.t.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(s[q] * a.t.cap_in)));
-      }
+      const bool partial = __any_sync(0xffffffffu, min(limit[0], limit[1]) < k0 + kTile);
+      if constexpr (kCap) cap_scores(s, a.t, partial);
       if constexpr (kBias) {
-        const float4* ft = reinterpret_cast<const float4*>(a.frame_of + k0);
+        const float2* ft = reinterpret_cast<const float2*>(a.frame_of + k0 + c0);
+        const uint64_t fp0 = f32x2_pack(-fpos[0], -fpos[0]), fp1 = f32x2_pack(-fpos[1], -fpos[1]);
+        const uint64_t ns0 = f32x2_pack(-slope[0], -slope[0]), ns1 = f32x2_pack(-slope[1], -slope[1]);
+        const uint64_t sc2 = f32x2_pack(sl2, sl2);
 #pragma unroll
-        for (int q = 0; q < 32; ++q) {
-          const float4 f = __ldg(ft + q);
-          const float w[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[4 * q + e] = fmaf(-slope, fabsf(fpos - w[e]), kCap ? s[4 * q + e] : s[4 * q + e] * sl2);
+        for (int k = 0; k < 16; ++k) {
+          const float2 f = __ldg(ft + 4 * k);
+          const uint64_t ff = f32x2_pack(f.x, f.y);
+          const uint64_t d0 = f32x2_add(ff, fp0) & 0x7fffffff7fffffffull, d1 = f32x2_add(ff, fp1) & 0x7fffffff7fffffffull;
+          uint64_t v0 = f32x2_pack(s[4 * k], s[4 * k + 1]), v1 = f32x2_pack(s[4 * k + 2], s[4 * k + 3]);
+          if (!kCap) v0 = f32x2_mul(v0, sc2), v1 = f32x2_mul(v1, sc2);
+          f32x2_unpack(f32x2_fma(d0, ns0, v0), s[4 * k], s[4 * k + 1]);
+          f32x2_unpack(f32x2_fma(d1, ns1, v1), s[4 * k + 2], s[4 * k + 3]);
         }
       }
       constexpr bool kScaled = kCap || kBias;  // s already in the log2 domain
-      if (__any_sync(0xffffffffu, lim < kTile)) {
+      if (partial) {
+        const int lim0 = limit[0] - k0 - c0, lim1 = limit[1] - k0 - c0;
 #pragma unroll
-        for (int q = 0; q < 128; ++q)
-          if (q >= lim) s[q] = -INFINITY;
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (8 * k + e >= lim0) s[4 * k + e] = -INFINITY;
+            if (8 * k + e >= lim1) s[4 * k + 2 + e] = -INFINITY;
+          }
       }
-      // Row maximum as a tree of 3-input maxima.
-      float mx8[8];
+      float mx[2];
+      row_maxima(s, mx);
+      bool grow[2];
+      float alpha[2];
+      uint64_t neg2[2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx8[i] = max3f(s[i], s[8 + i], s[16 + i]);
-#pragma unroll
-      for (int q = 24; q < 120; q += 16)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mx8[i] = max3f(mx8[i], s[q + i], s[q + 8 + i]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx8[i] = fmaxf(mx8[i], s[120 + i]);
-      float mx = max3f(max3f(mx8[0], mx8[1], mx8[2]), max3f(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
-      if (!kScaled) mx *= sl2;
-      const bool grow = mx > m + kGrow;  // m = -inf: as soon as a key is seen
-      const float m_new = grow ? mx : m;
-      const float alpha = grow ? ex2(m - m_new) : 1.0f;
-      const float neg = m_new == -INFINITY ? 0.0f : kOffset - m_new;  // no key yet: every x is -inf
-      const uint64_t sc2 = f32x2_pack(sl2, sl2), neg2 = f32x2_pack(neg, neg);
-      uint32_t pk[64];
-      uint64_t acc[4];
-#pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        const uint64_t v = f32x2_pack(s[2 * i], s[2 * i + 1]);
-        float x0, x1;
-        f32x2_unpack(kScaled ? f32x2_add(v, neg2) : f32x2_fma(v, sc2, neg2), x0, x1);
-        const float p0 = ex2(x0), p1 = ex2(x1);
-        const uint64_t pp = f32x2_pack(p0, p1);
-        acc[i & 3] = i < 4 ? pp : f32x2_add(acc[i & 3], pp);
-        pk[i] = kF16 ? f16x2_from_f32(p0, p1) : pack_bf16x2(p0, p1);
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        if (!kScaled) mx[i] *= sl2;
+        grow[i] = mx[i] > m[i] + kGrow;  // m = -inf: as soon as a key is seen
+        alpha[i] = 1.0f;
+        if (grow[i]) {
+          alpha[i] = ex2(m[i] - mx[i]);
+          m[i] = mx[i];
+        }
+        const float neg = m[i] == -INFINITY ? 0.0f : kOffset - m[i];  // no key yet: every x is -inf
+        neg2[i] = f32x2_pack(neg, neg);
       }
-      float s0, s1;
-      f32x2_unpack(f32x2_add(f32x2_add(acc[0], acc[1]), f32x2_add(acc[2], acc[3])), s0, s1);
+      const uint64_t sc2 = f32x2_pack(sl2, sl2);
+      uint32_t pk[32];  // 16x128b order: block k: (row 0 pair k), (row 1 pair k)
+      uint64_t acc[2];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint64_t v = f32x2_pack(s[4 * k + 2 * i], s[4 * k + 2 * i + 1]);
+          float x0, x1;
+          f32x2_unpack(kScaled ? f32x2_add(v, neg2[i]) : f32x2_fma(v, sc2, neg2[i]), x0, x1);
+          const uint64_t pp = f32x2_pack(ex2(x0), ex2(x1));
+          acc[i] = k == 0 ? pp : f32x2_add(acc[i], pp);
+          pk[2 * k + i] = kF16 ? pack_f16x2_bits(pp) : pack_bf16x2_of(pp);
+        }
+      }
       if (j > 0) {
         // PV(j-1) has finished reading P and adding into O.
         ok = mbar_wait(c.pv_done(), (j - 1) & 1, abort_flag, err, kDevTimeoutConsumer);
@@ -427,19 +505,24 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (!ok) break;
         tc_fence_after();
       }
-      tmem_st64(tP, pk);
-      if (j > 0 && __any_sync(0xffffffffu, grow)) {
-        float o[64];
-        tmem_ld32(tO, o);
-        tmem_ld32(tO + 32, o + 32);
-        uint32_t u[64];
+      tmem_st_16x128b_x16(tP, pk);
+      if (j > 0 && __any_sync(0xffffffffu, grow[0] || grow[1])) {
+        float o[32];  // block k: o[4k], o[4k+1] row 0; o[4k+2], o[4k+3] row 1
+        tmem_ld_16x256b_x8(tO, o);
+        uint32_t w[32];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) u[i] = __float_as_uint(o[i] * alpha);
-        tmem_st64(tO, u);
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[4 * k + e] = __float_as_uint(o[4 * k + e] * alpha[e >> 1]);
+        tmem_st_16x256b_x8(tO, w);
       }
       tmem_wait_st();
-      l = l * alpha + (s0 + s1);
-      m = m_new;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float u0, u1;
+        f32x2_unpack(acc[i], u0, u1);
+        l[i] = l[i] * alpha[i] + (u0 + u1);
+      }
       tc_fence_before();
       mbar_arrive(c.p_full());
     }
@@ -447,69 +530,74 @@ __global__ void __launch_bounds__(kThreads, 2)
       ok = mbar_wait(c.o_final(), 0, abort_flag, err, kDevTimeoutConsumer);
       ok = __all_sync(0xffffffffu, ok);
     }
-    const bool f16 = kF16;
+    float o[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+    if (ok && warp_live && g.n > 0) {
+      tc_fence_after();
+      tmem_ld_16x256b_x8(tO, o);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
     uint8_t* out = static_cast<uint8_t*>(a.out.data);
     if (a.splits == 1) {
-      if (ok && warp_live) {
-        float o[64];
-        if (g.n > 0) {
-          tc_fence_after();
-          tmem_ld32(tO, o);
-          tmem_ld32(tO + 32, o + 32);
-        }
-        if (l == 0.0f) {  // no key seen
 #pragma unroll
-          for (int i = 0; i < 64; ++i) o[i] = 0.0f;
+      for (int i = 0; i < 2; ++i) {
+        if (!ok || row[i] >= g.rows) continue;
+        const int tok = row[i] / a.group, head = g.kvh * a.group + (row[i] - tok * a.group);
+        uint8_t* dst = out + 2 * ((g.it.q_row + static_cast<int64_t>(tok)) * a.out.token_stride + head * a.out.head_stride + c0);
+        const float inv = 1.0f / l[i];
+        const bool none = l[i] == 0.0f;  // no key seen
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float x0 = none ? 0.0f : o[4 * k + 2 * i] * inv, x1 = none ? 0.0f : o[4 * k + 2 * i + 1] * inv;
+          *reinterpret_cast<uint32_t*>(dst + 16 * k) = kF16 ? f16x2_from_f32(x0, x1) : pack_bf16x2(x0, x1);
         }
-        if (live)
-          store_row16(out + 2 * ((g.it.q_row + static_cast<int64_t>(tok)) * a.out.token_stride + head * a.out.head_stride),
-                      o, l == 0.0f ? 0.0f : 1.0f / l, f16);
       }
     } else {
       if (warp_live) {
-        float o[64];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) o[i] = 0.0f;
-        if (ok && g.n > 0) {
-          tc_fence_after();
-          tmem_ld32(tO, o);
-          tmem_ld32(tO + 32, o + 32);
+        for (int i = 0; i < 2; ++i) {
+          const int r = row[i];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            // channels 8k + c0, +1: half of 16-byte chunk 2k + c0 / 4
+            const uint32_t at = Smem::kPart + r * 256 + (((2 * k + (c0 >> 2)) ^ (r & 15)) << 4) + 4 * (c0 & 2);
+            *reinterpret_cast<float2*>(c.smem + at) = make_float2(o[4 * k + 2 * i], o[4 * k + 2 * i + 1]);
+          }
+          if ((lane & 3) == 0) {
+            c.ml()[2 * r] = m[i];
+            c.ml()[2 * r + 1] = l[i];
+          }
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          st_shared_v4(c.base + Smem::kPart + r * 256 + ((i ^ (r & 15)) << 4),
-                       make_uint4(__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]),
-                                  __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3])));
-        c.ml()[2 * r] = m;
-        c.ml()[2 * r + 1] = l;
       }
       __syncwarp();
       cluster_sync();
       // Rank q joins rows [q rows / splits, (q + 1) rows / splits): 16 threads a row.
       const int r0 = g.rank * g.rows / a.splits, r1 = (g.rank + 1) * g.rows / a.splits;
       const uint32_t part = c.base + Smem::kPart, ml = c.base + Smem::kMl;
-      for (int i = static_cast<int>(threadIdx.x) - 128; i < (r1 - r0) * 16; i += 128) {
-        const int row = r0 + (i >> 4), ch = i & 15;
+      for (int i = static_cast<int>(threadIdx.x) - 32 * kFirstSoftmaxWarp; i < (r1 - r0) * 16; i += kSoftmaxThreads) {
+        const int r = r0 + (i >> 4), ch = i & 15;
         float mt = -INFINITY;
-        for (int p = 0; p < a.splits; ++p) mt = fmaxf(mt, ld_cluster_v2(cluster_addr(ml + row * 8, p)).x);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < a.splits; ++p) mt = fmaxf(mt, ld_cluster_v2(cluster_addr(ml + r * 8, p)).x);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         float lt = 0.0f;
         for (int p = 0; p < a.splits; ++p) {
-          const float2 q = ld_cluster_v2(cluster_addr(ml + row * 8, p));
+          const float2 q = ld_cluster_v2(cluster_addr(ml + r * 8, p));
           const float f = q.x == -INFINITY ? 0.0f : ex2(q.x - mt);
-          const float4 v = ld_cluster_v4(cluster_addr(part + row * 256 + ((ch ^ (row & 15)) << 4), p));
-          o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+          const float4 v = ld_cluster_v4(cluster_addr(part + r * 256 + ((ch ^ (r & 15)) << 4), p));
+          sum.x += f * v.x, sum.y += f * v.y, sum.z += f * v.z, sum.w += f * v.w;
           lt += f * q.y;
         }
-        const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-        if (lt == 0.0f) o = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int t = row / a.group, h = g.kvh * a.group + (row - t * a.group);
-        uint2 w;
-        if (f16) {
-          w = make_uint2(f16x2_from_f32(o.x * inv, o.y * inv), f16x2_from_f32(o.z * inv, o.w * inv));
-        } else {
-          w = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-        }
+        const float inv = 1.0f / lt;
+        if (lt == 0.0f) sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        else sum.x *= inv, sum.y *= inv, sum.z *= inv, sum.w *= inv;
+        const int t = r / a.group, h = g.kvh * a.group + (r - t * a.group);
+        const uint2 w = kF16 ? make_uint2(f16x2_from_f32(sum.x, sum.y), f16x2_from_f32(sum.z, sum.w))
+                             : make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
         if (ok)
           *reinterpret_cast<uint2*>(
               out + 2 * ((g.it.q_row + static_cast<int64_t>(t)) * a.out.token_stride + h * a.out.head_stride + 4 * ch)) = w;
