@@ -9,24 +9,25 @@
 // query row.  A row block is 8 query rows of one key head (tokens x the heads that share
 // it), so the products are m16n8k16 tensor-core instructions (mma.sync: the tcgen05 tile
 // of 128 rows would be 94 % padding, and the operands come from registers): rows 0..7
-// hold the high bf16 part of the row, rows 8..15 the rest, which makes the product of an
-// f16 row, and of the F32 probabilities, good to 2^-16 at no further instruction.
+// hold the high f16 part of the row, rows 8..15 the rest, which makes the products good to
+// 2^-21 of the row's largest element at no further product.  f16 because both code formats
+// become f16 in one or two instructions a pair (bf16 took four or five, and the conversions
+// are most of the loop).  Its range is met by powers of two: a query row is scaled to a
+// largest magnitude in [1, 2) and the factor goes to the scores; a probability times its
+// value scale is scaled by 2^(kTop - E), E above the largest value scale so far.
 //
 // A cluster of CTAs shares one (document, key head, row block); its warps take 32-key
-// chunks in turn straight from global memory into registers (one chunk ahead), each warp
-// with its own running maximum and sum, and the partial results meet in shared memory
+// chunks in turn through a ring of its own in shared memory (cp.async, two chunks ahead), each
+// warp with its own running maximum and sum, and the partial results meet in shared memory
 // and then, through distributed shared memory, across the cluster in rank order: one
 // launch, no workspace, no atomics, and the same bits on every run.
 //
 // Operand layout: the channel order inside a product is free as long as both operands
 // use the same, so lane (g, c) = (lane / 4, lane % 4) loads 16 consecutive code bytes
-// [16c, 16c + 16) of key g of an 8-key tile (one 512-byte warp load), and its word s
-// holds the lane's k indices of step s; the query row is loaded with the same
-// order.  For the second product the key order is free: lane (g, c) loads channels [8g, 8g + 8)
+// [16c, 16c + 16) of one key of an 8-key tile, and its word s holds the lane's k indices of
+// step s; the query row is loaded with the same order.  For the second product the key order is free: lane (g, c) loads channels [8g, 8g + 8)
 // of the four keys whose probabilities it holds.
 #include <algorithm>
-
-#include <cooperative_groups.h>
 
 #include "va_internal.h"
 #include "va_ptx.cuh"
@@ -40,8 +41,11 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRowsPerBlock = 8;
 constexpr int kChunk = 32;         // keys a warp takes at a time
+constexpr int kStages = 3;         // chunks of a warp in shared memory
 constexpr int kMaxCluster = 16;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTop = 14;       // probabilities times value scales are brought below 2^kTop
+constexpr int kMinExp = -100;  // value scales below 2^-100 lose precision
 
 struct CacheAttnArgs {
   KvCacheRef c;
@@ -63,9 +67,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -77,31 +81,28 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return r;
 }
 
-// Two code bytes of w -> bf16x2, exactly.  kHigh: bytes 2 and 3, else 0 and 1.
-// int8 c: with the byte under 0x43, 0x4300 | (c & 0x7f) is the bf16 128 + (c & 127) and
-//   0x4300 | (c & 0x80) is 128 or, for a negative code, 256: their difference is c.
-// e4m3 s.eeee.mmm: moved under bf16's exponent the bits read as the value times 2^-120
-//   (subnormals included), undone by an exact multiplication.  The NaN code reads as 480.
+// Two code bytes of w -> f16x2, exactly.  kHigh: bytes 2 and 3, else 0 and 1.  int8 codes come
+// with their sign bits flipped (flip): u = c + 128 under 0x64 is the f16 1024 + u.
+template <bool kE4m3>
+__device__ __forceinline__ uint32_t flip(uint32_t w) { return kE4m3 ? w : w ^ 0x80808080u; }
 template <bool kE4m3, bool kHigh>
-__device__ __forceinline__ uint32_t codes_to_bf16x2(uint32_t w) {
+__device__ __forceinline__ uint32_t codes_to_f16x2(uint32_t w) {
+  uint32_t r;
   if constexpr (kE4m3) {
-    const uint32_t t = prmt(w, 0u, kHigh ? 0x3424u : 0x1404u);  // bytes: 0, c0, 0, c1
-    const uint32_t u = ((t >> 4) & 0x07f007f0u) | (t & 0x80008000u);
-    uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x7b807b80u));  // 2^120
-    return r;
+    const uint16_t h = static_cast<uint16_t>(kHigh ? w >> 16 : w);
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(h));
   } else {
-    const uint32_t t = prmt(w, 0x43434343u, kHigh ? 0x4342u : 0x4140u);  // bytes: c0, 43, c1, 43
-    uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t & 0xff7fff7fu), "r"(t & 0xff80ff80u));
-    return r;
+    const uint32_t t = prmt(w, 0x64646464u, kHigh ? 0x4342u : 0x4140u);  // bytes: u0, 64, u1, 64
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0x64806480u));  // - (1024 + 128)
   }
+  return r;
 }
 
-// x in two bf16 parts, packed with a neighbour's: hi = bf16(x), lo = bf16(x - hi).
+// x in two f16 parts, packed with a neighbour's: hi = f16(x), lo = f16(x - hi).
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  hi = pack_bf16x2(x0, x1);
-  lo = pack_bf16x2(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+  hi = f16x2_from_f32(x0, x1);
+  const float2 h = __half22float2(*reinterpret_cast<__half2*>(&hi));
+  lo = f16x2_from_f32(x0 - h.x, x1 - h.y);
 }
 
 // floor(p / frame), magic = floor(2^32 / frame).
@@ -113,58 +114,111 @@ __device__ __forceinline__ int frame_index(int p, int frame, uint32_t magic) {
   return p < 0 ? -1 - static_cast<int>(q) : static_cast<int>(q);
 }
 
-// One 32-key chunk in registers: lane (g, c) holds key 8t + g's bytes [16c, 16c + 16) for
-// t = 0..3, and of each 16-key half u the value bytes [8g, 8g + 8) of keys 16u + {2c,
-// 2c + 1, 8 + 2c, 9 + 2c}; scales of the keys whose scores it will hold.
+// A warp's ring of 32-key chunks in shared memory, filled by cp.async (16 bytes of codes, 4 of
+// scales a copy: no alignment beyond the cache's own).  Code rows of 64 bytes; the
+// 16-byte piece p of row r lies at piece p ^ (2 bit2(r)).  Column n of an 8-key tile is key n ^ bit1(n):
+// with that order a warp's 16-byte key loads and 8-byte value loads meet no bank twice.
 struct Chunk {
-  uint4 k[4];
-  uint2 v[2][4];
-  float ks[4][2], vs[4][2];
+  uint8_t k[kChunk][kHeadDim];
+  uint8_t v[kChunk][kHeadDim];
+  float ks[kChunk], vs[kChunk];
 };
+__device__ __forceinline__ int tile_key(int n) { return n ^ ((n >> 1) & 1); }
 
+__device__ __forceinline__ void cp16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Rows past `last` repeat it (they are hidden, and the codes of any row are finite).
 __device__ __forceinline__ void load_chunk(Chunk& ch, const uint8_t* kc, const uint8_t* vc, const float* ks,
-                                           const float* vs, int key0, int last, int g, int c) {
+                                           const float* vs, int key0, int last, int lane) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int64_t key = min(key0 + 8 * t + g, last);
-    ch.k[t] = __ldcs(reinterpret_cast<const uint4*>(kc + key * kHeadDim + 16 * c));
-    const int64_t j0 = min(key0 + 8 * t + 2 * c, last), j1 = min(key0 + 8 * t + 2 * c + 1, last);
-    ch.ks[t][0] = __ldg(ks + j0), ch.ks[t][1] = __ldg(ks + j1);
-    ch.vs[t][0] = __ldg(vs + j0), ch.vs[t][1] = __ldg(vs + j1);
-    ch.v[t >> 1][2 * (t & 1)] = __ldcs(reinterpret_cast<const uint2*>(vc + j0 * kHeadDim + 8 * g));
-    ch.v[t >> 1][2 * (t & 1) + 1] = __ldcs(reinterpret_cast<const uint2*>(vc + j1 * kHeadDim + 8 * g));
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2), p = lane & 3;
+    const int64_t at = static_cast<int64_t>(min(key0 + r, last)) * kHeadDim + 16 * p;
+    const int q = 16 * (p ^ ((r >> 1) & 2));
+    cp16(&ch.k[r][q], kc + at);
+    cp16(&ch.v[r][q], vc + at);
+  }
+  const int64_t key = min(key0 + lane, last);
+  cp4(&ch.ks[lane], ks + key);
+  cp4(&ch.vs[lane], vs + key);
+}
+
+// The warps' results of a row block.  Channel ch of a row lies at slot(ch): the order in which
+// a lane's accumulators are neighbours; rows are padded against bank conflicts.
+__device__ __forceinline__ int slot(int ch) { return (ch & 7) * 8 + (ch >> 3); }
+struct Join {
+  float o[kWarps][kRowsPerBlock][kHeadDim + 8];
+  float m[kWarps][kRowsPerBlock], l[kWarps][kRowsPerBlock];
+};
+// What the cluster's CTAs send to the CTA that finishes a row: rows r, r + splits, ... go to
+// CTA r % splits, so a CTA receives at most 16 (splits x rows) parts.
+struct Part {
+  float o[kHeadDim];
+  float m, l;
+};
+struct Shared {
+  union {
+    Chunk ring[kWarps][kStages];
+    Join join;  // once the block's last chunk is used
+  };
+  Part part[kMaxCluster];  // [own row][cluster rank]
+};
+static_assert(2 * (sizeof(Shared) + 1024) <= 228 * 1024, "two CTAs per SM");
+
+// Stores v at this address of CTA `rank` of the cluster.
+__device__ __forceinline__ void st_cluster(float* p, int rank, float v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// 16 consecutive elements (two 16-byte loads).
+__device__ __forceinline__ void load16(const __nv_bfloat16* p, float* x) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint4 u = reinterpret_cast<const uint4*>(p)[h];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[8 * h + 2 * i] = __uint_as_float(w[i] << 16);
+      x[8 * h + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
   }
 }
-
-struct Shared {
-  float o[kWarps][kRowsPerBlock][kHeadDim];
-  float m[kWarps][kRowsPerBlock], l[kWarps][kRowsPerBlock];
-  // the CTA's result, read by the cluster
-  float co[kRowsPerBlock][kHeadDim];
-  float cm[kRowsPerBlock], cl[kRowsPerBlock];
-};
-
-__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
-  uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void load16(const __half* p, float* x) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint4 u = reinterpret_cast<const uint4*>(p)[h];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[8 * h + 2 * i] = f.x;
+      x[8 * h + 2 * i + 1] = f.y;
+    }
+  }
 }
-
-template <class T>
-__device__ __forceinline__ float elem(const T* p);
-template <>
-__device__ __forceinline__ float elem(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-template <>
-__device__ __forceinline__ float elem(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x); }
 
 template <class T, bool kE4m3>
 __global__ void __launch_bounds__(kThreads, 2)
     cache_attn_kernel(const __grid_constant__ CacheAttnArgs a, int splits, int* err) {
-  __shared__ Shared sh;
+  extern __shared__ uint4 smem_raw[];
+  Shared& smem = *reinterpret_cast<Shared*>(smem_raw);
+  Join& sh = smem.join;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int rank = static_cast<int>(blockIdx.x) % splits;
@@ -205,6 +259,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   };
 
   for (int rb = block0; rb * kRowsPerBlock < q_rows; rb += a.row_blocks) {
+    // Every CTA of the cluster has started, and is done with the parts of the last block.
+    if (splits > 1) cluster_arrive();
     const int r = rb * kRowsPerBlock + g;  // this lane's query row
     const bool valid = r < q_rows;
     const int token = valid ? r / a.group : tokens - 1;
@@ -216,17 +272,30 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     // Query row in fragment order: word s of the lane's 16 channels [16c, 16c + 16).
     uint32_t qa[4][4];
+    float q_scale;
     {
       const T* p = qd + (begin + static_cast<int64_t>(token)) * a.q.token_stride + head * a.q.head_stride + 16 * c;
+      float x[16];
+      load16(p, x);
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (!valid) x[e] = 0.0f;
+        top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t ex = min(max(top >> 23, 2u), 252u);  // a non-finite row stays non-finite
+      q_scale = __uint_as_float(ex << 23);
+      const float inv = __uint_as_float((254u - ex) << 23);
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = valid ? elem(p + 4 * s + e) : 0.0f;
-        split2(x[0], x[1], qa[s][0], qa[s][1]);
-        split2(x[2], x[3], qa[s][2], qa[s][3]);
+        split2(x[4 * s] * inv, x[4 * s + 1] * inv, qa[s][0], qa[s][1]);
+        split2(x[4 * s + 2] * inv, x[4 * s + 3] * inv, qa[s][2], qa[s][3]);
       }
     }
+    const float score_scale = q_scale * a.t.scale_log2, cap_scale = q_scale * a.t.cap_in;
+    int v_exp = kMinExp;  // E: every visible value scale so far is below 2^E
 
     float o[8][4];
 #pragma unroll
@@ -237,36 +306,53 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     const int chunks = (block_limit + kChunk - 1) / kChunk;
     const int stride = splits * kWarps;
-    int ch = rank * kWarps + warp;
-    Chunk cur;
-    if (ch < chunks) load_chunk(cur, kc, vc, ks, vs, ch * kChunk, len - 1, g, c);
-    for (; ch < chunks; ch += stride) {
+    const int first = rank * kWarps + warp;
+    Chunk* ring = smem.ring[warp];
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (first + i * stride < chunks) load_chunk(ring[i], kc, vc, ks, vs, (first + i * stride) * kChunk, len - 1, lane);
+      cp_commit();
+    }
+    int stage = 0;
+    for (int ch = first; ch < chunks; ch += stride) {
+      cp_wait<kStages - 2>();
+      __syncwarp();  // every lane's copies have landed, and the stage below is read out
+      {
+        const int next = ch + (kStages - 1) * stride;
+        const int to = stage == 0 ? kStages - 1 : stage - 1;
+        if (next < chunks) load_chunk(ring[to], kc, vc, ks, vs, next * kChunk, len - 1, lane);
+        cp_commit();
+      }
+      const Chunk& cur = ring[stage];
+      stage = stage + 1 == kStages ? 0 : stage + 1;
       const int key0 = ch * kChunk;
-      // Scores of 8 rows x 32 keys: lane (g, c) gets row g, keys 8t + 2c and 8t + 2c + 1.
+      // Scores of 8 rows x 32 keys: lane (g, c) gets row g, columns 2c and 2c + 1 of each tile.
       float x[4][2];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         float d[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t w[4] = {cur.k[t].x, cur.k[t].y, cur.k[t].z, cur.k[t].w};
+        const int kr = 8 * t + tile_key(g);
+        const uint4 kw = *reinterpret_cast<const uint4*>(&cur.k[kr][16 * (c ^ ((kr >> 1) & 2))]);
+        const uint32_t w[4] = {flip<kE4m3>(kw.x), flip<kE4m3>(kw.y), flip<kE4m3>(kw.z), flip<kE4m3>(kw.w)};
 #pragma unroll
         for (int s = 0; s < 4; ++s)
-          mma_bf16(d, qa[s], codes_to_bf16x2<kE4m3, false>(w[s]), codes_to_bf16x2<kE4m3, true>(w[s]));
+          mma_f16(d, qa[s], codes_to_f16x2<kE4m3, false>(w[s]), codes_to_f16x2<kE4m3, true>(w[s]));
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float dot = (d[e] + d[2 + e]) * cur.ks[t][e];
+          const int kk = 8 * t + ((2 * c + e) ^ (c & 1));
+          const float dot = (d[e] + d[2 + e]) * cur.ks[kk];
           float y;
           if (a.t.cap_out > 0.0f) {
             // cap log2(e) tanh(z) = cap log2(e) (1 - 2 / (1 + e^(2z)))
-            y = a.t.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(dot * a.t.cap_in)));
+            y = a.t.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(dot * cap_scale)));
           } else {
-            y = dot * a.t.scale_log2;
+            y = dot * score_scale;
           }
-          const int key = key0 + 8 * t + 2 * c + e;
           if (a.slopes) {
-            const int dist = fp - frame_index(key, a.t.frame, a.frame_magic);
+            const int dist = fp - frame_index(key0 + kk, a.t.frame, a.frame_magic);
             y -= slope * static_cast<float>(abs(dist));
           }
-          x[t][e] = key < limit ? y : -INFINITY;
+          x[t][e] = key0 + kk < limit ? y : -INFINITY;
         }
       }
       float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])),
@@ -274,9 +360,16 @@ __global__ void __launch_bounds__(kThreads, 2)
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const float m_new = fmaxf(m, top);
-      if (__any_sync(0xffffffffu, m_new > m)) {
-        const float alpha = m_new > m ? ex2(m - m_new) : 1.0f;  // 0 for the first keys
+      // The largest value scale of the keys some row sees (NaN and infinity set no scale; they
+      // reach the rows that see them on their own).
+      const uint32_t vbits = __float_as_uint(cur.vs[lane]);
+      const uint32_t vtop = __reduce_max_sync(0xffffffffu, key0 + lane < block_limit && vbits < 0x7f800000u ? vbits : 0u);
+      const int e_new = max(v_exp, static_cast<int>(vtop >> 23) - 126);
+      if (__any_sync(0xffffffffu, m_new > m) || e_new > v_exp) {
+        float alpha = m_new > m ? ex2(m - m_new) : 1.0f;  // 0 for the first keys
         l *= alpha;
+        alpha *= __uint_as_float(static_cast<uint32_t>(max(v_exp - e_new, -126) + 127) << 23);
+        v_exp = e_new;
         // Accumulator rows g (elements 0, 1) and g + 8 (2, 3) are parts of query row g.
 #pragma unroll
         for (int n = 0; n < 8; ++n)
@@ -285,53 +378,63 @@ __global__ void __launch_bounds__(kThreads, 2)
         m = m_new;
       }
       const float base = m == -INFINITY ? 0.0f : m;
+      const float v_scale = __uint_as_float(static_cast<uint32_t>(kTop - v_exp + 127) << 23);  // 2^(kTop - E)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t pa[4];
+        uint2 vw[4];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int t = 2 * u + half;
           float w[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
+            const int kk = 8 * t + ((2 * c + e) ^ (c & 1));
+            vw[2 * half + e] = *reinterpret_cast<const uint2*>(&cur.v[kk][(8 * g) ^ ((kk << 3) & 32)]);
             const float p = ex2(x[t][e] - base);
             l += p;
             // A hidden key's value scale may be anything (stale rows): not multiplied.
-            w[e] = x[t][e] == -INFINITY ? 0.0f : p * cur.vs[t][e];
+            w[e] = x[t][e] == -INFINITY ? 0.0f : p * (cur.vs[kk] * v_scale);
           }
           split2(w[0], w[1], pa[2 * half], pa[2 * half + 1]);
         }
 #pragma unroll
         for (int word = 0; word < 2; ++word) {
-          // Four channels of keys (2c, 2c + 1) and (8 + 2c, 9 + 2c), interleaved in pairs.
-          const uint32_t a0 = word ? cur.v[u][0].y : cur.v[u][0].x, a1 = word ? cur.v[u][1].y : cur.v[u][1].x;
-          const uint32_t b0 = word ? cur.v[u][2].y : cur.v[u][2].x, b1 = word ? cur.v[u][3].y : cur.v[u][3].x;
+          // Four channels of two keys each, interleaved in pairs.
+          const uint32_t a0 = flip<kE4m3>(word ? vw[0].y : vw[0].x), a1 = flip<kE4m3>(word ? vw[1].y : vw[1].x);
+          const uint32_t b0 = flip<kE4m3>(word ? vw[2].y : vw[2].x), b1 = flip<kE4m3>(word ? vw[3].y : vw[3].x);
           const uint32_t lo0 = prmt(a0, a1, 0x5140), hi0 = prmt(a0, a1, 0x7362);
           const uint32_t lo1 = prmt(b0, b1, 0x5140), hi1 = prmt(b0, b1, 0x7362);
-          mma_bf16(o[4 * word + 0], pa, codes_to_bf16x2<kE4m3, false>(lo0), codes_to_bf16x2<kE4m3, false>(lo1));
-          mma_bf16(o[4 * word + 1], pa, codes_to_bf16x2<kE4m3, true>(lo0), codes_to_bf16x2<kE4m3, true>(lo1));
-          mma_bf16(o[4 * word + 2], pa, codes_to_bf16x2<kE4m3, false>(hi0), codes_to_bf16x2<kE4m3, false>(hi1));
-          mma_bf16(o[4 * word + 3], pa, codes_to_bf16x2<kE4m3, true>(hi0), codes_to_bf16x2<kE4m3, true>(hi1));
+          mma_f16(o[4 * word + 0], pa, codes_to_f16x2<kE4m3, false>(lo0), codes_to_f16x2<kE4m3, false>(lo1));
+          mma_f16(o[4 * word + 1], pa, codes_to_f16x2<kE4m3, true>(lo0), codes_to_f16x2<kE4m3, true>(lo1));
+          mma_f16(o[4 * word + 2], pa, codes_to_f16x2<kE4m3, false>(hi0), codes_to_f16x2<kE4m3, false>(hi1));
+          mma_f16(o[4 * word + 3], pa, codes_to_f16x2<kE4m3, true>(hi0), codes_to_f16x2<kE4m3, true>(hi1));
         }
       }
-      if (ch + stride < chunks) load_chunk(cur, kc, vc, ks, vs, (ch + stride) * kChunk, len - 1, g, c);
     }
+    cp_wait<0>();
+    __syncthreads();  // every warp is done with its ring: the join buffers may cover it
     // Row sums over the four lanes of a row; accumulator column 2c + e of tile n is
     // channel 8 (2c + e) + n (the value operand's column g holds channel 8g + n).
+    const int rows = min(kRowsPerBlock, q_rows - rb * kRowsPerBlock);
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (g < rows) {
+      const float back = __uint_as_float(static_cast<uint32_t>(v_exp - kTop + 127) << 23);  // 2^(E - kTop)
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) sh.o[warp][g][8 * (2 * c + e) + n] = o[n][e] + o[n][2 + e];
-    if (c == 0) {
-      sh.m[warp][g] = m;
-      sh.l[warp][g] = l;
+      for (int n = 0; n < 8; ++n)
+        *reinterpret_cast<float2*>(&sh.o[warp][g][8 * n + 2 * c]) =
+            make_float2((o[n][0] + o[n][2]) * back, (o[n][1] + o[n][3]) * back);
+      if (c == 0) {
+        sh.m[warp][g] = m;
+        sh.l[warp][g] = l;
+      }
     }
     __syncthreads();
-    // Join the warps: 512 outputs over 256 threads.
-    for (int i = threadIdx.x; i < kRowsPerBlock * kHeadDim; i += kThreads) {
-      const int row = i / kHeadDim, col = i % kHeadDim;
+    if (splits > 1) cluster_wait();
+    // Join the warps and hand each row to the CTA that finishes it.
+    for (int i = threadIdx.x; i < rows * kHeadDim; i += kThreads) {
+      const int row = i / kHeadDim, at = i % kHeadDim;
       float mt = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, sh.m[w][row]);
@@ -339,62 +442,56 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = sh.m[w][row] == -INFINITY ? 0.0f : ex2(sh.m[w][row] - mt);
-        os += f * sh.o[w][row][col];
+        os += f * sh.o[w][row][at];
         ls += f * sh.l[w][row];
       }
-      sh.co[row][col] = os;
-      if (col == 0) {
-        sh.cm[row] = mt;
-        sh.cl[row] = ls;
+      const int owner = row % splits;
+      Part& to = smem.part[row / splits * splits + rank];
+      st_cluster(&to.o[at], owner, os);
+      if (at == 0) {
+        st_cluster(&to.m, owner, mt);
+        st_cluster(&to.l, owner, ls);
       }
     }
     if (splits > 1) {
-      cooperative_groups::this_cluster().sync();
+      cluster_arrive();
+      cluster_wait();
     } else {
       __syncthreads();
     }
-    // Join the cluster: CTA `rank` writes outputs rank, rank + splits, ... in blocks of 64
-    // divided evenly.
-    for (int i = rank * kThreads + threadIdx.x; i < kRowsPerBlock * kHeadDim; i += splits * kThreads) {
-      const int row = i / kHeadDim, col = i % kHeadDim;
-      const int rr = rb * kRowsPerBlock + row;
-      if (rr >= q_rows) continue;
+    // This CTA's rows rank, rank + splits, ...: the cluster's parts in rank order.
+    for (int i = threadIdx.x; rank + i / kHeadDim * splits < rows; i += kThreads) {
+      const int own = i / kHeadDim, ch = i % kHeadDim;
+      const Part* part = smem.part + own * splits;
       float mt = -INFINITY, os = 0.0f, ls = 0.0f;
-      if (splits > 1) {
-        for (int p = 0; p < splits; ++p) mt = fmaxf(mt, ld_cluster(&sh.cm[row], p));
-        for (int p = 0; p < splits; ++p) {
-          const float mp = ld_cluster(&sh.cm[row], p);
-          const float f = mp == -INFINITY ? 0.0f : ex2(mp - mt);
-          os += f * ld_cluster(&sh.co[row][col], p);
-          ls += f * ld_cluster(&sh.cl[row], p);
-        }
-      } else {
-        os = sh.co[row][col];
-        ls = sh.cl[row];
+      for (int p = 0; p < splits; ++p) mt = fmaxf(mt, part[p].m);
+      for (int p = 0; p < splits; ++p) {
+        const float f = part[p].m == -INFINITY ? 0.0f : ex2(part[p].m - mt);
+        os += f * part[p].o[slot(ch)];
+        ls += f * part[p].l;
       }
+      const int rr = rb * kRowsPerBlock + rank + own * splits;
       put(od + (begin + static_cast<int64_t>(rr / a.group)) * a.out.token_stride +
-              static_cast<int64_t>(kvh * a.group + rr % a.group) * a.out.head_stride + col,
+              static_cast<int64_t>(kvh * a.group + rr % a.group) * a.out.head_stride + ch,
           ls == 0.0f ? 0.0f : os / ls);
     }
-    // The next row block, or the exit, must not overwrite what a peer still reads.
-    if (splits > 1) {
-      cooperative_groups::this_cluster().sync();
-    } else {
-      __syncthreads();
-    }
+    __syncthreads();  // before the next block's loads and parts
   }
 }
 
 template <class T, bool kE4m3>
 cudaError_t launch(const CacheAttnArgs& a, int splits, int64_t blocks, int* err, cudaStream_t st) {
   auto kern = cache_attn_kernel<T, kE4m3>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+  if (e != cudaSuccess) return e;
   if (splits > 8) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -427,10 +524,12 @@ cudaError_t launch_cache_attention(const KvCacheRef& c, const AttnTerms& t, int 
   a.q = q;
   a.out = out;
   const int64_t units = static_cast<int64_t>(c.documents) * c.kv_heads * a.row_blocks;
-  // CTAs per unit: enough for two per SM, at least four chunks per warp of the capacity.
-  const int64_t most = std::max<int64_t>(1, c.capacity / (4 * kChunk * kWarps));
+  // CTAs per unit: the lengths are on the device, so by the capacity: enough for kTarget CTAs per
+  // SM (documents differ in length), at least two chunks per warp.
+  static const int kTarget = getenv("VAT") ? atoi(getenv("VAT")) : 4;
+  const int64_t most = std::max<int64_t>(1, c.capacity / (2 * kChunk * kWarps));
   int splits = 1;
-  while (splits < kMaxCluster && units * splits < 2 * sms && 2 * splits <= most) splits *= 2;
+  while (splits < kMaxCluster && units * splits < kTarget * sms && 2 * splits <= most) splits *= 2;
   const int64_t blocks = units * splits;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   if (c.e4m3)

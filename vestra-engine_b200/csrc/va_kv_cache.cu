@@ -135,7 +135,70 @@ struct KvArgs {
   HeadsRef x[2];        // k, v
 };
 
-// Work item of an eight-lane group: (tensor, head, row); rows fastest within a warp.
+// Codes and scale of one head's eight channels (the eight lanes of a group hold 64).
+template <bool kE4m3>
+__device__ __forceinline__ uint2 quantise(const float* v, uint32_t group_mask, float* scale_out) {
+  // The largest magnitude as an integer maximum of the bit patterns, which order like the
+  // values with infinities and NaN on top.
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(group_mask, top, o));
+  uint2 u = make_uint2(0u, 0u);
+  *scale_out = __uint_as_float(0x7fffffffu);  // NaN: a head with a non-finite value
+  if (top >= 0x7f800000u) return u;
+  if (kE4m3) {
+    // amax = f 2^e, 1 <= f < 2: 2^(e - 8), or 2^(e - 7) when f > 1.75.
+    const int e = static_cast<int>(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u);
+    const int ec = max(e, -126);
+    *scale_out = __uint_as_float(static_cast<uint32_t>(ec + 127) << 23);
+    const float inv = __uint_as_float(static_cast<uint32_t>(127 - ec) << 23);
+    u.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
+    u.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
+  } else {
+    const float scale = fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 1.17549435e-38f);
+    *scale_out = scale;
+    const float inv = __fdiv_rn(1.0f, scale);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u.x |= static_cast<uint32_t>(int8_code(v[i], scale, inv) & 255) << (8 * i);
+      u.y |= static_cast<uint32_t>(int8_code(v[4 + i], scale, inv) & 255) << (8 * i);
+    }
+  }
+  return u;
+}
+
+template <bool kE4m3>
+__device__ __forceinline__ void dequantise(uint2 u, float scale, float top, float* v) {
+  if (kE4m3) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = e4m3x2_to_f32((i < 2 ? u.x : u.y) >> (16 * (i & 1)));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = static_cast<float>(static_cast<int8_t>(u.x >> (8 * i)));
+      v[4 + i] = static_cast<float>(static_cast<int8_t>(u.y >> (8 * i)));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = v[i] * scale;
+    v[i] = y != y ? y : fminf(fmaxf(y, -top), top);  // fmin and fmax drop a NaN
+  }
+}
+
+// An eight-lane group takes one row and kHeads heads of K and of V: all its loads are
+// issued before the first is used.
+#ifndef KH
+#define KH 1
+#endif
+constexpr int kHeads = KH;
+
 template <class T, bool kE4m3, bool kWrite>
 __global__ void __launch_bounds__(kThreads) kv_rows_kernel(const __grid_constant__ KvArgs a, int* err) {
   const int heads = a.c.kv_heads;
@@ -151,6 +214,7 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(const __grid_constant
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 8) + (threadIdx.x >> 3);
   // The eight lanes of a group share the row; the group leaves together.
   if (row >= a.rows) return;
+  const int h0 = blockIdx.y * kHeads;
   const int doc = document_of(a.offsets, a.c.documents, static_cast<int>(row));
   if (doc < 0) return;
   const int32_t begin = __ldg(a.offsets + doc), end = __ldg(a.offsets + doc + 1);
@@ -158,73 +222,49 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(const __grid_constant
   const int64_t first = kWrite ? __ldg(a.edge + doc) - n : (a.edge ? __ldg(a.edge + doc) : 0);
   if (row < begin || row >= end || !document_ok(begin, end, first, a.rows, a.c.capacity)) return;
   const int64_t token = first + (row - begin);
+  const int64_t slot0 = (static_cast<int64_t>(doc) * heads + h0) * a.c.capacity + token;
   const uint32_t group_mask = 0xffu << (threadIdx.x & 24);
-  for (int w = 0; w < 2; ++w) {
-    const HeadsRef& x = a.x[w];
-    for (int h = blockIdx.y; h < heads; h += gridDim.y) {
-      const int64_t slot = (static_cast<int64_t>(doc) * heads + h) * a.c.capacity + token;
-      T* p = static_cast<T*>(x.data) + row * x.token_stride + h * x.head_stride + 8 * lane8;
-      uint8_t* codes = a.c.codes[w] + slot * kHeadDim + 8 * lane8;
-      if (kWrite) {
-        float v[8];
-        load8<T>(p, v);
-        // The largest magnitude as an integer maximum of the bit patterns, which order
-        // like the values with infinities and NaN on top.
-        uint32_t top = 0;
+  if (kWrite) {
+    float v[2][kHeads][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(group_mask, top, o));
-        uint2 u = make_uint2(0u, 0u);
-        float scale = __uint_as_float(0x7fffffffu);  // NaN: a head with a non-finite value
-        if (top < 0x7f800000u) {
-          if (kE4m3) {
-            // amax = f 2^e, 1 <= f < 2: 2^(e - 8), or 2^(e - 7) when f > 1.75.
-            const int e = static_cast<int>(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u);
-            const int ec = max(e, -126);
-            scale = __uint_as_float(static_cast<uint32_t>(ec + 127) << 23);
-            const float inv = __uint_as_float(static_cast<uint32_t>(127 - ec) << 23);
-            u.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
-            u.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
-          } else {
-            scale = fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 1.17549435e-38f);
-            const float inv = __fdiv_rn(1.0f, scale);
+      for (int i = 0; i < kHeads; ++i)
+        if (h0 + i < heads)
+          load8<T>(static_cast<const T*>(a.x[w].data) + row * a.x[w].token_stride + (h0 + i) * a.x[w].head_stride + 8 * lane8,
+                   v[w][i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              u.x |= static_cast<uint32_t>(int8_code(v[i], scale, inv) & 255) << (8 * i);
-              u.y |= static_cast<uint32_t>(int8_code(v[4 + i], scale, inv) & 255) << (8 * i);
-            }
-          }
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i)
+        if (h0 + i < heads) {
+          const int64_t slot = slot0 + i * a.c.capacity;
+          float scale;
+          const uint2 u = quantise<kE4m3>(v[w][i], group_mask, &scale);
+          *reinterpret_cast<uint2*>(a.c.codes[w] + slot * kHeadDim + 8 * lane8) = u;
+          if (lane8 == 0) a.c.scales[w][slot] = scale;
         }
-        *reinterpret_cast<uint2*>(codes) = u;
-        if (lane8 == 0) a.c.scales[w][slot] = scale;
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(codes);
-        const float scale = a.c.scales[w][slot];
-        float v[8];
-        if (kE4m3) {
+  } else {
+    uint2 u[2][kHeads];
+    float scale[2][kHeads];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = e4m3x2_to_f32((i < 2 ? u.x : u.y) >> (16 * (i & 1)));
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-          }
-        } else {
+    for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[i] = static_cast<float>(static_cast<int8_t>(u.x >> (8 * i)));
-            v[4 + i] = static_cast<float>(static_cast<int8_t>(u.y >> (8 * i)));
-          }
+      for (int i = 0; i < kHeads; ++i)
+        if (h0 + i < heads) {
+          const int64_t slot = slot0 + i * a.c.capacity;
+          u[w][i] = *reinterpret_cast<const uint2*>(a.c.codes[w] + slot * kHeadDim + 8 * lane8);
+          scale[w][i] = a.c.scales[w][slot];
         }
-        const float top = finite_max<T>();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = v[i] * scale;
-          v[i] = y != y ? y : fminf(fmaxf(y, -top), top);  // fmin and fmax drop a NaN
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i)
+        if (h0 + i < heads) {
+          float v[8];
+          dequantise<kE4m3>(u[w][i], scale[w][i], finite_max<T>(), v);
+          store8<T>(static_cast<T*>(a.x[w].data) + row * a.x[w].token_stride + (h0 + i) * a.x[w].head_stride + 8 * lane8, v);
         }
-        store8<T>(p, v);
-      }
-    }
   }
 }
 
@@ -232,7 +272,7 @@ template <class T, bool kWrite>
 cudaError_t launch_rows(const KvArgs& a, int* err, cudaStream_t st) {
   const int64_t bx = std::max<int64_t>(1, (a.rows + kThreads / 8 - 1) / (kThreads / 8));
   if (bx > 0x7fffffff) return cudaErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(a.c.kv_heads));
+  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>((a.c.kv_heads + kHeads - 1) / kHeads));
   if (a.c.e4m3)
     kv_rows_kernel<T, true, kWrite><<<grid, kThreads, 0, st>>>(a, err);
   else

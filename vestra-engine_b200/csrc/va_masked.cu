@@ -268,19 +268,10 @@ __device__ __forceinline__ uint32_t pack_bf16x2_of(uint64_t p) {
   return pack_bf16x2(lo, hi);
 }
 
-// (lo, hi) F32 in [0, 65488) -> f16x2, round half up.  cvt.rn.f16x2.f32 runs on the MUFU's pipe at a
-// quarter of its rate (measured: that pipe 90 % busy, 289 us for four packed documents against
-// 82 GFLOP); this runs on the FMA and integer pipes: times 2^-112 the F32 bits hold
-// the f16 exponent (subnormals included) and mantissa in bits 13..28; 8 u + 2^15 brings
-// them to the upper half, rounded.
-__device__ __forceinline__ uint32_t pack_f16x2_bits(uint64_t p) {
-  const float k = 1.925929944387236e-34f;  // 2^-112
+__device__ __forceinline__ uint32_t pack_f16x2_of(uint64_t p) {
   float lo, hi;
-  f32x2_unpack(f32x2_mul(p, f32x2_pack(k, k)), lo, hi);
-  const uint32_t a = __float_as_uint(lo) * 8u + 0x8000u, b = __float_as_uint(hi) * 8u + 0x8000u;
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
+  f32x2_unpack(p, lo, hi);
+  return f16x2_from_f32(lo, hi);
 }
 
 // s <- cap log2(e) tanh(scale s / cap).  While every |s| of the warp's part of the tile is at most
@@ -495,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           f32x2_unpack(kScaled ? f32x2_add(v, neg2[i]) : f32x2_fma(v, sc2, neg2[i]), x0, x1);
           const uint64_t pp = f32x2_pack(ex2(x0), ex2(x1));
           acc[i] = k == 0 ? pp : f32x2_add(acc[i], pp);
-          pk[2 * k + i] = kF16 ? pack_f16x2_bits(pp) : pack_bf16x2_of(pp);
+          pk[2 * k + i] = kF16 ? pack_f16x2_of(pp) : pack_bf16x2_of(pp);
         }
       }
       if (j > 0) {

@@ -3,11 +3,12 @@
 //   (x0, x1) -> (x0 cos a - x1 sin a, x1 cos a + x0 sin a),  a = position[axis] * freq
 //
 // One pass: every element is read once and written once, so the kernel is bound by HBM
-// (or, for a handful of tokens, by the launch).  A block takes kRows token rows.  It
-// first tabulates the rows' (cos, sin) per pair in shared memory, once for all heads of
-// q and k (a 32-pair row is shared by 12 + 12 heads, so the trigonometry is 4 % of the
-// pairs), then its threads walk (row, head, chunk) items: a chunk is V pairs, read and
-// written as one or two vectors of up to 16 bytes.
+// (or, for a handful of tokens, by the launch).  A thread owns one (head, chunk) of kRows
+// consecutive token rows, a chunk being V pairs held in one or two vectors of up to 16
+// bytes: it issues all its rows' loads, then the block tabulates the rows' (cos, sin) per
+// pair in shared memory, once for all heads of q and k (a 32-pair row is shared by 12 + 12
+// heads, so the trigonometry is 4 % of the pairs and hides behind the loads), then the
+// thread turns its chunks and writes them.  No index is divided inside the row loop.
 //
 // Angles: a position may be any int32 and the product with the frequency is needed
 // modulo one turn, which F32 loses beyond a few thousand turns.  The frequency in turns
@@ -21,9 +22,8 @@ namespace va {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kRows = 4;
-constexpr int kBatch = 4;  // items a thread has in flight
+constexpr int kMaxThreads = 256;
+constexpr int kRows = 8;
 
 template <class T>
 __device__ __forceinline__ float to_f32(T x);
@@ -60,89 +60,91 @@ __device__ __forceinline__ float2 turn_cos_sin(double t) {
 // V pairs per chunk; kInter: pairs are neighbours (2i, 2i+1), one vector of 2V elements;
 // otherwise two vectors of V elements, min_half a multiple of V.
 template <class T, int V, bool kInter>
-__global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a) {
+__global__ void __launch_bounds__(kMaxThreads) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a) {
   extern __shared__ float2 cs[];  // [kRows][pairs]
+  using Part = Vec<T, kInter ? 2 * V : V>;
+  constexpr int kVecs = kInter ? 1 : 2;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
   const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), a.rows - row0));
-  for (int i = threadIdx.x; i < rows * a.pairs; i += kThreads) {
+  const int chunks = a.pairs / V;
+  const int item = blockIdx.y * blockDim.x + threadIdx.x;
+  const bool active = item < (a.in[0].heads + a.in[1].heads) * chunks;
+  int h = active ? item / chunks : 0;
+  const int pair = active ? (item - h * chunks) * V : 0;
+  const int which = h >= a.in[0].heads;
+  if (which) h -= a.in[0].heads;
+  const int ch[2] = {a.first[pair], a.second[pair]};
+  Part x[kRows][kVecs];
+  if (active) {
+    const T* src = static_cast<const T*>(a.in[which].data) + row0 * a.in[which].token_stride + h * a.in[which].head_stride;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      if (r < rows) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+          x[r][i] = *reinterpret_cast<const Part*>(src + r * a.in[which].token_stride + ch[i]);
+      }
+  }
+  for (int i = threadIdx.x; i < rows * a.pairs; i += blockDim.x) {
     const int r = i / a.pairs, p = i - r * a.pairs;
     const int pos = __ldg(a.positions + (row0 + r) * a.axes + a.axis[p]);
     cs[i] = turn_cos_sin(static_cast<double>(pos) * a.turns[p]);
   }
   __syncthreads();
-
-  const int chunks = a.pairs / V;
-  const int heads = a.in[0].heads + a.in[1].heads;
-  const int items = rows * heads * chunks;
-  using Part = Vec<T, kInter ? 2 * V : V>;
-  for (int i0 = threadIdx.x; i0 < items; i0 += kThreads * kBatch) {
-    Part x0[kBatch], x1[kBatch];
-    T* dst[kBatch];
-    int pair[kBatch], row[kBatch];
+  if (active) {
+    T* dst = static_cast<T*>(a.out[which].data) + row0 * a.out[which].token_stride + h * a.out[which].head_stride;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * kThreads;
-      if (i < items) {
-        const int rh = i / chunks;
-        row[b] = rh / heads;
-        int h = rh - row[b] * heads;
-        pair[b] = (i - rh * chunks) * V;
-        const int which = h >= a.in[0].heads;
-        if (which) h -= a.in[0].heads;
-        const HeadsRef& in = a.in[which];
-        const HeadsRef& out = a.out[which];
-        const T* src = static_cast<const T*>(in.data) + (row0 + row[b]) * in.token_stride + h * in.head_stride;
-        dst[b] = static_cast<T*>(out.data) + (row0 + row[b]) * out.token_stride + h * out.head_stride;
-        x0[b] = *reinterpret_cast<const Part*>(src + a.first[pair[b]]);
-        if (!kInter) x1[b] = *reinterpret_cast<const Part*>(src + a.second[pair[b]]);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * kThreads;
-      if (i < items) {
-        const float2* t = cs + row[b] * a.pairs + pair[b];
+    for (int r = 0; r < kRows; ++r) {
+      if (r < rows) {
+        const float2* t = cs + r * a.pairs + pair;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float2 w = t[e];
-          T& lo = kInter ? x0[b].v[(2 * e) % (kInter ? 2 * V : V)] : x0[b].v[e % (kInter ? 2 * V : V)];
-          T& hi = kInter ? x0[b].v[(2 * e + 1) % (kInter ? 2 * V : V)] : x1[b].v[e % (kInter ? 2 * V : V)];
+          T& lo = x[r][0].v[kInter ? 2 * e : e];
+          T& hi = kInter ? x[r][0].v[2 * e + 1] : x[r][kVecs - 1].v[e];
           const float p0 = to_f32(lo), p1 = to_f32(hi);
           lo = from_f32<T>(p0 * w.x - p1 * w.y);
           hi = from_f32<T>(p1 * w.x + p0 * w.y);
         }
-        *reinterpret_cast<Part*>(dst[b] + a.first[pair[b]]) = x0[b];
-        if (!kInter) *reinterpret_cast<Part*>(dst[b] + a.second[pair[b]]) = x1[b];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+          *reinterpret_cast<Part*>(dst + r * a.out[which].token_stride + ch[i]) = x[r][i];
       }
     }
   }
 
   // Channels past the sections pass through (nothing to do in place).
   const int rest = a.head_dim - a.rotated;
-  if (rest == 0) return;
-  for (int i = threadIdx.x; i < rows * heads * rest; i += kThreads) {
+  if (rest == 0 || blockIdx.y != 0) return;
+  const int heads = a.in[0].heads + a.in[1].heads;
+  for (int i = threadIdx.x; i < rows * heads * rest; i += blockDim.x) {
     const int rh = i / rest, c = a.rotated + (i - rh * rest);
     const int r = rh / heads;
-    int h = rh - r * heads;
-    const int which = h >= a.in[0].heads;
-    if (which) h -= a.in[0].heads;
-    const HeadsRef& in = a.in[which];
-    const HeadsRef& out = a.out[which];
+    int hh = rh - r * heads;
+    const int w = hh >= a.in[0].heads;
+    if (w) hh -= a.in[0].heads;
+    const HeadsRef& in = a.in[w];
+    const HeadsRef& out = a.out[w];
     if (in.data == out.data) continue;
-    static_cast<T*>(out.data)[(row0 + r) * out.token_stride + h * out.head_stride + c] =
-        static_cast<const T*>(in.data)[(row0 + r) * in.token_stride + h * in.head_stride + c];
+    static_cast<T*>(out.data)[(row0 + r) * out.token_stride + hh * out.head_stride + c] =
+        static_cast<const T*>(in.data)[(row0 + r) * in.token_stride + hh * in.head_stride + c];
   }
 }
 
 template <class T, int V>
 cudaError_t launch_v(const RopeAxesArgs& a, cudaStream_t st) {
   const int64_t blocks = (a.rows + kRows - 1) / kRows;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  const int items = (a.in[0].heads + a.in[1].heads) * (a.pairs / V);
+  // As few threads past the items as the warp size allows.
+  const int parts = (items + kMaxThreads - 1) / kMaxThreads;
+  const int threads = ((items + parts - 1) / parts + 31) / 32 * 32;
+  if (blocks > 0x7fffffff || parts > 65535) return cudaErrorInvalidValue;
   const size_t smem = sizeof(float2) * kRows * a.pairs;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
   if (a.pairing)
-    rope_axes_kernel<T, V, true><<<static_cast<unsigned>(blocks), kThreads, smem, st>>>(a);
+    rope_axes_kernel<T, V, true><<<grid, threads, smem, st>>>(a);
   else
-    rope_axes_kernel<T, V, false><<<static_cast<unsigned>(blocks), kThreads, smem, st>>>(a);
+    rope_axes_kernel<T, V, false><<<grid, threads, smem, st>>>(a);
   return cudaGetLastError();
 }
 

@@ -255,38 +255,47 @@ def _f32(a):
     return None if a is None else np.ascontiguousarray(a, dtype=np.float32)
 
 
-_HEADS_DTYPES = {"torch.bfloat16": VA_BF16, "torch.float16": VA_F16, "torch.float32": VA_F32}
+_DTYPE_CODES = {}  # torch dtype -> VA_* of the streaming operators, filled on first use
 
 
-def _on_device(x, device, what):
-    d = getattr(x, "device", None)
-    if d is None or d.type != "cuda" or d.index != device:
-        raise VestraError(VA_ERR_INVALID, f"{what} must be a tensor on CUDA device {device}")
+def _dtype_code(dtype):
+    code = _DTYPE_CODES.get(dtype)
+    if code is None:
+        code = {"torch.bfloat16": VA_BF16, "torch.float16": VA_F16, "torch.float32": VA_F32}.get(str(dtype), -1)
+        _DTYPE_CODES[dtype] = code
+    return code
+
+
+def _refuse(msg):
+    raise VestraError(VA_ERR_INVALID, msg)
 
 
 def _heads(x, device, what, channels=None):
     """va_heads of a [rows, heads, channels] torch tensor; any token and head strides."""
-    _on_device(x, device, what)
-    if x.dim() != 3 or str(x.dtype) not in _HEADS_DTYPES or (channels is not None and x.shape[2] != channels):
-        raise VestraError(VA_ERR_INVALID, f"{what} must be [rows, heads, {channels or 'channels'}] bf16, f16 or f32")
-    rows, heads, d = x.shape
+    if not getattr(x, "is_cuda", False) or x.get_device() != device:
+        _refuse(f"{what} must be a tensor on CUDA device {device}")
+    shape, code = x.shape, _dtype_code(x.dtype)
+    if len(shape) != 3 or code < 0 or (channels is not None and shape[2] != channels):
+        _refuse(f"{what} must be [rows, heads, {channels or 'channels'}] bf16, f16 or f32")
+    rows, heads, d = shape
     ts, hs, cs = x.stride()
     if cs != 1:
-        raise VestraError(VA_ERR_INVALID, f"{what} needs contiguous channels")
+        _refuse(f"{what} needs contiguous channels")
     if heads == 1:
         hs = d
     if rows <= 1:  # never stepped over
-        ts = heads * max(hs, d) if hs >= 0 else 0
-    return VaHeads(x.data_ptr(), ts, hs, heads, _HEADS_DTYPES[str(x.dtype)])
+        ts = heads * max(hs, d)
+    return VaHeads(x.data_ptr(), ts, hs, heads, code)
 
 
 def _device_array(x, device, what, dtype, count):
     """Address of a contiguous device tensor of one dtype and element count (None passes)."""
     if x is None:
         return None
-    _on_device(x, device, what)
-    if str(x.dtype) != dtype or not x.is_contiguous() or x.numel() != count:
-        raise VestraError(VA_ERR_INVALID, f"{what} must be a contiguous {dtype} tensor of {count} elements")
+    if not getattr(x, "is_cuda", False) or x.get_device() != device:
+        _refuse(f"{what} must be a tensor on CUDA device {device}")
+    if not x.is_contiguous() or x.numel() != count or str(x.dtype) != dtype:
+        _refuse(f"{what} must be a contiguous {dtype} tensor of {count} elements")
     return x.data_ptr()
 
 
@@ -758,10 +767,12 @@ class KvCache:
                 raise VestraError(VA_ERR_INVALID, "cache codes and scales must be contiguous, of matching shapes, "
                                                   "scales float32, on one device")
         self.tensors = (k_codes, v_codes, k_scales, v_scales)  # kept alive
+        self.device = k_codes.get_device()
         self.c = VaKvCache(docs, heads, capacity, fmt, 0, *[x.data_ptr() for x in self.tensors])
 
     def check_device(self, device):
-        _on_device(self.tensors[0], device, "the cache")
+        if self.device != device:
+            _refuse(f"the cache must be on CUDA device {device}")
 
 
 class _FromGguf:
