@@ -92,7 +92,7 @@ def test_the_mirror_refuses_host_tensors():
     with pytest.raises(va.VestraError):
         va._heads(x, 0, "q", 64)
     with pytest.raises(va.VestraError):
-        va._device_array(torch.zeros(3, dtype=torch.int32), 0, "offsets", "torch.int32", 3)
+        va._device_array(torch.zeros(3, dtype=torch.int32), 0, "offsets", va._INT32, 3)
     with pytest.raises(va.VestraError):
         va.RopeAxes((16, 16, 16, 8, 8))
     codes, scales = torch.zeros(1, 2, 8, 64, dtype=torch.int8), torch.zeros(1, 2, 8)

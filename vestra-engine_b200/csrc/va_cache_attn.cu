@@ -28,6 +28,7 @@
 // step s; the query row is loaded with the same order.  For the second product the key order is free: lane (g, c) loads channels [8g, 8g + 8)
 // of the four keys whose probabilities it holds.
 #include <algorithm>
+#include <atomic>
 
 #include "va_internal.h"
 #include "va_ptx.cuh"
@@ -37,7 +38,10 @@ namespace va {
 namespace {
 
 constexpr int kHeadDim = 64;
-constexpr int kWarps = 8;
+#ifndef KW
+#define KW 8
+#endif
+constexpr int kWarps = KW;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRowsPerBlock = 8;
 constexpr int kChunk = 32;         // keys a warp takes at a time
@@ -67,8 +71,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -137,20 +147,31 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Rows past `last` repeat it (they are hidden, and the codes of any row are finite).
+// Rows past `last` repeat it (they are hidden, and the codes of any row held are finite).
 __device__ __forceinline__ void load_chunk(Chunk& ch, const uint8_t* kc, const uint8_t* vc, const float* ks,
                                            const float* vs, int key0, int last, int lane) {
+  const int row = lane >> 2, p = lane & 3;
+  uint8_t* to = &ch.k[row][16 * (p ^ ((row >> 1) & 2))];  // bit 2 of 8 i + row is that of row
+  if (key0 + kChunk - 1 <= last) {
+    const int64_t at = (static_cast<int64_t>(key0) + row) * kHeadDim + 16 * p;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + (lane >> 2), p = lane & 3;
-    const int64_t at = static_cast<int64_t>(min(key0 + r, last)) * kHeadDim + 16 * p;
-    const int q = 16 * (p ^ ((r >> 1) & 2));
-    cp16(&ch.k[r][q], kc + at);
-    cp16(&ch.v[r][q], vc + at);
+    for (int i = 0; i < 4; ++i) {
+      cp16(to + 8 * i * kHeadDim, kc + at + 8 * i * kHeadDim);
+      cp16(to + (kChunk + 8 * i) * kHeadDim, vc + at + 8 * i * kHeadDim);
+    }
+    cp4(&ch.ks[lane], ks + key0 + lane);
+    cp4(&ch.vs[lane], vs + key0 + lane);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = static_cast<int64_t>(min(key0 + 8 * i + row, last)) * kHeadDim + 16 * p;
+      cp16(to + 8 * i * kHeadDim, kc + at);
+      cp16(to + (kChunk + 8 * i) * kHeadDim, vc + at);
+    }
+    const int64_t key = min(key0 + lane, last);
+    cp4(&ch.ks[lane], ks + key);
+    cp4(&ch.vs[lane], vs + key);
   }
-  const int64_t key = min(key0 + lane, last);
-  cp4(&ch.ks[lane], ks + key);
-  cp4(&ch.vs[lane], vs + key);
 }
 
 // The warps' results of a row block.  Channel ch of a row lies at slot(ch): the order in which
@@ -214,7 +235,7 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bf
 __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x); }
 
 template <class T, bool kE4m3>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 16 / kWarps)
     cache_attn_kernel(const __grid_constant__ CacheAttnArgs a, int splits, int* err) {
   extern __shared__ uint4 smem_raw[];
   Shared& smem = *reinterpret_cast<Shared*>(smem_raw);
@@ -326,35 +347,49 @@ __global__ void __launch_bounds__(kThreads, 2)
       const Chunk& cur = ring[stage];
       stage = stage + 1 == kStages ? 0 : stage + 1;
       const int key0 = ch * kChunk;
+      const float ahead = static_cast<float>(fp - key0);  // tokens (frame 1) past the chunk's first
       // Scores of 8 rows x 32 keys: lane (g, c) gets row g, columns 2c and 2c + 1 of each tile.
-      float x[4][2];
+      float x[4][2], d[4][4];
+      uint32_t w[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
         const int kr = 8 * t + tile_key(g);
         const uint4 kw = *reinterpret_cast<const uint4*>(&cur.k[kr][16 * (c ^ ((kr >> 1) & 2))]);
-        const uint32_t w[4] = {flip<kE4m3>(kw.x), flip<kE4m3>(kw.y), flip<kE4m3>(kw.z), flip<kE4m3>(kw.w)};
+        w[t][0] = flip<kE4m3>(kw.x), w[t][1] = flip<kE4m3>(kw.y), w[t][2] = flip<kE4m3>(kw.z), w[t][3] = flip<kE4m3>(kw.w);
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          mma_f16(d, qa[s], codes_to_f16x2<kE4m3, false>(w[s]), codes_to_f16x2<kE4m3, true>(w[s]));
+        for (int e = 0; e < 4; ++e) d[t][e] = 0.0f;
+      }
+      // Four independent chains: a tile's four steps follow each other, the tiles do not.
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int kk = 8 * t + ((2 * c + e) ^ (c & 1));
-          const float dot = (d[e] + d[2 + e]) * cur.ks[kk];
-          float y;
-          if (a.t.cap_out > 0.0f) {
-            // cap log2(e) tanh(z) = cap log2(e) (1 - 2 / (1 + e^(2z)))
-            y = a.t.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(dot * cap_scale)));
-          } else {
-            y = dot * score_scale;
-          }
-          if (a.slopes) {
-            const int dist = fp - frame_index(key0 + kk, a.t.frame, a.frame_magic);
-            y -= slope * static_cast<float>(abs(dist));
-          }
-          x[t][e] = key0 + kk < limit ? y : -INFINITY;
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          mma_f16(d[t], qa[s], codes_to_f16x2<kE4m3, false>(w[t][s]), codes_to_f16x2<kE4m3, true>(w[t][s]));
+      // Each term over all eight scores of the lane under one branch, so they overlap.
+#define VA_EACH_SCORE(...)                          \
+  _Pragma("unroll") for (int t = 0; t < 4; ++t) {   \
+    _Pragma("unroll") for (int e = 0; e < 2; ++e) { \
+      const int kk = 8 * t + ((2 * c + e) ^ (c & 1)); \
+      __VA_ARGS__                                   \
+    }                                               \
+  }
+      VA_EACH_SCORE(x[t][e] = (d[t][e] + d[t][2 + e]) * cur.ks[kk];)
+      if (a.t.cap_out > 0.0f) {
+        // cap log2(e) tanh(z) = cap log2(e) (1 - 2 / (1 + e^(2z)))
+        VA_EACH_SCORE((void)kk; x[t][e] = fmaf(-2.0f * a.t.cap_out, rcp(1.0f + ex2(x[t][e] * cap_scale)), a.t.cap_out);)
+      } else {
+        VA_EACH_SCORE((void)kk; x[t][e] *= score_scale;)
+      }
+      if (a.slopes) {
+        if (a.t.frame == 1) {
+          VA_EACH_SCORE(x[t][e] = fmaf(-slope, fabsf(ahead - static_cast<float>(kk)), x[t][e]);)
+        } else {
+          VA_EACH_SCORE(const float dist = static_cast<float>(fp - frame_index(key0 + kk, a.t.frame, a.frame_magic));
+                        x[t][e] = fmaf(-slope, fabsf(dist), x[t][e]);)
         }
       }
+      VA_EACH_SCORE(x[t][e] = key0 + kk < limit ? x[t][e] : -INFINITY;)
+#undef VA_EACH_SCORE
       float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])),
                         fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -482,12 +517,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 template <class T, bool kE4m3>
 cudaError_t launch(const CacheAttnArgs& a, int splits, int64_t blocks, int* err, cudaStream_t st) {
   auto kern = cache_attn_kernel<T, kE4m3>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), sizeof(Shared), ready);
   if (e != cudaSuccess) return e;
-  if (splits > 8) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kThreads);

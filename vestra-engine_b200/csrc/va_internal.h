@@ -6,6 +6,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <stddef.h>
 #include <stdint.h>
 
@@ -309,6 +310,8 @@ struct HeadsRef {
   int64_t token_stride, head_stride;
   int heads;
 };
+// A cluster kernel's attributes, set once per device (`ready`: one bit per device below 64).
+cudaError_t prepare_kernel(const void* kernel, int smem_bytes, std::atomic<uint64_t>& ready);
 enum ElemType { kBf16 = 0, kF16 = 1, kF32 = 2 };
 
 constexpr int kRopeMaxPairs = 128;

@@ -26,6 +26,7 @@
 // partial rows meet through distributed shared memory in rank order: no workspace, no
 // second launch, the same bits on every run.
 #include <algorithm>
+#include <atomic>
 #include <queue>
 #include <vector>
 
@@ -618,9 +619,8 @@ template <bool kF16, bool kCap, bool kBias>
 cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const MaskedArgs& a,
                    int64_t blocks, int* err, cudaStream_t st) {
   auto kern = masked_attn_kernel<kF16, kCap, kBias>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem::kLaunchBytes);
-  if (e == cudaSuccess && a.splits > 8)
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), Smem::kLaunchBytes, ready);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));

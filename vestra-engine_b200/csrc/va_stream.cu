@@ -226,6 +226,21 @@ int cache_rows_call(va_ctx* c, const va_kv_cache* cache, int64_t rows, const int
 
 }  // namespace
 
+namespace va {
+cudaError_t prepare_kernel(const void* kernel, int smem_bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (ready.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+  // clusters of up to 16 CTAs
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+}  // namespace va
+
 extern "C" {
 
 int va_rope_axes_device(va_ctx* c, const va_rope_axes* rope, int64_t rows, int head_dim,

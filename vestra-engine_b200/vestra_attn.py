@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -261,7 +262,8 @@ _DTYPE_CODES = {}  # torch dtype -> VA_* of the streaming operators, filled on f
 def _dtype_code(dtype):
     code = _DTYPE_CODES.get(dtype)
     if code is None:
-        code = {"torch.bfloat16": VA_BF16, "torch.float16": VA_F16, "torch.float32": VA_F32}.get(str(dtype), -1)
+        code = {"torch.bfloat16": VA_BF16, "torch.float16": VA_F16, "torch.float32": VA_F32,
+                "torch.int32": -2}.get(str(dtype), -1)
         _DTYPE_CODES[dtype] = code
     return code
 
@@ -270,32 +272,41 @@ def _refuse(msg):
     raise VestraError(VA_ERR_INVALID, msg)
 
 
+# A va_heads as bytes (the C side only reads it): packing costs a third of a ctypes structure.
+_PACK_HEADS = struct.Struct("=QqqiI").pack
+
+
 def _heads(x, device, what, channels=None):
-    """va_heads of a [rows, heads, channels] torch tensor; any token and head strides."""
+    """(va_heads, rows, heads) of a [rows, heads, channels] torch tensor; any token and head strides."""
     if not getattr(x, "is_cuda", False) or x.get_device() != device:
         _refuse(f"{what} must be a tensor on CUDA device {device}")
-    shape, code = x.shape, _dtype_code(x.dtype)
-    if len(shape) != 3 or code < 0 or (channels is not None and shape[2] != channels):
+    code = _DTYPE_CODES.get(x.dtype)
+    if code is None:
+        code = _dtype_code(x.dtype)
+    if code < 0 or x.dim() != 3:
         _refuse(f"{what} must be [rows, heads, {channels or 'channels'}] bf16, f16 or f32")
-    rows, heads, d = shape
+    rows, heads, d = x.shape
     ts, hs, cs = x.stride()
-    if cs != 1:
-        _refuse(f"{what} needs contiguous channels")
+    if cs != 1 or (channels is not None and d != channels):
+        _refuse(f"{what} needs {channels or ''} contiguous channels")
     if heads == 1:
         hs = d
     if rows <= 1:  # never stepped over
         ts = heads * max(hs, d)
-    return VaHeads(x.data_ptr(), ts, hs, heads, code)
+    return _PACK_HEADS(x.data_ptr(), ts, hs, heads, code), rows, heads
 
 
-def _device_array(x, device, what, dtype, count):
+_INT32, _FLOAT32 = -2, VA_F32  # kinds of _device_array
+
+
+def _device_array(x, device, what, kind, count):
     """Address of a contiguous device tensor of one dtype and element count (None passes)."""
     if x is None:
         return None
     if not getattr(x, "is_cuda", False) or x.get_device() != device:
         _refuse(f"{what} must be a tensor on CUDA device {device}")
-    if not x.is_contiguous() or x.numel() != count or str(x.dtype) != dtype:
-        _refuse(f"{what} must be a contiguous {dtype} tensor of {count} elements")
+    if _dtype_code(x.dtype) != kind or x.numel() != count or not x.is_contiguous():
+        _refuse(f"{what} must be a contiguous {'int32' if kind == _INT32 else 'float32'} tensor of {count} elements")
     return x.data_ptr()
 
 
@@ -548,24 +559,38 @@ class Context:
     def rope_axes(self, rope: "RopeAxes", positions, q, q_out, k=None, k_out=None, stream=0):
         """Rotates q (and k) [rows, heads, head_dim] by positions int32 [rows, axes] (device);
         an output may be its input."""
-        rows, d = q.shape[0], q.shape[-1]
-        t = [None if x is None else _heads(x, self.device, name, d)
-             for x, name in ((q, "q"), (q_out, "q_out"), (k, "k"), (k_out, "k_out"))]
-        for x in (q_out, k, k_out):
-            if x is not None and x.shape[0] != rows:
-                raise VestraError(VA_ERR_INVALID, "q, k and their outputs must have the same rows")
-        pos = _device_array(positions, self.device, "positions", "torch.int32", rows * rope.c.axes)
-        self.check(self.lib.va_rope_axes_device(self.h, ctypes.byref(rope.c), rows, d, pos, *map(_byref, t), stream))
+        d = q.shape[-1]
+        qh, rows, _ = _heads(q, self.device, "q", d)
+        qo, n, _ = _heads(q_out, self.device, "q_out", d)
+        kh = ko = None
+        if k is not None or k_out is not None:
+            kh, n1, _ = _heads(k, self.device, "k", d)
+            ko, n2, _ = _heads(k_out, self.device, "k_out", d)
+            if n1 != rows or n2 != rows:
+                _refuse("k and k_out must have the rows of q")
+        if n != rows:
+            _refuse("q and q_out must have the same rows")
+        rc = self.lib.va_rope_axes_device(self.h, rope.ref, rows, d,
+                                          _device_array(positions, self.device, "positions", _INT32, rows * rope.c.axes),
+                                          qh, qo, kh, ko, stream)
+        if rc:
+            self.check(rc)
 
     def masked_attention(self, plan: "AttentionPlan", q, k, v, out, stream=0):
         """out = attention of the plan's documents: q, out [rows, heads, 64], k, v [rows,
         kv_heads, 64], bf16 or f16 on the device.  Rows of no document are left alone."""
-        t = [_heads(x, self.device, name, 64) for x, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out"))]
-        if min(q.shape[0], out.shape[0]) < plan.q_rows or min(k.shape[0], v.shape[0]) < plan.k_rows:
-            raise VestraError(VA_ERR_INVALID, "the plan's documents reach past the tensors' rows")
+        device = self.device
+        qh, nq, _ = _heads(q, device, "q", 64)
+        kh, nk, _ = _heads(k, device, "k", 64)
+        vh, nv, _ = _heads(v, device, "v", 64)
+        oh, no, _ = _heads(out, device, "out", 64)
+        if nq < plan.q_rows or no < plan.q_rows or nk < plan.k_rows or nv < plan.k_rows:
+            _refuse("the plan's documents reach past the tensors' rows")
         if not plan.h:
             raise VestraError(VA_ERR_STATE, "the attention plan is closed")
-        self.check(self.lib.va_masked_attention_device(self.h, plan.h, *map(_byref, t), stream))
+        rc = self.lib.va_masked_attention_device(self.h, plan.h, qh, kh, vh, oh, stream)
+        if rc:
+            self.check(rc)
 
     def kv_cache_write(self, cache: "KvCache", k, v, offsets, lens, stream=0):
         """Appends rows offsets[b]..offsets[b+1] of k and v [rows, kv_heads, 64] as the last of
@@ -578,32 +603,38 @@ class Context:
         self._cache_rows(self.lib.va_kv_cache_read_device, cache, k_out, v_out, offsets, first, "first", stream)
 
     def _cache_rows(self, fn, cache, k, v, offsets, edge, name, stream):
-        cache.check_device(self.device)
-        kh, vh = _heads(k, self.device, "k", 64), _heads(v, self.device, "v", 64)
-        if k.shape[0] != v.shape[0]:
-            raise VestraError(VA_ERR_INVALID, "k and v must have the same rows")
-        n = cache.c.documents
-        self.check(fn(self.h, ctypes.byref(cache.c), k.shape[0],
-                      _device_array(offsets, self.device, "offsets", "torch.int32", n + 1),
-                      _device_array(edge, self.device, name, "torch.int32", n), _byref(kh), _byref(vh), stream))
+        device = self.device
+        cache.check_device(device)
+        kh, rows, _ = _heads(k, device, "k", 64)
+        vh, n, _ = _heads(v, device, "v", 64)
+        if n != rows:
+            _refuse("k and v must have the same rows")
+        docs = cache.documents
+        rc = fn(self.h, cache.ref, rows, _device_array(offsets, device, "offsets", _INT32, docs + 1),
+                _device_array(edge, device, name, _INT32, docs), kh, vh, stream)
+        if rc:
+            self.check(rc)
 
     def cache_attention(self, cache: "KvCache", q, out, offsets, lens, max_tokens, causal=True, frame=1, prefix=None,
                         slopes=None, score_cap=0.0, scale=0.0, stream=0):
         """Attention of the last offsets[b+1] - offsets[b] of document b's lens[b] tokens over
         the cache: q, out [rows, heads, 64]; offsets, lens, prefix int32 and slopes f32 on the
         device, read when the kernel runs."""
-        cache.check_device(self.device)
-        qh, oh = _heads(q, self.device, "q", 64), _heads(out, self.device, "out", 64)
-        if q.shape != out.shape:
-            raise VestraError(VA_ERR_INVALID, "q and out must have the same shape")
-        n, heads = cache.c.documents, q.shape[1]
-        terms = VaAttnTerms(heads, cache.c.kv_heads, int(bool(causal)), frame, scale, score_cap)
-        self.check(self.lib.va_cache_attention_device(
-            self.h, ctypes.byref(cache.c), ctypes.byref(terms), q.shape[0],
-            _device_array(offsets, self.device, "offsets", "torch.int32", n + 1),
-            _device_array(lens, self.device, "lens", "torch.int32", n), max_tokens,
-            _device_array(prefix, self.device, "prefix", "torch.int32", n),
-            _device_array(slopes, self.device, "slopes", "torch.float32", heads), _byref(qh), _byref(oh), stream))
+        device = self.device
+        cache.check_device(device)
+        qh, rows, heads = _heads(q, device, "q", 64)
+        oh, n, out_heads = _heads(out, device, "out", 64)
+        if n != rows or out_heads != heads:
+            _refuse("q and out must have the same shape")
+        docs = cache.documents
+        terms = VaAttnTerms(heads, cache.kv_heads, 1 if causal else 0, frame, scale, score_cap)
+        rc = self.lib.va_cache_attention_device(
+            self.h, cache.ref, ctypes.byref(terms), rows, _device_array(offsets, device, "offsets", _INT32, docs + 1),
+            _device_array(lens, device, "lens", _INT32, docs), max_tokens,
+            _device_array(prefix, device, "prefix", _INT32, docs),
+            _device_array(slopes, device, "slopes", _FLOAT32, heads), qh, oh, stream)
+        if rc:
+            self.check(rc)
 
     def check_device(self):
         self.check(self.lib.va_check_device(self.h))
@@ -684,10 +715,6 @@ class Context:
         return self.lib.va_last_error(self.h).decode()
 
 
-def _byref(x):
-    return None if x is None else ctypes.byref(x)
-
-
 class RopeAxes:
     """va_rope_axes: channels turned by each position axis (for example (16, 24, 24) for
     time, height, width), frequency base, layout "per_axis" or "shared", pairing 0 (i, i + half)
@@ -698,6 +725,7 @@ class RopeAxes:
         if not 1 <= len(sections) <= 4 or layout not in ROPE_LAYOUTS:
             raise VestraError(VA_ERR_INVALID, "rope needs 1 to 4 sections and layout 'per_axis' or 'shared'")
         self.c = VaRopeAxes(len(sections), (ctypes.c_int32 * 4)(*sections), ROPE_LAYOUTS[layout], pairing, base)
+        self.ref = ctypes.byref(self.c)
 
 
 def _plan_arrays(q_offsets, k_offsets, prefix):
@@ -769,6 +797,8 @@ class KvCache:
         self.tensors = (k_codes, v_codes, k_scales, v_scales)  # kept alive
         self.device = k_codes.get_device()
         self.c = VaKvCache(docs, heads, capacity, fmt, 0, *[x.data_ptr() for x in self.tensors])
+        self.ref = ctypes.byref(self.c)
+        self.documents, self.kv_heads = docs, heads
 
     def check_device(self, device):
         if self.device != device:
