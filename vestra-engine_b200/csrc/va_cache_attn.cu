@@ -16,8 +16,8 @@
 // largest magnitude in [1, 2) and the factor goes to the scores; a probability times its
 // value scale is scaled by 2^(kTop - E), E above the largest value scale so far.
 //
-// A cluster of CTAs shares one (document, key head, row block); its warps take 32-key
-// chunks in turn through a ring of its own in shared memory (cp.async, two chunks ahead), each
+// A cluster of CTAs shares one (document, key head, row block); its warps take 64-key
+// chunks in turn through a ring of its own in shared memory (cp.async, one chunk ahead), each
 // warp with its own running maximum and sum, and the partial results meet in shared memory
 // and then, through distributed shared memory, across the cluster in rank order: one
 // launch, no workspace, no atomics, and the same bits on every run.
@@ -29,6 +29,7 @@
 // of the four keys whose probabilities it holds.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "va_internal.h"
 #include "va_ptx.cuh"
@@ -38,14 +39,13 @@ namespace va {
 namespace {
 
 constexpr int kHeadDim = 64;
-#ifndef KW
-#define KW 8
-#endif
-constexpr int kWarps = KW;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRowsPerBlock = 8;
-constexpr int kChunk = 32;         // keys a warp takes at a time
-constexpr int kStages = 3;         // chunks of a warp in shared memory
+constexpr int kChunk = 64;         // keys a warp takes at a time
+constexpr int kTiles = kChunk / 8;
+constexpr int kStages = 2;         // chunks of a warp in shared memory
+constexpr int kCtasPerSm = 3;
 constexpr int kMaxCluster = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTop = 14;       // probabilities times value scales are brought below 2^kTop
@@ -155,22 +155,28 @@ __device__ __forceinline__ void load_chunk(Chunk& ch, const uint8_t* kc, const u
   if (key0 + kChunk - 1 <= last) {
     const int64_t at = (static_cast<int64_t>(key0) + row) * kHeadDim + 16 * p;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kTiles; ++i) {
       cp16(to + 8 * i * kHeadDim, kc + at + 8 * i * kHeadDim);
       cp16(to + (kChunk + 8 * i) * kHeadDim, vc + at + 8 * i * kHeadDim);
     }
-    cp4(&ch.ks[lane], ks + key0 + lane);
-    cp4(&ch.vs[lane], vs + key0 + lane);
+#pragma unroll
+    for (int i = 0; i < kChunk; i += 32) {
+      cp4(&ch.ks[i + lane], ks + key0 + i + lane);
+      cp4(&ch.vs[i + lane], vs + key0 + i + lane);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kTiles; ++i) {
       const int64_t at = static_cast<int64_t>(min(key0 + 8 * i + row, last)) * kHeadDim + 16 * p;
       cp16(to + 8 * i * kHeadDim, kc + at);
       cp16(to + (kChunk + 8 * i) * kHeadDim, vc + at);
     }
-    const int64_t key = min(key0 + lane, last);
-    cp4(&ch.ks[lane], ks + key);
-    cp4(&ch.vs[lane], vs + key);
+#pragma unroll
+    for (int i = 0; i < kChunk; i += 32) {
+      const int64_t key = min(key0 + i + lane, last);
+      cp4(&ch.ks[i + lane], ks + key);
+      cp4(&ch.vs[i + lane], vs + key);
+    }
   }
 }
 
@@ -194,7 +200,7 @@ struct Shared {
   };
   Part part[kMaxCluster];  // [own row][cluster rank]
 };
-static_assert(2 * (sizeof(Shared) + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(kCtasPerSm * (sizeof(Shared) + 1024) <= 228 * 1024, "shared memory of an SM");
 
 // Stores v at this address of CTA `rank` of the cluster.
 __device__ __forceinline__ void st_cluster(float* p, int rank, float v) {
@@ -205,29 +211,29 @@ __device__ __forceinline__ void st_cluster(float* p, int rank, float v) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// 16 consecutive elements (two 16-byte loads).
-__device__ __forceinline__ void load16(const __nv_bfloat16* p, float* x) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint4 u = reinterpret_cast<const uint4*>(p)[h];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[8 * h + 2 * i] = __uint_as_float(w[i] << 16);
-      x[8 * h + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
+// 16 consecutive two-byte elements.
+struct RawRow {
+  uint4 u[2];
+};
+__device__ __forceinline__ void load_row(RawRow& r, const void* p) {
+  r.u[0] = __ldg(static_cast<const uint4*>(p));
+  r.u[1] = __ldg(static_cast<const uint4*>(p) + 1);
 }
-__device__ __forceinline__ void load16(const __half* p, float* x) {
+template <class T>
+__device__ __forceinline__ void unpack_row(const RawRow& r, float* x) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint4 u = reinterpret_cast<const uint4*>(p)[h];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const uint32_t w[4] = {r.u[h].x, r.u[h].y, r.u[h].z, r.u[h].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      x[8 * h + 2 * i] = f.x;
-      x[8 * h + 2 * i + 1] = f.y;
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[8 * h + 2 * i] = f.x;
+        x[8 * h + 2 * i + 1] = f.y;
+      } else {
+        x[8 * h + 2 * i] = __uint_as_float(w[i] << 16);
+        x[8 * h + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
     }
   }
 }
@@ -235,7 +241,7 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bf
 __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x); }
 
 template <class T, bool kE4m3>
-__global__ void __launch_bounds__(kThreads, 16 / kWarps)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
     cache_attn_kernel(const __grid_constant__ CacheAttnArgs a, int splits, int* err) {
   extern __shared__ uint4 smem_raw[];
   Shared& smem = *reinterpret_cast<Shared*>(smem_raw);
@@ -291,13 +297,25 @@ __global__ void __launch_bounds__(kThreads, 16 / kWarps)
     const int fp = frame_index(token + len - tokens, a.t.frame, a.frame_magic);
     const float slope = a.slopes ? __ldg(a.slopes + head) * kLog2e : 0.0f;
 
+    // The row's load, then the first chunks', go off together; the row is used while the chunks
+    // arrive.
+    RawRow raw;
+    load_row(raw, qd + (begin + static_cast<int64_t>(token)) * a.q.token_stride + head * a.q.head_stride + 16 * c);
+    const int chunks = (block_limit + kChunk - 1) / kChunk;
+    const int stride = splits * kWarps;
+    const int first = rank * kWarps + warp;
+    Chunk* ring = smem.ring[warp];
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (first + i * stride < chunks) load_chunk(ring[i], kc, vc, ks, vs, (first + i * stride) * kChunk, len - 1, lane);
+      cp_commit();
+    }
     // Query row in fragment order: word s of the lane's 16 channels [16c, 16c + 16).
     uint32_t qa[4][4];
     float q_scale;
     {
-      const T* p = qd + (begin + static_cast<int64_t>(token)) * a.q.token_stride + head * a.q.head_stride + 16 * c;
       float x[16];
-      load16(p, x);
+      unpack_row<T>(raw, x);
       uint32_t top = 0;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -325,15 +343,6 @@ __global__ void __launch_bounds__(kThreads, 16 / kWarps)
       for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    const int chunks = (block_limit + kChunk - 1) / kChunk;
-    const int stride = splits * kWarps;
-    const int first = rank * kWarps + warp;
-    Chunk* ring = smem.ring[warp];
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-      if (first + i * stride < chunks) load_chunk(ring[i], kc, vc, ks, vs, (first + i * stride) * kChunk, len - 1, lane);
-      cp_commit();
-    }
     int stage = 0;
     for (int ch = first; ch < chunks; ch += stride) {
       cp_wait<kStages - 2>();
@@ -349,10 +358,10 @@ __global__ void __launch_bounds__(kThreads, 16 / kWarps)
       const int key0 = ch * kChunk;
       const float ahead = static_cast<float>(fp - key0);  // tokens (frame 1) past the chunk's first
       // Scores of 8 rows x 32 keys: lane (g, c) gets row g, columns 2c and 2c + 1 of each tile.
-      float x[4][2], d[4][4];
-      uint32_t w[4][4];
+      float x[kTiles][2], d[kTiles][4];
+      uint32_t w[kTiles][4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int t = 0; t < kTiles; ++t) {
         const int kr = 8 * t + tile_key(g);
         const uint4 kw = *reinterpret_cast<const uint4*>(&cur.k[kr][16 * (c ^ ((kr >> 1) & 2))]);
         w[t][0] = flip<kE4m3>(kw.x), w[t][1] = flip<kE4m3>(kw.y), w[t][2] = flip<kE4m3>(kw.z), w[t][3] = flip<kE4m3>(kw.w);
@@ -363,11 +372,11 @@ __global__ void __launch_bounds__(kThreads, 16 / kWarps)
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < kTiles; ++t)
           mma_f16(d[t], qa[s], codes_to_f16x2<kE4m3, false>(w[t][s]), codes_to_f16x2<kE4m3, true>(w[t][s]));
       // Each term over all eight scores of the lane under one branch, so they overlap.
 #define VA_EACH_SCORE(...)                          \
-  _Pragma("unroll") for (int t = 0; t < 4; ++t) {   \
+  _Pragma("unroll") for (int t = 0; t < kTiles; ++t) { \
     _Pragma("unroll") for (int e = 0; e < 2; ++e) { \
       const int kk = 8 * t + ((2 * c + e) ^ (c & 1)); \
       __VA_ARGS__                                   \
@@ -390,15 +399,21 @@ __global__ void __launch_bounds__(kThreads, 16 / kWarps)
       }
       VA_EACH_SCORE(x[t][e] = key0 + kk < limit ? x[t][e] : -INFINITY;)
 #undef VA_EACH_SCORE
-      float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])),
-                        fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
+      float top = x[0][0];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) top = max3f(top, x[t][0], x[t][1]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const float m_new = fmaxf(m, top);
       // The largest value scale of the keys some row sees (NaN and infinity set no scale; they
       // reach the rows that see them on their own).
-      const uint32_t vbits = __float_as_uint(cur.vs[lane]);
-      const uint32_t vtop = __reduce_max_sync(0xffffffffu, key0 + lane < block_limit && vbits < 0x7f800000u ? vbits : 0u);
+      uint32_t vmax = 0;
+#pragma unroll
+      for (int i = 0; i < kChunk; i += 32) {
+        const uint32_t vbits = __float_as_uint(cur.vs[i + lane]);
+        if (key0 + i + lane < block_limit && vbits < 0x7f800000u) vmax = max(vmax, vbits);
+      }
+      const uint32_t vtop = __reduce_max_sync(0xffffffffu, vmax);
       const int e_new = max(v_exp, static_cast<int>(vtop >> 23) - 126);
       if (__any_sync(0xffffffffu, m_new > m) || e_new > v_exp) {
         float alpha = m_new > m ? ex2(m - m_new) : 1.0f;  // 0 for the first keys
@@ -415,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 16 / kWarps)
       const float base = m == -INFINITY ? 0.0f : m;
       const float v_scale = __uint_as_float(static_cast<uint32_t>(kTop - v_exp + 127) << 23);  // 2^(kTop - E)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < kTiles / 2; ++u) {
         uint32_t pa[4];
         uint2 vw[4];
 #pragma unroll
@@ -558,7 +573,7 @@ cudaError_t launch_cache_attention(const KvCacheRef& c, const AttnTerms& t, int 
   const int64_t units = static_cast<int64_t>(c.documents) * c.kv_heads * a.row_blocks;
   // CTAs per unit: the lengths are on the device, so by the capacity: enough for kTarget CTAs per
   // SM (documents differ in length), at least two chunks per warp.
-  static const int kTarget = getenv("VAT") ? atoi(getenv("VAT")) : 4;
+  constexpr int kTarget = 4;
   const int64_t most = std::max<int64_t>(1, c.capacity / (2 * kChunk * kWarps));
   int splits = 1;
   while (splits < kMaxCluster && units * splits < kTarget * sms && 2 * splits <= most) splits *= 2;

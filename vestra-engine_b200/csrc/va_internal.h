@@ -371,7 +371,6 @@ struct MaskedArgs {
   int group, tile_tokens, items, splits;
   const MaskedItem* item;
   const float* slopes;      // [heads] device, times log2(e); nullptr: no bias
-  const float* frame_of;    // [keys + padding] F32 frame index of a key position (bias only)
   HeadsRef out;
 };
 cudaError_t launch_masked(const HeadsRef& q, const HeadsRef& k, const HeadsRef& v, int64_t q_rows, int64_t k_rows,

@@ -194,10 +194,7 @@ __device__ __forceinline__ void dequantise(uint2 u, float scale, float top, floa
 
 // An eight-lane group takes one row and kHeads heads of K and of V: all its loads are
 // issued before the first is used.
-#ifndef KH
-#define KH 1
-#endif
-constexpr int kHeads = KH;
+constexpr int kHeads = 1;
 
 template <class T, bool kE4m3, bool kWrite>
 __global__ void __launch_bounds__(kThreads) kv_rows_kernel(const __grid_constant__ KvArgs a, int* err) {

@@ -49,6 +49,8 @@ constexpr uint32_t kTileBytes = kTile * kHeadDim * 2;
 constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 192;
 constexpr int kMaxSplits = 16;
+// See masked_attn_kernel: caps up to 50 (72.13 in the log2 domain), probabilities from 2^-120 up.
+constexpr float kFixedCap = 72.2f, kFixedTop = 2.0f * kFixedCap - 120.0f;
 
 struct Smem {
   static constexpr uint32_t kQ = 0;
@@ -109,6 +111,12 @@ __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
   }
 }
 
+// One arrival for the warp, after every lane's work before it.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -151,35 +159,42 @@ __device__ __forceinline__ Geom make_geom(const MaskedArgs& a) {
   return g;
 }
 
-__device__ __forceinline__ void run_producer(const Ctl& c, const Geom& g, const MaskedArgs& a,
-                                             const CUtensorMap* mq, const CUtensorMap* mk,
-                                             const CUtensorMap* mv, int* err) {
-  if (g.n == 0) return;
-  volatile int* abort_flag = c.abort_flag();
+__device__ __forceinline__ void load_k(const Ctl& c, const Geom& g, const CUtensorMap* mk, int j) {
+  const int s = j % kKStages;
+  mbar_arrive_expect_tx(c.k_full(s), kTileBytes);
+  tma_load_3d(c.sK(s), mk, c.k_full(s), 0, g.kvh, g.it.k_row + (g.t0 + j) * kTile);
+  *c.k_issued() = j + 1;
+}
+__device__ __forceinline__ void load_v(const Ctl& c, const Geom& g, const CUtensorMap* mv, int j) {
+  const int s = j % kVStages;
+  mbar_arrive_expect_tx(c.v_full(s), kTileBytes);
+  tma_load_3d(c.sV(s), mv, c.v_full(s), 0, g.kvh, g.it.k_row + (g.t0 + j) * kTile);
+  *c.v_issued() = j + 1;
+}
+
+// Q, K(0), K(1) and V(0): their stages start out free.
+__device__ __forceinline__ void first_loads(const Ctl& c, const Geom& g, const MaskedArgs& a, const CUtensorMap* mq,
+                                            const CUtensorMap* mk, const CUtensorMap* mv) {
   // The box always brings tile_tokens x group rows; past the tensor's end they are zeros.
   mbar_arrive_expect_tx(c.q_full(), a.tile_tokens * a.group * kHeadDim * 2);
   tma_load_3d(c.sQ(), mq, c.q_full(), 0, g.kvh * a.group, g.it.q_row);
-  auto load_k = [&](int j) {
-    const int s = j % kKStages;
-    if (!mbar_wait(c.k_empty(s), ((j / kKStages) & 1) ^ 1, abort_flag, err, kDevTimeoutProducer)) return false;
-    mbar_arrive_expect_tx(c.k_full(s), kTileBytes);
-    tma_load_3d(c.sK(s), mk, c.k_full(s), 0, g.kvh, g.it.k_row + (g.t0 + j) * kTile);
-    *c.k_issued() = j + 1;
-    return true;
-  };
-  auto load_v = [&](int j) {
-    const int s = j % kVStages;
-    if (!mbar_wait(c.v_empty(s), ((j / kVStages) & 1) ^ 1, abort_flag, err, kDevTimeoutProducer)) return false;
-    mbar_arrive_expect_tx(c.v_full(s), kTileBytes);
-    tma_load_3d(c.sV(s), mv, c.v_full(s), 0, g.kvh, g.it.k_row + (g.t0 + j) * kTile);
-    *c.v_issued() = j + 1;
-    return true;
-  };
-  bool ok = load_k(0);
-  if (ok && g.n > 1) ok = load_k(1);
-  for (int j = 0; ok && j < g.n; ++j) {
-    ok = load_v(j);
-    if (ok && j + 2 < g.n) ok = load_k(j + 2);
+  load_k(c, g, mk, 0);
+  if (g.n > 1) load_k(c, g, mk, 1);
+  load_v(c, g, mv, 0);
+}
+
+// The rest of the loads (one thread), in the order the UMMA chain reads them.
+__device__ __forceinline__ void run_producer(const Ctl& c, const Geom& g, const CUtensorMap* mk,
+                                             const CUtensorMap* mv, int* err) {
+  volatile int* abort_flag = c.abort_flag();
+  for (int j = 2; j < g.n + 1; ++j) {
+    if (j < g.n) {
+      if (!mbar_wait(c.k_empty(j % kKStages), ((j / kKStages) & 1) ^ 1, abort_flag, err, kDevTimeoutProducer)) return;
+      load_k(c, g, mk, j);
+    }
+    const int v = j - 1;
+    if (!mbar_wait(c.v_empty(v % kVStages), ((v / kVStages) & 1) ^ 1, abort_flag, err, kDevTimeoutProducer)) return;
+    load_v(c, g, mv, v);
   }
 }
 
@@ -283,14 +298,13 @@ __device__ __forceinline__ uint32_t pack_f16x2_of(uint64_t p) {
 __device__ __forceinline__ void cap_scores(float* s, const AttnTerms& t, bool partial) {
   bool wide = partial;
   if (!partial) {
-    float mx[2], mn[2] = {s[0], s[2]};
-    row_maxima(s, mx);
+    float mx[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
+    for (int q = 0; q < 64; q += 8)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) asm("min.f32 %0, %0, %1, %2;" : "+f"(mn[i]) : "f"(s[4 * k + 2 * i]), "f"(s[4 * k + 2 * i + 1]));
+      for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], fabsf(s[q + 2 * i]), fabsf(s[q + 2 * i + 1]));
     // a NaN fails no comparison: the polynomial hands it on as well
-    wide = fmaxf(fmaxf(mx[0], mx[1]), -fminf(mn[0], mn[1])) > t.cap_range;
+    wide = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) > t.cap_range;
   }
   if (__any_sync(0xffffffffu, wide)) {
 #pragma unroll
@@ -310,7 +324,102 @@ __device__ __forceinline__ void cap_scores(float* s, const AttnTerms& t, bool pa
   }
 }
 
-template <bool kF16, bool kCap, bool kBias>
+// s <- s (times scale log2(e) unless capped before) - slope |f(row) - f(key)|, f(x) = floor(x / frame),
+// for the thread's columns k0 + c0 + 8k + {0, 1}, the rows' frame indices and slopes (times
+// log2(e)) given.  Frame indices stay below 2^24, so their differences are exact.
+//   frame 1: the distances step by 8 from block to block;
+//   no frame starts inside the tile: one distance per row;
+//   else: floor((x + 1/2) / frame) by an addition of 3 * 2^22 rounded down, x = the key's offset
+//   from a frame start inside or just before the tile, so below 256 and never near a step.
+// side: -1 when no visible key of the tile lies in a later frame than a row, +1 when none lies in an
+// earlier one (the distance is then the difference or its negative), else 0.
+template <bool kCap>
+__device__ __forceinline__ void bias_scores(float* s, const AttnTerms& t, int k0, int c0, const int* frame,
+                                            const float* slope, int side) {
+  const uint64_t sc2 = f32x2_pack(t.scale_log2, t.scale_log2);
+  uint64_t ns[2], d[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float v = side < 0 ? slope[i] : -slope[i];
+    ns[i] = f32x2_pack(v, v);
+  }
+  auto add_bias = [&](int k, int i) {
+    uint64_t v = f32x2_pack(s[4 * k + 2 * i], s[4 * k + 2 * i + 1]);
+    if (!kCap) v = f32x2_mul(v, sc2);
+    f32x2_unpack(f32x2_fma(d[i] & 0x7fffffff7fffffffull, ns[i], v), s[4 * k + 2 * i], s[4 * k + 2 * i + 1]);
+  };
+  if (t.frame == 1) {
+    const uint64_t step = f32x2_pack(8.0f, 8.0f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float at = static_cast<float>(k0 + c0 - frame[i]);
+      d[i] = f32x2_pack(at, at + 1.0f);
+    }
+    if (side != 0) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint64_t v = f32x2_pack(s[4 * k + 2 * i], s[4 * k + 2 * i + 1]);
+          if (!kCap) v = f32x2_mul(v, sc2);
+          f32x2_unpack(f32x2_fma(d[i], ns[i], v), s[4 * k + 2 * i], s[4 * k + 2 * i + 1]);
+          d[i] = f32x2_add(d[i], step);
+        }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        add_bias(k, i);
+        d[i] = f32x2_add(d[i], step);
+      }
+    return;
+  }
+  if (side < 0) ns[0] ^= 0x8000000080000000ull, ns[1] ^= 0x8000000080000000ull;  // below: distances
+  int base = k0 / t.frame;              // frame of the tile's first key
+  int start = base * t.frame - k0;      // its start, at most 0
+  if (start + t.frame >= kTile) {       // the next frame starts past the tile
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float v = static_cast<float>(base - frame[i]);
+      d[i] = f32x2_pack(v, v);
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) add_bias(k, i);
+    return;
+  }
+  if (start < -kTile) base += 1, start += t.frame;  // (frame > 128)
+  const float magic = 12582912.0f, inv = 1.0f / static_cast<float>(t.frame);
+  const uint64_t step = f32x2_pack(8.0f, 8.0f), m2 = f32x2_pack(magic, magic), inv2 = f32x2_pack(inv, inv);
+  const float x0 = static_cast<float>(c0 - start) + 0.5f;
+  uint64_t x = f32x2_pack(x0, x0 + 1.0f), rel[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float v = static_cast<float>(base - frame[i]);
+    rel[i] = f32x2_pack(v, v);
+  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    uint64_t f;
+    asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(f) : "l"(x), "l"(inv2), "l"(m2));
+    f = f32x2_sub(f, m2);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      d[i] = f32x2_add(f, rel[i]);
+      add_bias(k, i);
+    }
+    x = f32x2_add(x, step);
+  }
+}
+
+// kFixed (capped scores without a bias, bf16, cap log2(e) <= kFixedCap): every score lies in
+// [-cap, cap], so the exponent's reference is the constant cap log2(e) - kFixedTop instead
+// of the row's maximum: probabilities lie in [2^(kFixedTop - 2 kFixedCap), 2^kFixedTop], inside
+// bf16's and F32's normal range, and no maximum, exchange or rescaling is needed.
+template <bool kF16, bool kCap, bool kBias, bool kFixed>
 __global__ void __launch_bounds__(kThreads, 2)
     masked_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ MaskedArgs a, int* err) {
@@ -328,6 +437,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   const Geom g = make_geom(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Warp 0 sets up the barriers and sends the first loads off while warp 1 waits for TMEM; the
+  // other warps meet them at the CTA-wide barrier.
   if (threadIdx.x == 0) {
     mbar_init(c.q_full(), 1);
     for (int s = 0; s < kKStages; ++s) {
@@ -339,17 +450,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(c.v_empty(s), 1);
     }
     mbar_init(c.s_full(), 1);
-    mbar_init(c.s_free(), kSoftmaxThreads);
-    mbar_init(c.p_full(), kSoftmaxThreads);
+    mbar_init(c.s_free(), kSoftmaxThreads / 32);  // one arrival per warp
+    mbar_init(c.p_full(), kSoftmaxThreads / 32);
     mbar_init(c.pv_done(), 1);
     mbar_init(c.o_final(), 1);
     for (int i = 1; i < 7; ++i) *c.misc(i) = 0;
     fence_mbar_init();
-  }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&map_q);
-    tma_prefetch_desc(&map_k);
-    tma_prefetch_desc(&map_v);
+    if (g.n > 0) first_loads(c, g, a, &map_q, &map_k, &map_v);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(c.tmem_slot()), kTmemCols);
@@ -363,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp < kFirstSoftmaxWarp) {
     if (warp == 0) {
-      if (lane == 0) run_producer(c, g, a, &map_q, &map_k, &map_v, err);
+      if (lane == 0) run_producer(c, g, &map_k, &map_v, err);
       __syncwarp();
     } else {
       run_mma<kF16>(c, g, tmem, err);
@@ -381,7 +488,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     const bool warp_live = lane_base < g.rows;
     // The thread's two rows of the tile.
     int limit[2], row[2];
-    float slope[2], fpos[2];
+    int frame[2];
+    float slope[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       row[i] = lane_base + (lane >> 2) + 8 * i;
@@ -390,19 +498,20 @@ __global__ void __launch_bounds__(kThreads, 2)
       const bool live = row[i] < g.rows;
       const int pos = g.it.first + tok;  // key position of the row
       // floor(pos / frame), also below zero
-      const int frame = pos >= 0 ? pos / a.t.frame : -1 - (-1 - pos) / a.t.frame;
+      frame[i] = pos >= 0 ? pos / a.t.frame : -1 - (-1 - pos) / a.t.frame;
       limit[i] = g.it.doc_keys;
       if (a.t.causal) {
-        const int64_t e = (static_cast<int64_t>(frame) + 1) * a.t.frame;
+        const int64_t e = (static_cast<int64_t>(frame[i]) + 1) * a.t.frame;
         limit[i] = static_cast<int>(max(static_cast<int64_t>(0),
                                         min(static_cast<int64_t>(limit[i]), max(e, static_cast<int64_t>(g.it.prefix)))));
       }
       if (!live) limit[i] = 0;
       slope[i] = kBias ? a.slopes[live ? head : 0] : 0.0f;
-      fpos[i] = static_cast<float>(frame);
     }
     const float sl2 = a.t.scale_log2;
-    float m[2] = {-INFINITY, -INFINITY};  // running maxima, log2 domain, may lag by kGrow
+    const float fixed = kFixedTop - a.t.cap_out;
+    // Running maxima, log2 domain, may lag by kGrow (kFixed: the constant reference).
+    float m[2] = {kFixed ? 0.0f : -INFINITY, kFixed ? 0.0f : -INFINITY};
     float l[2] = {0.0f, 0.0f};            // partial sums over the thread's columns
     bool ok = true;
     for (int j = 0; j < g.n; ++j) {
@@ -412,38 +521,27 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (!warp_live) {
         // Rows nobody reads: hand the tile on, P only once PV(j-1) is done, as the live warps
         // do, so that this arrival counts for tile j.
-        mbar_arrive(c.s_free());
+        warp_arrive(c.s_free());
         if (j > 0) {
           ok = mbar_wait(c.pv_done(), (j - 1) & 1, abort_flag, err, kDevTimeoutConsumer);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
-        mbar_arrive(c.p_full());
+        warp_arrive(c.p_full());
         continue;
       }
       tc_fence_after();
       float s[64];  // block k: s[4k], s[4k+1] row 0, columns 8k + c0, +1; s[4k+2], s[4k+3] row 1
       tmem_ld_16x256b_x16(tS, s);
       tc_fence_before();
-      mbar_arrive(c.s_free());  // QK of the next tile may overwrite S
+      warp_arrive(c.s_free());  // QK of the next tile may overwrite S
       const int k0 = (g.t0 + j) * kTile;
       const bool partial = __any_sync(0xffffffffu, min(limit[0], limit[1]) < k0 + kTile);
       if constexpr (kCap) cap_scores(s, a.t, partial);
       if constexpr (kBias) {
-        const float2* ft = reinterpret_cast<const float2*>(a.frame_of + k0 + c0);
-        const uint64_t fp0 = f32x2_pack(-fpos[0], -fpos[0]), fp1 = f32x2_pack(-fpos[1], -fpos[1]);
-        const uint64_t ns0 = f32x2_pack(-slope[0], -slope[0]), ns1 = f32x2_pack(-slope[1], -slope[1]);
-        const uint64_t sc2 = f32x2_pack(sl2, sl2);
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float2 f = __ldg(ft + 4 * k);
-          const uint64_t ff = f32x2_pack(f.x, f.y);
-          const uint64_t d0 = f32x2_add(ff, fp0) & 0x7fffffff7fffffffull, d1 = f32x2_add(ff, fp1) & 0x7fffffff7fffffffull;
-          uint64_t v0 = f32x2_pack(s[4 * k], s[4 * k + 1]), v1 = f32x2_pack(s[4 * k + 2], s[4 * k + 3]);
-          if (!kCap) v0 = f32x2_mul(v0, sc2), v1 = f32x2_mul(v1, sc2);
-          f32x2_unpack(f32x2_fma(d0, ns0, v0), s[4 * k], s[4 * k + 1]);
-          f32x2_unpack(f32x2_fma(d1, ns1, v1), s[4 * k + 2], s[4 * k + 3]);
-        }
+        const bool past = k0 + kTile - 1 <= g.it.first || (a.t.causal && g.it.prefix == 0);
+        const bool ahead = k0 >= g.it.first + g.it.tokens - 1;
+        bias_scores<kCap>(s, a.t, k0, c0, frame, slope, past ? -1 : ahead ? 1 : 0);
       }
       constexpr bool kScaled = kCap || kBias;  // s already in the log2 domain
       if (partial) {
@@ -456,18 +554,21 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (8 * k + e >= lim1) s[4 * k + 2 + e] = -INFINITY;
           }
       }
-      float mx[2];
-      row_maxima(s, mx);
-      bool grow[2];
-      float alpha[2];
+      bool grow[2] = {false, false};
+      float alpha[2] = {1.0f, 1.0f};
       uint64_t neg2[2];
+      float mx[2];
+      if (!kFixed) row_maxima(s, mx);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        if (kFixed) {
+          neg2[i] = f32x2_pack(fixed, fixed);
+          continue;
+        }
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
         if (!kScaled) mx[i] *= sl2;
         grow[i] = mx[i] > m[i] + kGrow;  // m = -inf: as soon as a key is seen
-        alpha[i] = 1.0f;
         if (grow[i]) {
           alpha[i] = ex2(m[i] - mx[i]);
           m[i] = mx[i];
@@ -498,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         tc_fence_after();
       }
       tmem_st_16x128b_x16(tP, pk);
-      if (j > 0 && __any_sync(0xffffffffu, grow[0] || grow[1])) {
+      if (!kFixed && j > 0 && __any_sync(0xffffffffu, grow[0] || grow[1])) {
         float o[32];  // block k: o[4k], o[4k+1] row 0; o[4k+2], o[4k+3] row 1
         tmem_ld_16x256b_x8(tO, o);
         uint32_t w[32];
@@ -513,10 +614,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int i = 0; i < 2; ++i) {
         float u0, u1;
         f32x2_unpack(acc[i], u0, u1);
-        l[i] = l[i] * alpha[i] + (u0 + u1);
+        l[i] = kFixed ? l[i] + (u0 + u1) : l[i] * alpha[i] + (u0 + u1);
       }
       tc_fence_before();
-      mbar_arrive(c.p_full());
+      warp_arrive(c.p_full());
     }
     if (ok && g.n > 0) {
       ok = mbar_wait(c.o_final(), 0, abort_flag, err, kDevTimeoutConsumer);
@@ -573,16 +674,30 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t part = c.base + Smem::kPart, ml = c.base + Smem::kMl;
       for (int i = static_cast<int>(threadIdx.x) - 32 * kFirstSoftmaxWarp; i < (r1 - r0) * 16; i += kSoftmaxThreads) {
         const int r = r0 + (i >> 4), ch = i & 15;
-        float mt = -INFINITY;
-        for (int p = 0; p < a.splits; ++p) mt = fmaxf(mt, ld_cluster_v2(cluster_addr(ml + r * 8, p)).x);
+        // Every CTA's (maximum, sum) of the row, then its chunk: each batch of remote loads is
+        // issued before the first is used.
+        float2 q[kMaxSplits];
+        float mt = -INFINITY, lt = 0.0f;
+#pragma unroll
+        for (int p = 0; p < kMaxSplits; ++p)
+          if (p < a.splits) q[p] = ld_cluster_v2(cluster_addr(ml + r * 8, p));
+#pragma unroll
+        for (int p = 0; p < kMaxSplits; ++p)
+          if (p < a.splits) mt = fmaxf(mt, q[p].x);
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        float lt = 0.0f;
-        for (int p = 0; p < a.splits; ++p) {
-          const float2 q = ld_cluster_v2(cluster_addr(ml + r * 8, p));
-          const float f = q.x == -INFINITY ? 0.0f : ex2(q.x - mt);
-          const float4 v = ld_cluster_v4(cluster_addr(part + r * 256 + ((ch ^ (r & 15)) << 4), p));
-          sum.x += f * v.x, sum.y += f * v.y, sum.z += f * v.z, sum.w += f * v.w;
-          lt += f * q.y;
+#pragma unroll
+        for (int p0 = 0; p0 < kMaxSplits; p0 += 4) {
+          float4 v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (p0 + e < a.splits) v[e] = ld_cluster_v4(cluster_addr(part + r * 256 + ((ch ^ (r & 15)) << 4), p0 + e));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (p0 + e < a.splits) {
+              const float f = q[p0 + e].x == -INFINITY ? 0.0f : ex2(q[p0 + e].x - mt);
+              sum.x += f * v[e].x, sum.y += f * v[e].y, sum.z += f * v[e].z, sum.w += f * v[e].w;
+              lt += f * q[p0 + e].y;
+            }
         }
         const float inv = 1.0f / lt;
         if (lt == 0.0f) sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -615,10 +730,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-template <bool kF16, bool kCap, bool kBias>
+template <bool kF16, bool kCap, bool kBias, bool kFixed = false>
 cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const MaskedArgs& a,
                    int64_t blocks, int* err, cudaStream_t st) {
-  auto kern = masked_attn_kernel<kF16, kCap, kBias>;
+  auto kern = masked_attn_kernel<kF16, kCap, kBias, kFixed>;
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), Smem::kLaunchBytes, ready);
   if (e != cudaSuccess) return e;
@@ -637,40 +752,72 @@ cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
   return cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, a, err);
 }
 
+// Time model of a launch, in key tiles of a CTA that has its SM alone (1.13 us plain, 1.5 us with a
+// cap or a bias): two CTAs on one SM run at kShared of that each (measured 1.56 and 2.0 us),
+// a CTA pays kFixed (barriers, TMEM, first loads, output) and a split one kJoin more.  CTAs go to
+// the first free slot in grid order.
+constexpr double kShared = 0.725, kFixed = 2.7, kJoin = 2.0;
+double masked_time(const int* key_tiles, int64_t items, int kv_heads, int sms, int splits) {
+  struct Sm {
+    double now = 0.0, left[2] = {0.0, 0.0};  // work left in its two slots
+    double next() const {                    // when one of them is free
+      const bool two = left[0] > 0.0 && left[1] > 0.0;
+      const double w = two ? std::min(left[0], left[1]) / kShared : std::max(left[0], left[1]);
+      return now + w;
+    }
+    void advance(double t) {
+      const double done = (t - now) * (left[0] > 0.0 && left[1] > 0.0 ? kShared : 1.0);
+      for (double& x : left) x = x - done > 1e-9 ? x - done : 0.0;
+      now = t;
+    }
+  };
+  std::vector<Sm> sm(sms);
+  using Entry = std::pair<double, int>;
+  std::priority_queue<Entry, std::vector<Entry>, std::greater<Entry>> busy;
+  int64_t placed = 0;
+  double end = 0.0;
+  for (int64_t i = 0; i < items; ++i) {
+    const double cost = static_cast<double>((key_tiles[i] + splits - 1) / splits) + kFixed + (splits > 1 ? kJoin : 0.0);
+    for (int h = 0; h < kv_heads * splits; ++h, ++placed) {
+      if (placed < 2 * sms) {  // the first CTAs: one on every SM, then a second
+        sm[placed % sms].left[placed / sms] = cost;
+        if (placed == 2 * sms - 1)
+          for (int m = 0; m < sms; ++m) busy.push({sm[m].next(), m});
+        continue;
+      }
+      const Entry e = busy.top();
+      busy.pop();
+      Sm& x = sm[e.second];
+      x.advance(e.first);
+      x.left[x.left[0] > 0.0 ? 1 : 0] = cost;
+      busy.push({x.next(), e.second});
+    }
+  }
+  for (Sm& x : sm)
+    while (x.left[0] > 0.0 || x.left[1] > 0.0) {
+      x.advance(x.next());
+      end = std::max(end, x.now);
+    }
+  return end;
+}
+
 }  // namespace
 
-// Time model of a launch in key-tile units: a CTA costs its key tiles plus kFixed (setup, first
-// loads, output), a split one kJoin more; CTAs go to 2 x sms slots in grid order.
 int masked_splits(const int* key_tiles, int64_t items, int kv_heads, int sms) {
-  constexpr double kFixed = 4.0, kJoin = 2.0;
-  const int slots = 2 * sms;
-  int most = 0;
-  double total = 0.0;
-  for (int64_t i = 0; i < items; ++i) {
-    most = std::max(most, key_tiles[i]);
-    total += key_tiles[i];
-  }
   // Work for many rounds: cutting it finer gains nothing that the order does not give.
-  if (items * kv_heads >= 16 * static_cast<int64_t>(slots)) return 1;
+  if (items == 0 || items * kv_heads >= 16 * static_cast<int64_t>(sms)) return 1;
   int best = 1;
-  double best_time = 0.0;
-  for (int s = 1; s <= kMaxSplits; s *= 2) {
-    if (s > 1 && 2 * s > most) break;  // at least two tiles a CTA in the longest item
-    std::priority_queue<double, std::vector<double>, std::greater<double>> free_at;
-    for (int i = 0; i < slots; ++i) free_at.push(0.0);
-    double end = 0.0;
-    for (int64_t i = 0; i < items; ++i) {
-      const double cost = static_cast<double>((key_tiles[i] + s - 1) / s) + kFixed + (s > 1 ? kJoin : 0.0);
-      for (int h = 0; h < kv_heads * s; ++h) {
-        const double t = free_at.top() + cost;
-        free_at.pop();
-        free_at.push(t);
-        end = std::max(end, t);
-      }
-    }
-    if (s == 1 || end < 0.97 * best_time) {
+  double best_time = masked_time(key_tiles, items, kv_heads, sms, 1);
+  int64_t tiles = 0;
+  for (int64_t i = 0; i < items; ++i) tiles += key_tiles[i];
+  for (int s = 2; s <= kMaxSplits && s <= key_tiles[0]; ++s) {  // key_tiles[0]: the most
+    // No launch of so much work ends sooner, and a finer cut only adds to it.
+    const double bound = kv_heads * (tiles + items * s * (kFixed + kJoin)) / (2.0 * kShared * sms);
+    if (bound >= 0.97 * best_time) break;
+    const double t = masked_time(key_tiles, items, kv_heads, sms, s);
+    if (t < 0.97 * best_time) {
       best = s;
-      best_time = end;
+      best_time = t;
     }
   }
   return best;
@@ -695,6 +842,7 @@ cudaError_t launch_masked(const HeadsRef& q, const HeadsRef& k, const HeadsRef& 
   static const Fn fn[2][2][2] = {
       {{launch<false, false, false>, launch<false, false, true>}, {launch<false, true, false>, launch<false, true, true>}},
       {{launch<true, false, false>, launch<true, false, true>}, {launch<true, true, false>, launch<true, true, true>}}};
+  if (!f16 && cap && !bias && a.t.cap_out <= kFixedCap) return launch<false, true, false, true>(mq, mk, mv, a, blocks, err, st);
   return fn[f16][cap][bias](mq, mk, mv, a, blocks, err, st);
 }
 

@@ -23,7 +23,7 @@ namespace va {
 namespace {
 
 constexpr int kMaxThreads = 256;
-constexpr int kRows = 8;
+constexpr int kRows = 4;  // 2 / 8 / 16 rows: 16.9 / 19.6 / 20.5 us at 10,392 bf16 rows of 24 heads, against 15.0
 
 template <class T>
 __device__ __forceinline__ float to_f32(T x);
@@ -96,10 +96,10 @@ __global__ void __launch_bounds__(kMaxThreads) rope_axes_kernel(const __grid_con
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       if (r < rows) {
-        const float2* t = cs + r * a.pairs + pair;
+        const Vec<float2, (V > 1 ? 2 : 1)>* t = reinterpret_cast<const Vec<float2, (V > 1 ? 2 : 1)>*>(cs + r * a.pairs + pair);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float2 w = t[e];
+          const float2 w = V > 1 ? t[e >> 1].v[e & (V > 1)] : t[e].v[0];
           T& lo = x[r][0].v[kInter ? 2 * e : e];
           T& hi = kInter ? x[r][0].v[2 * e + 1] : x[r][kVecs - 1].v[e];
           const float p0 = to_f32(lo), p1 = to_f32(hi);

@@ -18,7 +18,6 @@ struct va_attn_plan {
   std::vector<va::MaskedItem> items;
   va::MaskedItem* dev_items = nullptr;
   float* dev_slopes = nullptr;
-  float* dev_frames = nullptr;
 };
 
 namespace {
@@ -168,11 +167,10 @@ const char* build_plan(const va_attn_terms* t, int documents, const int64_t* qo,
 
 void free_plan(va_attn_plan* p) {
   if (!p) return;
-  if (p->dev_items || p->dev_slopes || p->dev_frames) {
+  if (p->dev_items || p->dev_slopes) {
     DeviceScope scope(p->device);
     cudaFree(p->dev_items);
     cudaFree(p->dev_slopes);
-    cudaFree(p->dev_frames);
   }
   delete p;
 }
@@ -363,14 +361,7 @@ int va_attn_plan_create(va_ctx* c, const va_attn_terms* terms, int documents, co
     DeviceScope scope(core.device);
     cudaError_t e = scope.error();
     if (e == cudaSuccess && !p->items.empty()) e = upload(&p->dev_items, p->items.data(), p->items.size());
-    if (e == cudaSuccess && slopes) {
-      int most = 0;
-      for (const va::MaskedItem& it : p->items) most = std::max(most, it.keys);
-      std::vector<float> f((static_cast<size_t>(most) + 127) / 128 * 128 + 128);
-      for (size_t i = 0; i < f.size(); ++i) f[i] = static_cast<float>(i / static_cast<size_t>(terms->frame));
-      e = upload(&p->dev_slopes, s.data(), s.size());
-      if (e == cudaSuccess) e = upload(&p->dev_frames, f.data(), f.size());
-    }
+    if (e == cudaSuccess && slopes) e = upload(&p->dev_slopes, s.data(), s.size());
     if (e != cudaSuccess) {
       free_plan(p);
       return launched(c, e, "attention plan upload");
@@ -417,7 +408,6 @@ int va_masked_attention_device(va_ctx* c, const va_attn_plan* p, const va_heads*
   a.splits = p->splits;
   a.item = p->dev_items;
   a.slopes = p->dev_slopes;
-  a.frame_of = p->dev_frames;
   a.out = ref(out);
   DeviceScope scope(core.device);
   if (scope.error() != cudaSuccess) return launched(c, scope.error(), "attention device");
