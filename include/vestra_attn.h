@@ -434,7 +434,8 @@ int va_attn_plan_shape(const va_attn_terms* terms, int documents, const int64_t*
 /* q, out: [.., heads]; k, v: [.., kv_heads]; all BF16 or all F16; data 16-byte
  * aligned, strides multiples of 8 elements, heads not overlapping.  Only rows of the
  * plan's documents are read or written, but a document's own key and value rows must be
- * finite: a NaN or infinity in one may reach rows that do not see it.  out may be q. */
+ * finite: a NaN or infinity in one may reach rows that do not see it; with BF16 and a
+ * score_cap up to 50 values stay below 2^79 (larger ones may overflow).  out may be q. */
 int va_masked_attention_device(va_ctx* ctx, const va_attn_plan* plan, const va_heads* q, const va_heads* k,
                                const va_heads* v, const va_heads* out, void* stream);
 
@@ -450,7 +451,7 @@ int va_masked_attention_device(va_ctx* ctx, const va_attn_plan* plan, const va_h
 typedef struct va_kv_cache {
   int32_t documents;
   int32_t kv_heads;
-  int64_t capacity; /* tokens per document, below 2^31 */
+  int64_t capacity; /* tokens per document, at most 2^30 */
   int32_t format;
   int32_t reserved; /* 0 */
   void* k_codes;
@@ -460,11 +461,11 @@ typedef struct va_kv_cache {
 } va_kv_cache;
 /* Appends: rows [offsets[b], offsets[b+1]) of k and v become tokens [lens[b] - n,
  * lens[b]) of document b, n = offsets[b+1] - offsets[b]; lens = tokens held after the
- * call.  offsets int32 [documents + 1] and lens int32 [documents] are device arrays,
+ * call (a document without rows is left alone, its lens not looked at beyond the check).  offsets int32 [documents + 1] and lens int32 [documents] are device arrays,
  * read when the kernel runs (a captured call follows their contents).  rows = rows of
  * k and v; rows outside every document are not read.  A document with lens[b] - n < 0, lens[b] >
  * capacity, or offsets out of [0, rows] or descending is skipped and reported by
- * va_check_device (VA_ERR_DEVICE).  k, v [rows, kv_heads] of one type. */
+ * va_check_device (VA_ERR_DEVICE); where offsets descend, others may be skipped too.  k, v [rows, kv_heads] of one type. */
 int va_kv_cache_write_device(va_ctx* ctx, const va_kv_cache* cache, int64_t rows, const int32_t* offsets,
                              const int32_t* lens, const va_heads* k, const va_heads* v, void* stream);
 /* Reads back: rows [offsets[b], offsets[b+1]) of k and v receive tokens first[b].. of
@@ -480,7 +481,8 @@ int va_kv_cache_read_device(va_ctx* ctx, const va_kv_cache* cache, int64_t rows,
  * are served too, more slowly).  q, out [rows, heads] BF16 or F16, 16-byte aligned,
  * strides multiples of 8 elements.  Bad offsets, or lens outside [0, capacity]: as
  * above, and the document's rows of out are left as they were.  For many new tokens
- * read the cache back and run va_masked_attention_device. */
+ * read the cache back and run va_masked_attention_device.  The codes of the tokens held
+ * must not be e4m3's NaN (writing never makes one). */
 int va_cache_attention_device(va_ctx* ctx, const va_kv_cache* cache, const va_attn_terms* terms, int64_t rows,
                               const int32_t* offsets, const int32_t* lens, int max_tokens, const int32_t* prefix,
                               const float* slopes, const va_heads* q, const va_heads* out, void* stream);

@@ -223,6 +223,24 @@ def test_masked_cap_over_its_whole_range(ctx, cap):
     run_masked(ctx, [200], [333], 2, 2, F16, cap=cap, gain=0.01, seed=4)
 
 
+@pytest.mark.parametrize("cap,gain", [(50.0, 1.5), (50.0, 60.0), (30.0, 8.0), (2.0, 1.5), (60.0, 30.0)])
+def test_masked_cap_with_many_keys(ctx, cap, gain):
+    """Rows that all see many keys (a constant exponent reference up to cap 50), scores from
+    ordinary to saturated at both ends of the cap; one document, two, and split keys."""
+    run_masked(ctx, [150], [1500], 2, 2, BF16, cap=cap, gain=gain, seed=11)
+    run_masked(ctx, [70, 300], [1100, 2000], 4, 2, BF16, cap=cap, gain=gain, seed=12)
+    # every key scores -cap: the smallest probabilities the reference allows
+    g = gen(13)
+    q = torch.ones(3, 1, D, device="cuda", dtype=BF16) * 30
+    k = -torch.ones(1300, 1, D, device="cuda", dtype=BF16) * 30
+    v = randn(g, 1300, 1, D, dtype=BF16)
+    out = torch.empty_like(q)
+    ctx.masked_attention(va.AttentionPlan(ctx, 1, 1, [0, 3], [0, 1300], score_cap=cap), q, k, v, out)
+    check_attention(out, *attention_ref(q, k, v, False, 1, 0, None, cap))
+    ctx.masked_attention(va.AttentionPlan(ctx, 1, 1, [0, 3], [0, 1300], score_cap=cap), q, -k, v, out)
+    check_attention(out, *attention_ref(q, -k, v, False, 1, 0, None, cap))
+
+
 def test_masked_scale_and_growing_scores(ctx):
     run_masked(ctx, [140], [900], 2, 1, BF16, scale=1.0, seed=5)   # near one-hot rows
     run_masked(ctx, [140], [900], 2, 1, F16, scale=0.001, seed=6)  # flat rows

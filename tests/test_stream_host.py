@@ -14,7 +14,7 @@ def shape(q_lens, k_lens, heads=12, kv_heads=12, **kw):
 
 def test_structures_match_the_header():
     """Sizes of the C structures on this ABI (LP64)."""
-    assert ctypes.sizeof(va.VaHeads) == 32
+    assert len(va._PACK_HEADS(1, 2, 3, 4, 0)) == 32
     assert ctypes.sizeof(va.VaRopeAxes) == 32
     assert ctypes.sizeof(va.VaAttnTerms) == 24
     assert ctypes.sizeof(va.VaKvCache) == 56

@@ -369,6 +369,7 @@ struct MaskedItem {
 struct MaskedArgs {
   AttnTerms t;
   int group, tile_tokens, items, splits;
+  int fewest_keys;          // keys the row that sees fewest sees
   const MaskedItem* item;
   const float* slopes;      // [heads] device, times log2(e); nullptr: no bias
   HeadsRef out;

@@ -14,6 +14,7 @@ struct va_attn_plan {
   int device = 0;
   va::AttnTerms terms{};
   int group = 1, tile_tokens = 1, splits = 1;
+  int fewest_keys = 0x7fffffff;
   int64_t q_rows = 0, k_rows = 0;  // rows the documents reach to
   std::vector<va::MaskedItem> items;
   va::MaskedItem* dev_items = nullptr;
@@ -24,6 +25,7 @@ namespace {
 
 constexpr double kLog2e = 1.4426950408889634;
 constexpr int64_t kMaxRows = 0x7fffffff;
+constexpr int64_t kMaxCapacity = int64_t(1) << 30;  // chunk arithmetic stays in 32 bits
 constexpr int64_t kMaxDocKeys = int64_t(1) << 24;  // frame indices stay exact in F32
 
 // Makes the context's device current for one call and puts the caller's back.
@@ -145,12 +147,14 @@ const char* build_plan(const va_attn_terms* t, int documents, const int64_t* qo,
       it.first = static_cast<int>(i + lk - lq);
       it.doc_keys = static_cast<int>(lk);
       it.prefix = static_cast<int>(std::min(pre, lk));
-      it.keys = it.doc_keys;
-      if (t->causal) {
-        const int64_t last = static_cast<int64_t>(it.first) + it.tokens - 1;
-        const int64_t e = (floor_div(last, t->frame) + 1) * t->frame;
-        it.keys = static_cast<int>(std::max<int64_t>(0, std::min<int64_t>(lk, std::max<int64_t>(e, it.prefix))));
-      }
+      // Keys the row at a position sees; the tile's last row sees most, its first fewest.
+      auto limit = [&](int64_t at) {
+        if (!t->causal) return it.doc_keys;
+        const int64_t e = (floor_div(at, t->frame) + 1) * t->frame;
+        return static_cast<int>(std::max<int64_t>(0, std::min<int64_t>(lk, std::max<int64_t>(e, it.prefix))));
+      };
+      it.keys = limit(static_cast<int64_t>(it.first) + it.tokens - 1);
+      p->fewest_keys = std::min(p->fewest_keys, limit(it.first));
       p->items.push_back(it);
     }
   }
@@ -184,8 +188,8 @@ cudaError_t upload(T** dst, const T* src, size_t n) {
 
 const char* check_cache(const va_kv_cache* c) {
   if (!c) return "the cache is missing";
-  if (c->documents < 1 || c->kv_heads < 1 || c->kv_heads > 128 || c->capacity < 1 || c->capacity > kMaxRows)
-    return "cache needs documents >= 1, kv_heads 1..128 and capacity 1..2^31 - 1";
+  if (c->documents < 1 || c->kv_heads < 1 || c->kv_heads > 128 || c->capacity < 1 || c->capacity > kMaxCapacity)
+    return "cache needs documents >= 1, kv_heads 1..128 and capacity 1..2^30";
   if (c->format != VA_KV_INT8 && c->format != VA_KV_E4M3) return "unknown cache format";
   if (c->reserved != 0) return "reserved must be 0";
   for (const void* p : {static_cast<const void*>(c->k_codes), static_cast<const void*>(c->v_codes),
@@ -406,6 +410,7 @@ int va_masked_attention_device(va_ctx* c, const va_attn_plan* p, const va_heads*
   a.tile_tokens = p->tile_tokens;
   a.items = static_cast<int>(p->items.size());
   a.splits = p->splits;
+  a.fewest_keys = p->fewest_keys;
   a.item = p->dev_items;
   a.slopes = p->dev_slopes;
   a.out = ref(out);

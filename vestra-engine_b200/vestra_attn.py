@@ -105,13 +105,6 @@ _lib = None
 _vp = ctypes.c_void_p
 _f32p = ctypes.POINTER(ctypes.c_float)
 
-class VaHeads(ctypes.Structure):
-    """va_heads: a token-major [rows, heads, channels] operand with element strides."""
-
-    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
-                ("heads", ctypes.c_int32), ("dtype", ctypes.c_int32)]
-
-
 class VaRopeAxes(ctypes.Structure):
     _fields_ = [("axes", ctypes.c_int32), ("section", ctypes.c_int32 * 4), ("layout", ctypes.c_int32),
                 ("pairing", ctypes.c_int32), ("base", ctypes.c_float)]
