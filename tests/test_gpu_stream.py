@@ -256,6 +256,30 @@ def test_masked_scale_and_growing_scores(ctx):
         check_attention(out, *attention_ref(q, k, v, False, 1, 0, None, 0.0))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kvh", [(2, 2), (8, 1), (16, 2), (3, 3), (10, 2)])
+@pytest.mark.parametrize("causal,frame,prefix,bias,cap", [(True, 1, None, False, 0.0), (True, 5, [3, 0, 900, 0, 1], True, 30.0),
+                                                          (False, 1, None, True, 0.0), (False, 64, None, False, 50.0)])
+def test_masked_few_rows(ctx, dtype, heads, kvh, causal, frame, prefix, bias, cap):
+    """Every tile holds at most 16 rows (single tokens and their shared heads), long and short
+    documents, more rows than keys, no keys; strided operands; keys cut over a cluster."""
+    per = max(1, 16 * kvh // heads)
+    ql = [1, per, 1, min(2, per), per]
+    kl = [4097, 1, 1000, 0, 33]
+    run_masked(ctx, ql, kl, heads, kvh, dtype, causal, frame, prefix, bias, cap, seed=heads)
+    g = gen(21)
+    packed = randn(g, 300, heads + 2 * kvh, D, dtype=dtype)
+    q, k, v = packed[:, :heads], packed[:, heads:heads + kvh], packed[:, heads + kvh:]
+    k[290:] = float("nan")  # past the documents
+    v[290:] = float("inf")
+    plan = va.AttentionPlan(ctx, heads, kvh, [5, 6, 6 + per], [9, 200, 290], causal=True)
+    out = torch.full((heads, 300, D), 7.0, device="cuda", dtype=dtype).transpose(0, 1)
+    ctx.masked_attention(plan, q, k, v, out)
+    for ql0, ql1, kl0, kl1 in ((5, 6, 9, 200), (6, 6 + per, 200, 290)):
+        check_attention(out[ql0:ql1], *attention_ref(q[ql0:ql1], k[kl0:kl1], v[kl0:kl1], True, 1, 0, None, 0.0))
+    assert (out[:5] == 7).all() and (out[6 + per:] == 7).all()
+
+
 def test_masked_split_tiles_match_the_definition(ctx):
     """Few tiles: the keys of one tile are cut over a cluster; some CTAs get no key."""
     for n, m, heads, kvh, causal in ((1, 10392, 12, 12, True), (3, 5000, 8, 2, True), (129, 4000, 2, 2, False),

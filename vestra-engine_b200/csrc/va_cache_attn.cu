@@ -6,11 +6,9 @@
 // multiplies its scores, a value's scale its probability, so codes are never scaled.
 //
 // Bound by HBM: every visible key costs 2 * (64 + 4) bytes per key head and 256 FLOP per
-// query row.  A row block is 8 query rows of one key head (tokens x the heads that share
-// it), so the products are m16n8k16 tensor-core instructions (mma.sync: the tcgen05 tile
-// of 128 rows would be 94 % padding, and the operands come from registers): rows 0..7
-// hold the high f16 part of the row, rows 8..15 the rest, which makes the products good to
-// 2^-21 of the row's largest element at no further product.  f16 because both code formats
+// query row.  The fragments, and the joining of warps and cluster, are va_rows.cuh's: the rest of a
+// split operand costs no further product and makes products good to 2^-21 of the row's
+// largest element.  The operands are f16 because both code formats
 // become f16 in one or two instructions a pair (bf16 took four or five, and the conversions
 // are most of the loop).  Its range is met by powers of two: a query row is scaled to a
 // largest magnitude in [1, 2) and the factor goes to the scores; a probability times its
@@ -21,33 +19,25 @@
 // warp with its own running maximum and sum, and the partial results meet in shared memory
 // and then, through distributed shared memory, across the cluster in rank order: one
 // launch, no workspace, no atomics, and the same bits on every run.
-//
-// Operand layout: the channel order inside a product is free as long as both operands
-// use the same, so lane (g, c) = (lane / 4, lane % 4) loads 16 consecutive code bytes
-// [16c, 16c + 16) of one key of an 8-key tile, and its word s holds the lane's k indices of
-// step s; the query row is loaded with the same order.  For the second product the key order is free: lane (g, c) loads channels [8g, 8g + 8)
-// of the four keys whose probabilities it holds.
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "va_internal.h"
 #include "va_ptx.cuh"
+#include "va_rows.cuh"
 
 namespace va {
 
 namespace {
 
-constexpr int kHeadDim = 64;
+using namespace rows;
+
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRowsPerBlock = 8;
 constexpr int kChunk = 64;         // keys a warp takes at a time
 constexpr int kTiles = kChunk / 8;
 constexpr int kStages = 2;         // chunks of a warp in shared memory
 constexpr int kCtasPerSm = 3;
-constexpr int kMaxCluster = 16;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTop = 14;       // probabilities times value scales are brought below 2^kTop
 constexpr int kMinExp = -100;  // value scales below 2^-100 lose precision
 
@@ -64,32 +54,6 @@ struct CacheAttnArgs {
   const float* slopes;
   HeadsRef q, out;
 };
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-  return r;
-}
 
 // Two code bytes of w -> f16x2, exactly.  kHigh: bytes 2 and 3, else 0 and 1.  int8 codes come
 // with their sign bits flipped (flip): u = c + 128 under 0x64 is the f16 1024 + u.
@@ -108,45 +72,14 @@ __device__ __forceinline__ uint32_t codes_to_f16x2(uint32_t w) {
   return r;
 }
 
-// x in two f16 parts, packed with a neighbour's: hi = f16(x), lo = f16(x - hi).
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  hi = f16x2_from_f32(x0, x1);
-  const float2 h = __half22float2(*reinterpret_cast<__half2*>(&hi));
-  lo = f16x2_from_f32(x0 - h.x, x1 - h.y);
-}
-
-// floor(p / frame), magic = floor(2^32 / frame).
-__device__ __forceinline__ int frame_index(int p, int frame, uint32_t magic) {
-  if (frame == 1) return p;
-  const uint32_t x = static_cast<uint32_t>(p < 0 ? -1 - p : p);
-  uint32_t q = __umulhi(x, magic);  // x / frame or one less
-  if (x - q * frame >= static_cast<uint32_t>(frame)) ++q;
-  return p < 0 ? -1 - static_cast<int>(q) : static_cast<int>(q);
-}
-
-// A warp's ring of 32-key chunks in shared memory, filled by cp.async (16 bytes of codes, 4 of
+// A warp's ring of chunks in shared memory, filled by cp.async (16 bytes of codes, 4 of
 // scales a copy: no alignment beyond the cache's own).  Code rows of 64 bytes; the
-// 16-byte piece p of row r lies at piece p ^ (2 bit2(r)).  Column n of an 8-key tile is key n ^ bit1(n):
-// with that order a warp's 16-byte key loads and 8-byte value loads meet no bank twice.
+// 16-byte piece p of row r lies at piece p ^ (2 bit2(r)).
 struct Chunk {
   uint8_t k[kChunk][kHeadDim];
   uint8_t v[kChunk][kHeadDim];
   float ks[kChunk], vs[kChunk];
 };
-__device__ __forceinline__ int tile_key(int n) { return n ^ ((n >> 1) & 1); }
-
-__device__ __forceinline__ void cp16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Rows past `last` repeat it (they are hidden, and the codes of any row held are finite).
 __device__ __forceinline__ void load_chunk(Chunk& ch, const uint8_t* kc, const uint8_t* vc, const float* ks,
                                            const float* vs, int key0, int last, int lane) {
@@ -180,72 +113,21 @@ __device__ __forceinline__ void load_chunk(Chunk& ch, const uint8_t* kc, const u
   }
 }
 
-// The warps' results of a row block.  Channel ch of a row lies at slot(ch): the order in which
-// a lane's accumulators are neighbours; rows are padded against bank conflicts.
-__device__ __forceinline__ int slot(int ch) { return (ch & 7) * 8 + (ch >> 3); }
-struct Join {
-  float o[kWarps][kRowsPerBlock][kHeadDim + 8];
-  float m[kWarps][kRowsPerBlock], l[kWarps][kRowsPerBlock];
-};
-// What the cluster's CTAs send to the CTA that finishes a row: rows r, r + splits, ... go to
-// CTA r % splits, so a CTA receives at most 16 (splits x rows) parts.
-struct Part {
-  float o[kHeadDim];
-  float m, l;
-};
 struct Shared {
   union {
     Chunk ring[kWarps][kStages];
-    Join join;  // once the block's last chunk is used
+    Join<kWarps> join;  // once the block's last chunk is used
   };
   Part part[kMaxCluster];  // [own row][cluster rank]
 };
 static_assert(kCtasPerSm * (sizeof(Shared) + 1024) <= 228 * 1024, "shared memory of an SM");
-
-// Stores v at this address of CTA `rank` of the cluster.
-__device__ __forceinline__ void st_cluster(float* p, int rank, float v) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
-}
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
-// 16 consecutive two-byte elements.
-struct RawRow {
-  uint4 u[2];
-};
-__device__ __forceinline__ void load_row(RawRow& r, const void* p) {
-  r.u[0] = __ldg(static_cast<const uint4*>(p));
-  r.u[1] = __ldg(static_cast<const uint4*>(p) + 1);
-}
-template <class T>
-__device__ __forceinline__ void unpack_row(const RawRow& r, float* x) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t w[4] = {r.u[h].x, r.u[h].y, r.u[h].z, r.u[h].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __half>::value) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        x[8 * h + 2 * i] = f.x;
-        x[8 * h + 2 * i + 1] = f.y;
-      } else {
-        x[8 * h + 2 * i] = __uint_as_float(w[i] << 16);
-        x[8 * h + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    }
-  }
-}
-__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
-__device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x); }
 
 template <class T, bool kE4m3>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     cache_attn_kernel(const __grid_constant__ CacheAttnArgs a, int splits, int* err) {
   extern __shared__ uint4 smem_raw[];
   Shared& smem = *reinterpret_cast<Shared*>(smem_raw);
-  Join& sh = smem.join;
+  Join<kWarps>& sh = smem.join;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int rank = static_cast<int>(blockIdx.x) % splits;
@@ -271,7 +153,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const float* ks = a.c.scales[0] + head_base;
   const float* vs = a.c.scales[1] + head_base;
   const T* qd = static_cast<const T*>(a.q.data);
-  T* od = static_cast<T*>(a.out.data);
 
   // Keys a token sees: the first `limit` of the document.
   auto limit_of = [&](int token) {
@@ -329,8 +210,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const float inv = __uint_as_float((254u - ex) << 23);
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        split2(x[4 * s] * inv, x[4 * s + 1] * inv, qa[s][0], qa[s][1]);
-        split2(x[4 * s + 2] * inv, x[4 * s + 3] * inv, qa[s][2], qa[s][3]);
+        split2(__half(), x[4 * s] * inv, x[4 * s + 1] * inv, qa[s][0], qa[s][1]);
+        split2(__half(), x[4 * s + 2] * inv, x[4 * s + 3] * inv, qa[s][2], qa[s][3]);
       }
     }
     const float score_scale = q_scale * a.t.scale_log2, cap_scale = q_scale * a.t.cap_in;
@@ -356,7 +237,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const Chunk& cur = ring[stage];
       stage = stage + 1 == kStages ? 0 : stage + 1;
       const int key0 = ch * kChunk;
-      const float ahead = static_cast<float>(fp - key0);  // tokens (frame 1) past the chunk's first
       // Scores of 8 rows x 32 keys: lane (g, c) gets row g, columns 2c and 2c + 1 of each tile.
       float x[kTiles][2], d[kTiles][4];
       uint32_t w[kTiles][4];
@@ -373,32 +253,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
-          mma_f16(d[t], qa[s], codes_to_f16x2<kE4m3, false>(w[t][s]), codes_to_f16x2<kE4m3, true>(w[t][s]));
-      // Each term over all eight scores of the lane under one branch, so they overlap.
-#define VA_EACH_SCORE(...)                          \
-  _Pragma("unroll") for (int t = 0; t < kTiles; ++t) { \
-    _Pragma("unroll") for (int e = 0; e < 2; ++e) { \
-      const int kk = 8 * t + ((2 * c + e) ^ (c & 1)); \
-      __VA_ARGS__                                   \
-    }                                               \
-  }
-      VA_EACH_SCORE(x[t][e] = (d[t][e] + d[t][2 + e]) * cur.ks[kk];)
-      if (a.t.cap_out > 0.0f) {
-        // cap log2(e) tanh(z) = cap log2(e) (1 - 2 / (1 + e^(2z)))
-        VA_EACH_SCORE((void)kk; x[t][e] = fmaf(-2.0f * a.t.cap_out, rcp(1.0f + ex2(x[t][e] * cap_scale)), a.t.cap_out);)
-      } else {
-        VA_EACH_SCORE((void)kk; x[t][e] *= score_scale;)
-      }
-      if (a.slopes) {
-        if (a.t.frame == 1) {
-          VA_EACH_SCORE(x[t][e] = fmaf(-slope, fabsf(ahead - static_cast<float>(kk)), x[t][e]);)
-        } else {
-          VA_EACH_SCORE(const float dist = static_cast<float>(fp - frame_index(key0 + kk, a.t.frame, a.frame_magic));
-                        x[t][e] = fmaf(-slope, fabsf(dist), x[t][e]);)
-        }
-      }
-      VA_EACH_SCORE(x[t][e] = key0 + kk < limit ? x[t][e] : -INFINITY;)
-#undef VA_EACH_SCORE
+          mma(__half(), d[t], qa[s], codes_to_f16x2<kE4m3, false>(w[t][s]), codes_to_f16x2<kE4m3, true>(w[t][s]));
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) x[t][e] = (d[t][e] + d[t][2 + e]) * cur.ks[8 * t + ((2 * c + e) ^ (c & 1))];
+      apply_terms(x, a.t, score_scale, cap_scale, a.slopes != nullptr, slope, fp, key0, limit, c, a.frame_magic);
       float top = x[0][0];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) top = max3f(top, x[t][0], x[t][1]);
@@ -446,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             // A hidden key's value scale may be anything (stale rows): not multiplied.
             w[e] = x[t][e] == -INFINITY ? 0.0f : p * (cur.vs[kk] * v_scale);
           }
-          split2(w[0], w[1], pa[2 * half], pa[2 * half + 1]);
+          split2(__half(), w[0], w[1], pa[2 * half], pa[2 * half + 1]);
         }
 #pragma unroll
         for (int word = 0; word < 2; ++word) {
@@ -455,76 +315,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           const uint32_t b0 = flip<kE4m3>(word ? vw[2].y : vw[2].x), b1 = flip<kE4m3>(word ? vw[3].y : vw[3].x);
           const uint32_t lo0 = prmt(a0, a1, 0x5140), hi0 = prmt(a0, a1, 0x7362);
           const uint32_t lo1 = prmt(b0, b1, 0x5140), hi1 = prmt(b0, b1, 0x7362);
-          mma_f16(o[4 * word + 0], pa, codes_to_f16x2<kE4m3, false>(lo0), codes_to_f16x2<kE4m3, false>(lo1));
-          mma_f16(o[4 * word + 1], pa, codes_to_f16x2<kE4m3, true>(lo0), codes_to_f16x2<kE4m3, true>(lo1));
-          mma_f16(o[4 * word + 2], pa, codes_to_f16x2<kE4m3, false>(hi0), codes_to_f16x2<kE4m3, false>(hi1));
-          mma_f16(o[4 * word + 3], pa, codes_to_f16x2<kE4m3, true>(hi0), codes_to_f16x2<kE4m3, true>(hi1));
+          mma(__half(), o[4 * word + 0], pa, codes_to_f16x2<kE4m3, false>(lo0), codes_to_f16x2<kE4m3, false>(lo1));
+          mma(__half(), o[4 * word + 1], pa, codes_to_f16x2<kE4m3, true>(lo0), codes_to_f16x2<kE4m3, true>(lo1));
+          mma(__half(), o[4 * word + 2], pa, codes_to_f16x2<kE4m3, false>(hi0), codes_to_f16x2<kE4m3, false>(hi1));
+          mma(__half(), o[4 * word + 3], pa, codes_to_f16x2<kE4m3, true>(hi0), codes_to_f16x2<kE4m3, true>(hi1));
         }
       }
     }
     cp_wait<0>();
     __syncthreads();  // every warp is done with its ring: the join buffers may cover it
-    // Row sums over the four lanes of a row; accumulator column 2c + e of tile n is
-    // channel 8 (2c + e) + n (the value operand's column g holds channel 8g + n).
-    const int rows = min(kRowsPerBlock, q_rows - rb * kRowsPerBlock);
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (g < rows) {
-      const float back = __uint_as_float(static_cast<uint32_t>(v_exp - kTop + 127) << 23);  // 2^(E - kTop)
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-        *reinterpret_cast<float2*>(&sh.o[warp][g][8 * n + 2 * c]) =
-            make_float2((o[n][0] + o[n][2]) * back, (o[n][1] + o[n][3]) * back);
-      if (c == 0) {
-        sh.m[warp][g] = m;
-        sh.l[warp][g] = l;
-      }
-    }
-    __syncthreads();
-    if (splits > 1) cluster_wait();
-    // Join the warps and hand each row to the CTA that finishes it.
-    for (int i = threadIdx.x; i < rows * kHeadDim; i += kThreads) {
-      const int row = i / kHeadDim, at = i % kHeadDim;
-      float mt = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, sh.m[w][row]);
-      float os = 0.0f, ls = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = sh.m[w][row] == -INFINITY ? 0.0f : ex2(sh.m[w][row] - mt);
-        os += f * sh.o[w][row][at];
-        ls += f * sh.l[w][row];
-      }
-      const int owner = row % splits;
-      Part& to = smem.part[row / splits * splits + rank];
-      st_cluster(&to.o[at], owner, os);
-      if (at == 0) {
-        st_cluster(&to.m, owner, mt);
-        st_cluster(&to.l, owner, ls);
-      }
-    }
-    if (splits > 1) {
-      cluster_arrive();
-      cluster_wait();
-    } else {
-      __syncthreads();
-    }
-    // This CTA's rows rank, rank + splits, ...: the cluster's parts in rank order.
-    for (int i = threadIdx.x; rank + i / kHeadDim * splits < rows; i += kThreads) {
-      const int own = i / kHeadDim, ch = i % kHeadDim;
-      const Part* part = smem.part + own * splits;
-      float mt = -INFINITY, os = 0.0f, ls = 0.0f;
-      for (int p = 0; p < splits; ++p) mt = fmaxf(mt, part[p].m);
-      for (int p = 0; p < splits; ++p) {
-        const float f = part[p].m == -INFINITY ? 0.0f : ex2(part[p].m - mt);
-        os += f * part[p].o[slot(ch)];
-        ls += f * part[p].l;
-      }
-      const int rr = rb * kRowsPerBlock + rank + own * splits;
-      put(od + (begin + static_cast<int64_t>(rr / a.group)) * a.out.token_stride +
-              static_cast<int64_t>(kvh * a.group + rr % a.group) * a.out.head_stride + ch,
-          ls == 0.0f ? 0.0f : os / ls);
-    }
+    const float back = __uint_as_float(static_cast<uint32_t>(v_exp - kTop + 127) << 23);  // 2^(E - kTop)
+    finish_block<T>(sh, smem.part, o, m, l, back, rb, q_rows, a.group, kvh, rank, splits, begin, a.out);
     __syncthreads();  // before the next block's loads and parts
   }
 }

@@ -336,11 +336,11 @@ struct KvCacheRef {
   float* scales[2];
 };
 cudaError_t launch_kv_write(const KvCacheRef& c, int dtype, int64_t rows, const int32_t* offsets,
-                            const int32_t* lens, const HeadsRef& k, const HeadsRef& v, int* err,
-                            cudaStream_t st);
+                            const int32_t* lens, const HeadsRef& k, const HeadsRef& v, int sms,
+                            int* err, cudaStream_t st);
 cudaError_t launch_kv_read(const KvCacheRef& c, int dtype, int64_t rows, const int32_t* offsets,
-                           const int32_t* first, const HeadsRef& k, const HeadsRef& v, int* err,
-                           cudaStream_t st);
+                           const int32_t* first, const HeadsRef& k, const HeadsRef& v, int sms,
+                           int* err, cudaStream_t st);
 
 // Score terms of the masked and the cache attention.
 struct AttnTerms {
@@ -376,6 +376,12 @@ struct MaskedArgs {
 };
 cudaError_t launch_masked(const HeadsRef& q, const HeadsRef& k, const HeadsRef& v, int64_t q_rows, int64_t k_rows,
                           const MaskedArgs& a, int dtype, int* err, cudaStream_t st);
+// The form for tiles of few query rows (va_rows_attn.cu): whether tiles of at most most_rows rows
+// take it, its CTAs per (tile, key head, row block), and its launch.
+bool rows_form(int most_rows);
+int rows_splits(int64_t units, int most_keys, int sms);
+cudaError_t launch_rows(const HeadsRef& q, const HeadsRef& k, const HeadsRef& v, const MaskedArgs& a, int most_rows,
+                        int dtype, cudaStream_t st);
 // CTAs per query tile for tiles of these key counts (descending) on `sms` SMs.
 int masked_splits(const int* key_tiles, int64_t items, int kv_heads, int sms);
 

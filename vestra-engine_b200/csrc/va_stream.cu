@@ -15,6 +15,7 @@ struct va_attn_plan {
   va::AttnTerms terms{};
   int group = 1, tile_tokens = 1, splits = 1;
   int fewest_keys = 0x7fffffff;
+  int most_rows = 0;  // query rows of the fullest tile
   int64_t q_rows = 0, k_rows = 0;  // rows the documents reach to
   std::vector<va::MaskedItem> items;
   va::MaskedItem* dev_items = nullptr;
@@ -155,6 +156,7 @@ const char* build_plan(const va_attn_terms* t, int documents, const int64_t* qo,
       };
       it.keys = limit(static_cast<int64_t>(it.first) + it.tokens - 1);
       p->fewest_keys = std::min(p->fewest_keys, limit(it.first));
+      p->most_rows = std::max(p->most_rows, it.tokens * p->group);
       p->items.push_back(it);
     }
   }
@@ -163,9 +165,15 @@ const char* build_plan(const va_attn_terms* t, int documents, const int64_t* qo,
   // the tiles that read the same keys run together.
   std::stable_sort(p->items.begin(), p->items.end(),
                    [](const va::MaskedItem& a, const va::MaskedItem& b) { return a.keys > b.keys; });
+  if (p->items.empty()) return nullptr;
+  if (va::rows_form(p->most_rows)) {
+    p->splits = va::rows_splits(static_cast<int64_t>(p->items.size()) * t->kv_heads * ((p->most_rows + 7) / 8),
+                                p->items[0].keys, sms);
+    return nullptr;
+  }
   std::vector<int> tiles(p->items.size());
   for (size_t i = 0; i < tiles.size(); ++i) tiles[i] = (p->items[i].keys + 127) / 128;
-  p->splits = tiles.empty() ? 1 : va::masked_splits(tiles.data(), static_cast<int64_t>(tiles.size()), t->kv_heads, sms);
+  p->splits = va::masked_splits(tiles.data(), static_cast<int64_t>(tiles.size()), t->kv_heads, sms);
   return nullptr;
 }
 
@@ -333,7 +341,7 @@ int va_attn_plan_shape(const va_attn_terms* terms, int documents, const int64_t*
     plan[1] = p.splits;
     plan[2] = p.tile_tokens;
     plan[3] = tiles * terms->kv_heads;
-    plan[4] = plan[0] * p.splits;
+    plan[4] = plan[0] * p.splits * (va::rows_form(p.most_rows) ? (p.most_rows + 7) / 8 : 1);
     return VA_OK;
   } catch (...) {
     return VA_ERR_CAPACITY;
@@ -416,9 +424,11 @@ int va_masked_attention_device(va_ctx* c, const va_attn_plan* p, const va_heads*
   a.out = ref(out);
   DeviceScope scope(core.device);
   if (scope.error() != cudaSuccess) return launched(c, scope.error(), "attention device");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (va::rows_form(p->most_rows))
+    return launched(c, va::launch_rows(ref(q), ref(k), ref(v), a, p->most_rows, q->dtype, st), "masked attention launch");
   return launched(c, va::launch_masked(ref(q), ref(p->k_rows ? k : q), ref(p->k_rows ? v : q), p->q_rows,
-                                       p->k_rows, a, q->dtype, core.err,
-                                       static_cast<cudaStream_t>(stream)),
+                                       p->k_rows, a, q->dtype, core.err, st),
                   "masked attention launch");
 }
 
@@ -431,7 +441,7 @@ int va_kv_cache_write_device(va_ctx* c, const va_kv_cache* cache, int64_t rows, 
   const va::CtxCore core = va::ctx_core(c);
   DeviceScope scope(core.device);
   if (scope.error() != cudaSuccess) return launched(c, scope.error(), "cache device");
-  return launched(c, va::launch_kv_write(cache_ref(cache), k->dtype, rows, offsets, lens, ref(k), ref(v), core.err,
+  return launched(c, va::launch_kv_write(cache_ref(cache), k->dtype, rows, offsets, lens, ref(k), ref(v), core.sms, core.err,
                                          static_cast<cudaStream_t>(stream)),
                   "cache write launch");
 }
@@ -444,7 +454,7 @@ int va_kv_cache_read_device(va_ctx* c, const va_kv_cache* cache, int64_t rows, c
   const va::CtxCore core = va::ctx_core(c);
   DeviceScope scope(core.device);
   if (scope.error() != cudaSuccess) return launched(c, scope.error(), "cache device");
-  return launched(c, va::launch_kv_read(cache_ref(cache), k->dtype, rows, offsets, first, ref(k), ref(v), core.err,
+  return launched(c, va::launch_kv_read(cache_ref(cache), k->dtype, rows, offsets, first, ref(k), ref(v), core.sms, core.err,
                                         static_cast<cudaStream_t>(stream)),
                   "cache read launch");
 }
