@@ -348,8 +348,10 @@ struct AttnTerms {
   float scale_log2;  // scale * log2(e)
   float cap_in;      // 2 * log2(e) * scale / cap: ex2(cap_in * q.k) = e^(2 scale q.k / cap); 0: no cap
   float cap_out;     // cap * log2(e)
-  float cap_range;   // largest |q.k| of the polynomial form (va_masked.cu)
-  float cap_poly[4]; // cap log2(e) tanh(scale x / cap) = x (c0 + c1 x^2 + c2 x^4 + c3 x^6)
+  // cap log2(e) tanh(scale x / cap) = x (c0 + c1 x^2 + ...) for |x| up to cap_range[0] with
+  // cap_poly[0..2], up to cap_range[1] with cap_poly[3..6] (va_masked.cu)
+  float cap_range[2];
+  float cap_poly[7];
 };
 cudaError_t launch_cache_attention(const KvCacheRef& c, const AttnTerms& t, int dtype, int64_t rows,
                                    const int32_t* offsets, const int32_t* lens, int max_tokens,

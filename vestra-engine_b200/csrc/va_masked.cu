@@ -105,6 +105,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
   const unsigned long long t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity)) {
@@ -279,37 +285,55 @@ __device__ __forceinline__ void row_maxima(const float* s, float* mx) {
   }
 }
 
-// s <- cap log2(e) tanh(scale s / cap).  While every |s| of the warp's part of the tile is at most
-// cap_range (a score of 0.6 cap, at most 77) by an odd polynomial on the FMA pipe: tanh(z) =
-// z P(z^2), P cubic, fitted here (reweighted least squares on Chebyshev nodes of z^2 in [0, 0.36],
-// relative error below 2.2e-6, so a capped score is within 1.7e-4).  Else, and where hidden keys
-// may hold anything, cap log2(e) (1 - 2 / (1 + e^(2z))): two MUFU operations a score.
-__device__ __forceinline__ void cap_scores(float* s, const AttnTerms& t, bool partial) {
-  bool wide = partial;
-  if (!partial) {
-    float mx[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+// Scores of the thread's columns (relative to its first) from lim[i] on become v.
+__device__ __forceinline__ void hide(float* s, const int* lim, float v) {
 #pragma unroll
-    for (int q = 0; q < 64; q += 8)
+  for (int k = 0; k < 16; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], fabsf(s[q + 2 * i]), fabsf(s[q + 2 * i + 1]));
-    // a NaN fails no comparison: the polynomial hands it on as well
-    wide = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) > t.cap_range;
-  }
-  if (__any_sync(0xffffffffu, wide)) {
+    for (int e = 0; e < 2; ++e) {
+      if (8 * k + e >= lim[0]) s[4 * k + e] = v;
+      if (8 * k + e >= lim[1]) s[4 * k + 2 + e] = v;
+    }
+}
+
+// s <- cap log2(e) tanh(scale s / cap) + offset.  While every |s| of the warp's part of the tile is at
+// most a range, by an odd polynomial on the FMA pipe: tanh(z) = z P(z^2), fitted here (reweighted
+// least squares on Chebyshev nodes of z^2): P quadratic for |z| <= 0.3 (relative error 1.2e-6),
+// cubic for |z| <= 0.6 (2.2e-6, and scores of at most 77, so within 1.7e-4).  Else
+// cap log2(e) (1 - 2 / (1 + e^(2z))): two MUFU operations a score.
+__device__ __forceinline__ void cap_scores(float* s, const AttnTerms& t, float offset) {
+  float mx[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int q = 0; q < 64; ++q) s[q] = t.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(s[q] * t.cap_in)));
-  } else {
+  for (int q = 0; q < 64; q += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], fabsf(s[q + 2 * i]), fabsf(s[q + 2 * i + 1]));
+  // a NaN passes: the polynomial hands it on as well
+  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  const uint64_t off = f32x2_pack(offset, offset);
+  if (__all_sync(0xffffffffu, top <= t.cap_range[0])) {
     const uint64_t k0 = f32x2_pack(t.cap_poly[0], t.cap_poly[0]), k1 = f32x2_pack(t.cap_poly[1], t.cap_poly[1]);
-    const uint64_t k2 = f32x2_pack(t.cap_poly[2], t.cap_poly[2]), k3 = f32x2_pack(t.cap_poly[3], t.cap_poly[3]);
+    const uint64_t k2 = f32x2_pack(t.cap_poly[2], t.cap_poly[2]);
 #pragma unroll
     for (int q = 0; q < 32; ++q) {
       const uint64_t v = f32x2_pack(s[2 * q], s[2 * q + 1]);
       const uint64_t u = f32x2_mul(v, v);
-      uint64_t p = f32x2_fma(k3, u, k2);
-      p = f32x2_fma(p, u, k1);
-      p = f32x2_fma(p, u, k0);
-      f32x2_unpack(f32x2_mul(p, v), s[2 * q], s[2 * q + 1]);
+      const uint64_t p = f32x2_fma(f32x2_fma(k2, u, k1), u, k0);
+      f32x2_unpack(f32x2_fma(p, v, off), s[2 * q], s[2 * q + 1]);
     }
+  } else if (__all_sync(0xffffffffu, top <= t.cap_range[1])) {
+    const uint64_t k0 = f32x2_pack(t.cap_poly[3], t.cap_poly[3]), k1 = f32x2_pack(t.cap_poly[4], t.cap_poly[4]);
+    const uint64_t k2 = f32x2_pack(t.cap_poly[5], t.cap_poly[5]), k3 = f32x2_pack(t.cap_poly[6], t.cap_poly[6]);
+#pragma unroll
+    for (int q = 0; q < 32; ++q) {
+      const uint64_t v = f32x2_pack(s[2 * q], s[2 * q + 1]);
+      const uint64_t u = f32x2_mul(v, v);
+      const uint64_t p = f32x2_fma(f32x2_fma(f32x2_fma(k3, u, k2), u, k1), u, k0);
+      f32x2_unpack(f32x2_fma(p, v, off), s[2 * q], s[2 * q + 1]);
+    }
+  } else {
+    const float high = t.cap_out + offset, twice = -2.0f * t.cap_out;
+#pragma unroll
+    for (int q = 0; q < 64; ++q) s[q] = fmaf(twice, rcp(1.0f + ex2(s[q] * t.cap_in)), high);
   }
 }
 
@@ -486,9 +510,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       row[i] = lane_base + (lane >> 2) + 8 * i;
-      const int tok = row[i] / a.group;
-      const int head = g.kvh * a.group + (row[i] - tok * a.group);
-      const bool live = row[i] < g.rows;
+      // Rows past the tile's last take its place: nobody reads them, and no warp masks for them.
+      const int at = min(row[i], g.rows - 1);
+      const int tok = at / a.group;
+      const int head = g.kvh * a.group + (at - tok * a.group);
       const int pos = g.it.first + tok;  // key position of the row
       // floor(pos / frame), also below zero
       frame[i] = pos >= 0 ? pos / a.t.frame : -1 - (-1 - pos) / a.t.frame;
@@ -498,8 +523,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         limit[i] = static_cast<int>(max(static_cast<int64_t>(0),
                                         min(static_cast<int64_t>(limit[i]), max(e, static_cast<int64_t>(g.it.prefix)))));
       }
-      if (!live) limit[i] = 0;
-      slope[i] = kBias ? a.slopes[live ? head : 0] : 0.0f;
+      slope[i] = kBias ? a.slopes[head] : 0.0f;
     }
     const float sl2 = a.t.scale_log2;
     const float fixed = kFixedTop - a.t.cap_out;
@@ -530,34 +554,26 @@ __global__ void __launch_bounds__(kThreads, 2)
       warp_arrive(c.s_free());  // QK of the next tile may overwrite S
       const int k0 = (g.t0 + j) * kTile;
       const bool partial = __any_sync(0xffffffffu, min(limit[0], limit[1]) < k0 + kTile);
-      if constexpr (kCap) cap_scores(s, a.t, partial);
+      const int lim[2] = {limit[0] - k0 - c0, limit[1] - k0 - c0};
+      if constexpr (kCap) {
+        if (partial) hide(s, lim, 0.0f);  // hidden keys may hold anything: out of the range check
+        cap_scores(s, a.t, kFixed ? fixed : 0.0f);  // kFixed: the exponent itself
+      }
       if constexpr (kBias) {
         const bool past = k0 + kTile - 1 <= g.it.first || (a.t.causal && g.it.prefix == 0);
         const bool ahead = k0 >= g.it.first + g.it.tokens - 1;
         bias_scores<kCap>(s, a.t, k0, c0, frame, slope, past ? -1 : ahead ? 1 : 0);
       }
       constexpr bool kScaled = kCap || kBias;  // s already in the log2 domain
-      if (partial) {
-        const int lim0 = limit[0] - k0 - c0, lim1 = limit[1] - k0 - c0;
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if (8 * k + e >= lim0) s[4 * k + e] = -INFINITY;
-            if (8 * k + e >= lim1) s[4 * k + 2 + e] = -INFINITY;
-          }
-      }
+      if (partial) hide(s, lim, -INFINITY);
       bool grow[2] = {false, false};
       float alpha[2] = {1.0f, 1.0f};
-      uint64_t neg2[2];
+      uint64_t neg2[2] = {0, 0};
       float mx[2];
       if (!kFixed) row_maxima(s, mx);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (kFixed) {
-          neg2[i] = f32x2_pack(fixed, fixed);
-          continue;
-        }
+        if (kFixed) break;
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
         if (!kScaled) mx[i] *= sl2;
@@ -578,12 +594,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int i = 0; i < 2; ++i) {
           const uint64_t v = f32x2_pack(s[4 * k + 2 * i], s[4 * k + 2 * i + 1]);
           float x0, x1;
-          f32x2_unpack(kScaled ? f32x2_add(v, neg2[i]) : f32x2_fma(v, sc2, neg2[i]), x0, x1);
+          f32x2_unpack(kFixed ? v : kScaled ? f32x2_add(v, neg2[i]) : f32x2_fma(v, sc2, neg2[i]), x0, x1);
           const float p0 = ex2(x0), p1 = ex2(x1);
-          const uint32_t p2 = kF16 ? f16x2_from_f32(p0, p1) : pack_bf16x2(p0, p1);
           const uint64_t pp = f32x2_pack(p0, p1);
           acc[i] = k == 0 ? pp : f32x2_add(acc[i], pp);
-          pk[2 * k + i] = p2;
+          pk[2 * k + i] = kF16 ? f16x2_from_f32(p0, p1) : pack_bf16x2(p0, p1);
         }
       }
       if (j > 0) {
@@ -669,30 +684,33 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t part = c.base + Smem::kPart, ml = c.base + Smem::kMl;
       for (int i = static_cast<int>(threadIdx.x) - 32 * kFirstSoftmaxWarp; i < (r1 - r0) * 16; i += kSoftmaxThreads) {
         const int r = r0 + (i >> 4), ch = i & 15;
-        // Every CTA's (maximum, sum) of the row, then its chunk: each batch of remote loads is
-        // issued before the first is used.
-        float2 q[kMaxSplits];
+        // Every CTA's (maximum, sum) of the row and its chunk, four CTAs at a time: the eight remote
+        // loads are issued before the first is used, and the batch is folded in like a key tile.
         float mt = -INFINITY, lt = 0.0f;
-#pragma unroll
-        for (int p = 0; p < kMaxSplits; ++p)
-          if (p < a.splits) q[p] = ld_cluster_v2(cluster_addr(ml + r * 8, p));
-#pragma unroll
-        for (int p = 0; p < kMaxSplits; ++p)
-          if (p < a.splits) mt = fmaxf(mt, q[p].x);
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int p0 = 0; p0 < kMaxSplits; p0 += 4) {
+        for (int p0 = 0; p0 < a.splits; p0 += 4) {
+          float2 q[4];
           float4 v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (p0 + e < a.splits) v[e] = ld_cluster_v4(cluster_addr(part + r * 256 + ((ch ^ (r & 15)) << 4), p0 + e));
+            if (p0 + e < a.splits) {
+              q[e] = ld_cluster_v2(cluster_addr(ml + r * 8, p0 + e));
+              v[e] = ld_cluster_v4(cluster_addr(part + r * 256 + ((ch ^ (r & 15)) << 4), p0 + e));
+            } else {
+              q[e] = make_float2(-INFINITY, 0.0f);
+            }
+          const float m_new = fmaxf(fmaxf(mt, fmaxf(q[0].x, q[1].x)), fmaxf(q[2].x, q[3].x));
+          const float old = mt == -INFINITY ? 0.0f : ex2(mt - m_new);
+          sum.x *= old, sum.y *= old, sum.z *= old, sum.w *= old;
+          lt *= old;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (p0 + e < a.splits) {
-              const float f = q[p0 + e].x == -INFINITY ? 0.0f : ex2(q[p0 + e].x - mt);
+            if (q[e].x != -INFINITY) {
+              const float f = ex2(q[e].x - m_new);
               sum.x += f * v[e].x, sum.y += f * v[e].y, sum.z += f * v[e].z, sum.w += f * v[e].w;
-              lt += f * q[p0 + e].y;
+              lt += f * q[e].y;
             }
+          mt = m_new;
         }
         const float inv = 1.0f / lt;
         if (lt == 0.0f) sum = make_float4(0.f, 0.f, 0.f, 0.f);

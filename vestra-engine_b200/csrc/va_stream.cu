@@ -109,12 +109,17 @@ va::AttnTerms make_terms(const va_attn_terms* t) {
   a.cap_in = t->score_cap > 0.0f ? static_cast<float>(2.0 * kLog2e * scale / t->score_cap) : 0.0f;
   a.cap_out = t->score_cap > 0.0f ? static_cast<float>(t->score_cap * kLog2e) : 0.0f;
   if (t->score_cap > 0.0f) {
-    // tanh(z) = z (c0 + c1 z^2 + c2 z^4 + c3 z^6) for |z| <= 0.6 (fit: va_masked.cu), z = scale x / cap
-    static const double kTanh[4] = {0.9999978512525337, -0.3331403919023951, 0.13057855946359676, -0.040929422032535266};
+    // tanh(z) = z (c0 + c1 z^2 + ...) for |z| <= 0.3 and |z| <= 0.6 (fits: va_masked.cu), z = scale x / cap
+    static const double kTanh[7] = {0.9999988388472373, -0.3331002159727106, 0.126339459668236, 0.9999978512525337,
+                                    -0.3331403919023951, 0.13057855946359676, -0.040929422032535266};
     const double z = scale / t->score_cap;
     double k = scale * kLog2e;
-    for (int i = 0; i < 4; ++i, k *= z * z) a.cap_poly[i] = static_cast<float>(kTanh[i] * k);
-    a.cap_range = static_cast<float>(std::min(0.6 * t->score_cap, 77.0) / scale);
+    for (int i = 0; i < 4; ++i, k *= z * z) {
+      if (i < 3) a.cap_poly[i] = static_cast<float>(kTanh[i] * k);
+      a.cap_poly[3 + i] = static_cast<float>(kTanh[3 + i] * k);
+    }
+    a.cap_range[0] = static_cast<float>(std::min(0.3 * t->score_cap, 77.0) / scale);
+    a.cap_range[1] = static_cast<float>(std::min(0.6 * t->score_cap, 77.0) / scale);
   }
   return a;
 }
