@@ -316,7 +316,7 @@ enum ElemType { kBf16 = 0, kF16 = 1, kF32 = 2 };
 
 constexpr int kRopeMaxPairs = 128;
 struct RopeAxesArgs {
-  double turns[kRopeMaxPairs];        // turns per unit of position, by pair
+  uint64_t turns[kRopeMaxPairs];      // 2^-64 turns per unit of position, modulo one turn, by pair
   uint8_t first[kRopeMaxPairs];       // channel of the pair's first element
   uint8_t second[kRopeMaxPairs];      // and of its second
   uint8_t axis[kRopeMaxPairs];

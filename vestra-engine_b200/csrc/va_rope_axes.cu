@@ -3,7 +3,7 @@
 //   (x0, x1) -> (x0 cos a - x1 sin a, x1 cos a + x0 sin a),  a = position[axis] * freq
 //
 // One pass: every element is read once and written once, so the kernel is bound by HBM
-// (or, for a handful of tokens, by the launch).  A thread owns one (head, chunk) of kRows
+// (or, for a handful of tokens, by the launch).  A thread owns one (head, chunk) of a few
 // consecutive token rows, a chunk being V pairs held in one or two vectors of up to 16
 // bytes: it issues all its rows' loads, then the block tabulates the rows' (cos, sin) per
 // pair in shared memory, once for all heads of q and k (a 32-pair row is shared by 12 + 12
@@ -11,10 +11,10 @@
 // thread turns its chunks and writes them.  No index is divided inside the row loop.
 //
 // Angles: a position may be any int32 and the product with the frequency is needed
-// modulo one turn, which F32 loses beyond a few thousand turns.  The frequency in turns
-// is held in 64 bits, the product is formed and reduced to [-1/2, 1/2] in 64 bits, and
-// the reduced angle goes to sincospi in F32 with the F32 rounding of the angle put back
-// by one first-order step.
+// modulo one turn, which F32 loses beyond a few thousand turns.  The frequency in turns is
+// held as a 64-bit binary fraction, so the product modulo 2^64 is the exact fraction of a
+// turn in integer arithmetic (64-bit floating point made the table the block's longest
+// chain); its upper 32 bits are the reduced angle, a signed fraction of a turn.
 #include "va_internal.h"
 #include "va_ptx.cuh"
 
@@ -23,7 +23,11 @@ namespace va {
 namespace {
 
 constexpr int kMaxThreads = 256;
-constexpr int kRows = 4;  // 2 / 8 / 16 rows: 16.9 / 19.6 / 20.5 us at 10,392 bf16 rows of 24 heads, against 15.0
+// Rows per block: two where a row's chunk is two 16-byte vectors of 2-byte elements, else four.  Measured
+// at 10,392 bf16 rows of 24 heads, inputs out of L2, for 2 / 4 / 8 rows: sections 16,24,24 (8-byte
+// vectors) 18.9 / 16.7 / 23.5 us, sections 32,32 15.8 / 18.8 / 22.4, F32 (27,729 rows of 20 heads) 62.4 / 49.4 / 48.2.
+template <class T, int V, bool kInter>
+constexpr int rows_per_block() { return sizeof(T) == 2 && V == 8 && !kInter ? 2 : 4; }
 
 template <class T>
 __device__ __forceinline__ float to_f32(T x);
@@ -47,21 +51,33 @@ struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
 
-// (cos, sin) of 2 pi t for t in turns, |t| <= 1/2 after the reduction.
-__device__ __forceinline__ float2 turn_cos_sin(double t) {
-  t -= rint(t);
-  const float hi = static_cast<float>(t);
-  const float lo = static_cast<float>(t - static_cast<double>(hi)) * 6.283185307179586f;
+// (cos, sin) of position * turns (2^-64 turns a unit).  For 16-bit elements sin.approx and cos.approx on
+// [-pi, pi] (absolute error below 2^-21); for F32 sincospi of the F32 part of the angle, the rest put
+// back by one first-order step.
+template <class T>
+__device__ __forceinline__ float2 turn_cos_sin(int position, uint64_t turns) {
+  const int t = static_cast<int>((static_cast<uint64_t>(static_cast<int64_t>(position)) * turns) >> 32);
   float s, c;
-  sincospif(2.0f * hi, &s, &c);
-  return make_float2(fmaf(-s, lo, c), fmaf(c, lo, s));
+  if constexpr (sizeof(T) == 2) {
+    __sincosf(static_cast<float>(t) * 1.4629180792671596e-9f, &s, &c);  // 2 pi / 2^32
+    return make_float2(c, s);
+  } else {
+    const float hi = static_cast<float>(t);
+    // hi may be 2^31, which no int holds: the difference is taken in 64 bits
+    const float lo = static_cast<float>(static_cast<int>(t - static_cast<int64_t>(hi))) * 1.4629180792671596e-9f;
+    sincospif(hi * 4.656612873077393e-10f, &s, &c);  // 2^-31
+    return make_float2(fmaf(-s, lo, c), fmaf(c, lo, s));
+  }
 }
 
 // V pairs per chunk; kInter: pairs are neighbours (2i, 2i+1), one vector of 2V elements;
 // otherwise two vectors of V elements, min_half a multiple of V.
 template <class T, int V, bool kInter>
 __global__ void __launch_bounds__(kMaxThreads) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a) {
-  extern __shared__ float2 cs[];  // [kRows][pairs]
+  constexpr int kRows = rows_per_block<T, V, kInter>();
+  extern __shared__ float4 table[];  // cosines [kRows][pairs], then sines: a chunk's are one vector each
+  float* cosines = reinterpret_cast<float*>(table);
+  float* sines = cosines + kRows * a.pairs;
   using Part = Vec<T, kInter ? 2 * V : V>;
   constexpr int kVecs = kInter ? 1 : 2;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
@@ -88,7 +104,9 @@ __global__ void __launch_bounds__(kMaxThreads) rope_axes_kernel(const __grid_con
   for (int i = threadIdx.x; i < rows * a.pairs; i += blockDim.x) {
     const int r = i / a.pairs, p = i - r * a.pairs;
     const int pos = __ldg(a.positions + (row0 + r) * a.axes + a.axis[p]);
-    cs[i] = turn_cos_sin(static_cast<double>(pos) * a.turns[p]);
+    const float2 w = turn_cos_sin<T>(pos, a.turns[p]);
+    cosines[i] = w.x;
+    sines[i] = w.y;
   }
   __syncthreads();
   if (active) {
@@ -96,10 +114,15 @@ __global__ void __launch_bounds__(kMaxThreads) rope_axes_kernel(const __grid_con
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       if (r < rows) {
-        const Vec<float2, (V > 1 ? 2 : 1)>* t = reinterpret_cast<const Vec<float2, (V > 1 ? 2 : 1)>*>(cs + r * a.pairs + pair);
+        constexpr int kWide = V < 4 ? V : 4;
+        using Wide = Vec<float, kWide>;
+        const Wide* tc = reinterpret_cast<const Wide*>(cosines + r * a.pairs + pair);
+        const Wide* ts = reinterpret_cast<const Wide*>(sines + r * a.pairs + pair);
+        Wide wc, ws;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float2 w = V > 1 ? t[e >> 1].v[e & (V > 1)] : t[e].v[0];
+          if (e % kWide == 0) wc = tc[e / kWide], ws = ts[e / kWide];
+          const float2 w = make_float2(wc.v[e % kWide], ws.v[e % kWide]);
           T& lo = x[r][0].v[kInter ? 2 * e : e];
           T& hi = kInter ? x[r][0].v[2 * e + 1] : x[r][kVecs - 1].v[e];
           const float p0 = to_f32(lo), p1 = to_f32(hi);
@@ -133,13 +156,14 @@ __global__ void __launch_bounds__(kMaxThreads) rope_axes_kernel(const __grid_con
 
 template <class T, int V>
 cudaError_t launch_v(const RopeAxesArgs& a, cudaStream_t st) {
-  const int64_t blocks = (a.rows + kRows - 1) / kRows;
+  const int rows = a.pairing ? rows_per_block<T, V, true>() : rows_per_block<T, V, false>();
+  const int64_t blocks = (a.rows + rows - 1) / rows;
   const int items = (a.in[0].heads + a.in[1].heads) * (a.pairs / V);
   // As few threads past the items as the warp size allows.
   const int parts = (items + kMaxThreads - 1) / kMaxThreads;
   const int threads = ((items + parts - 1) / parts + 31) / 32 * 32;
   if (blocks > 0x7fffffff || parts > 65535) return cudaErrorInvalidValue;
-  const size_t smem = sizeof(float2) * kRows * a.pairs;
+  const size_t smem = 2 * sizeof(float) * rows * a.pairs;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
   if (a.pairing)
     rope_axes_kernel<T, V, true><<<grid, threads, smem, st>>>(a);

@@ -315,7 +315,10 @@ int va_rope_axes_device(va_ctx* c, const va_rope_axes* rope, int64_t rows, int h
       a.first[n] = static_cast<uint8_t>(origin + (rope->pairing ? 2 * j : j));
       a.second[n] = static_cast<uint8_t>(origin + (rope->pairing ? 2 * j + 1 : j + block / 2));
       a.axis[n] = static_cast<uint8_t>(ax);
-      a.turns[n] = std::pow(static_cast<double>(rope->base), -2.0 * j / block) / 6.283185307179586476925;
+      const double turns = std::pow(static_cast<double>(rope->base), -2.0 * j / block) / 6.283185307179586476925;
+      // 2^64 times the fraction of a turn (a product of 53 bits: exact), wrapping at 2^64
+      const double scaled = (turns - std::floor(turns)) * 18446744073709551616.0;
+      a.turns[n] = scaled < 18446744073709551615.0 ? static_cast<uint64_t>(scaled) : 0;
     }
     g = gcd(g, block / 2);
     start += s;
