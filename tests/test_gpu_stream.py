@@ -582,6 +582,120 @@ def test_a_streaming_window(ctx, fmt):
         assert torch.equal(vo[ro[b]:ro[b + 1]], want)
 
 
+def test_two_graphs_at_once(ctx):
+    """Two captured graphs over one plan and one cache, replayed at once on two streams with
+    inputs of their own: no call has scratch memory that another could overwrite."""
+    g = gen(31)
+    n, m, heads, kvh = 200, 3000, 4, 2
+    plans = [va.AttentionPlan(ctx, heads, kvh, [0, n], [0, m], causal=True, score_cap=30.0),
+             va.AttentionPlan(ctx, heads, kvh, [0, 1], [0, m], causal=True)]
+    assert va.attention_plan_shape(heads, kvh, [0, n], [0, m], True)["splits"] > 1
+    cache, codes, scales = new_cache(g, 1, kvh, m, torch.int8)
+    k, v = randn(g, m, kvh, D, dtype=BF16), randn(g, m, kvh, D, dtype=BF16)
+    ctx.kv_cache_write(cache, k, v, i32([0, m]), i32([m]))
+    off, lens = i32([0, 3]), i32([m])
+    sides = []
+    for i in range(2):
+        q = randn(g, n, heads, D, dtype=BF16)
+        outs = [torch.empty_like(q), torch.empty_like(q[:1]), torch.empty_like(q[:3])]
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            s = torch.cuda.current_stream().cuda_stream
+            for _ in range(10):
+                ctx.masked_attention(plans[0], q, k, v, outs[0], stream=s)
+                ctx.masked_attention(plans[1], q, k, v, outs[1], stream=s)
+                ctx.cache_attention(cache, q[:3], outs[2], off, lens, max_tokens=3, stream=s)
+        sides.append((q, outs, graph, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for _, _, graph, st in sides:
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    kd, vd = ((c[0].double() * sc[0, :, :, None].double()).transpose(0, 1) for c, sc in zip(codes, scales))
+    for q, outs, _, _ in sides:
+        check_attention(outs[0], *attention_ref(q, k, v, True, 1, 0, None, 30.0))
+        check_attention(outs[1], *attention_ref(q[:1], k, v, True, 1, 0, None, 0.0))
+        check_attention(outs[2], *attention_ref(q[:3], kd, vd, True, 1, 0, None, 0.0), p_step=2.0 ** -15)
+
+
+def test_addresses_past_32_bits(ctx):
+    """A cache of more than 2^32 bytes and key rows more than 2^32 bytes apart."""
+    g = gen(32)
+    cap, n = 23_000_001, 150  # odd: the scales of a head start anywhere
+    shape = (2, 2, cap)
+    codes = [torch.empty(shape + (D,), device="cuda", dtype=torch.int8) for _ in range(2)]
+    scales = [torch.empty(shape, device="cuda") for _ in range(2)]
+    cache = va.KvCache(*codes, *scales)
+    k, v = randn(g, 2 * n, 2, D, dtype=BF16), randn(g, 2 * n, 2, D, dtype=BF16)
+    # document 1's tokens at the far end of the buffer
+    ctx.kv_cache_write(cache, k, v, i32([0, n, 2 * n]), i32([n, cap]))
+    val, sc = quantise_ref(v[n:], torch.int8)
+    assert torch.equal(codes[1][1, :, cap - n:].double().transpose(0, 1), val)
+    ko, vo = torch.zeros_like(k[:n]), torch.zeros_like(v[:n])
+    ctx.kv_cache_read(cache, i32([0, 0, n]), ko, vo, first=i32([0, cap - n]))
+    assert torch.equal(vo, (val * sc[..., None]).float().to(BF16))
+    for c in codes:
+        c[1, :, :n] = c[1, :, cap - n:]
+    for x in scales:
+        x[1, :, :n] = x[1, :, cap - n:]
+    q = randn(g, 2, 4, D, dtype=BF16)
+    out = torch.empty_like(q)
+    ctx.cache_attention(cache, q, out, i32([0, 1, 2]), i32([n, n]), max_tokens=1)
+    for b in range(2):
+        kd, vd = ((c[b, :, :n].double() * x[b, :, :n, None].double()).transpose(0, 1) for c, x in zip(codes, scales))
+        check_attention(out[b:b + 1], *attention_ref(q[b:b + 1], kd, vd, True, 1, 0, None, 0.0), p_step=2.0 ** -15)
+    del cache, codes, scales, c, x
+    rows, step = 1200, 2 ** 21
+    big = torch.empty((rows - 1) * step + 2 * D, device="cuda", dtype=BF16)  # 5 GB
+    far = big.as_strided((rows, 2, D), (step, D, 1))
+    far.copy_(randn(g, rows, 2, D, dtype=BF16))
+    for n in (1, 200):
+        q = randn(g, n, 2, D, dtype=BF16)
+        out = torch.empty_like(q)
+        ctx.masked_attention(va.AttentionPlan(ctx, 2, 2, [0, n], [0, rows]), q, far, far, out)
+        check_attention(out, *attention_ref(q, far, far, False, 1, 0, None, 0.0))
+    pos = torch.randint(0, 100, (rows, 3), generator=g, device="cuda", dtype=torch.int32)
+    before = far.clone()
+    ctx.rope_axes(va.RopeAxes((16, 24, 24)), pos, far, far)
+    assert (far.double() - rope_ref(before, pos, (16, 24, 24), 100.0, "per_axis", 0)).abs().max() <= rope_tol(before, BF16)
+
+
+def test_many_documents_and_widest_heads(ctx):
+    g = gen(33)
+    docs = 1500
+    new = [int(x) for x in torch.randint(0, 3, (docs,), generator=torch.Generator().manual_seed(1))]
+    lens = [n + int(x) for n, x in zip(new, torch.randint(0, 20, (docs,), generator=torch.Generator().manual_seed(2)))]
+    cache, codes, scales = new_cache(g, docs, 2, 24, torch.float8_e4m3fn)
+    hist, off = np.cumsum([0] + lens), np.cumsum([0] + new)
+    k, v = randn(g, int(hist[-1]), 2, D, dtype=F16), randn(g, int(hist[-1]), 2, D, dtype=F16)
+    ctx.kv_cache_write(cache, k, v, i32(hist), i32(lens))
+    q = randn(g, int(off[-1]), 4, D, dtype=F16)
+    out, dense = torch.empty_like(q), torch.empty_like(q)
+    ctx.cache_attention(cache, q, out, i32(off), i32(lens), max_tokens=2)
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    ctx.kv_cache_read(cache, i32(hist), ko, vo)
+    ctx.masked_attention(va.AttentionPlan(ctx, 4, 2, off, hist, causal=True), q, ko, vo, dense)
+    for b in list(range(0, docs, 97)) + [docs - 1]:
+        if new[b]:
+            kd, vd = ((c[b, :, :lens[b]].double() * x[b, :, :lens[b], None].double()).transpose(0, 1) for c, x in zip(codes, scales))
+            ref, a = attention_ref(q[off[b]:off[b + 1]], kd, vd, True, 1, 0, None, 0.0)
+            check_attention(out[off[b]:off[b + 1]], ref, a, p_step=2.0 ** -15)
+            # the values read back carry one more f16 rounding
+            check_attention(dense[off[b]:off[b + 1]], ref, a, p_step=2.0 ** -9)
+    assert (out.float() - dense.float()).abs().max() <= 2.0 ** -7 * v.abs().max()
+    run_masked(ctx, [3, 40], [30, 45], 128, 128, BF16, causal=True, bias=True, seed=34)
+    run_masked(ctx, [1], [400], 128, 128, F16, causal=True, seed=35)
+
+
+@pytest.mark.parametrize("frame", [2 ** 31 - 1, 2 ** 24, 127, 128, 129, 200, 3])
+def test_masked_frames_at_their_edges(ctx, frame):
+    """Frames longer than any document, and around the tile's 128 keys; rows before the first key."""
+    run_masked(ctx, [300, 150], [500, 40], 2, 1, BF16, True, frame, [7, 30], True, 0.0, seed=frame % 1000)
+    run_masked(ctx, [2, 1], [500, 40], 2, 1, F16, False, frame, None, True, 30.0, seed=frame % 1000)
+
+
 # ---------------------------------------------------------------------------- refusals
 def test_refusals(ctx):
     q = torch.zeros(8, 4, D, device="cuda", dtype=BF16)

@@ -271,22 +271,23 @@ _PACK_HEADS = struct.Struct("=QqqiI").pack
 
 def _heads(x, device, what, channels=None):
     """(va_heads, rows, heads) of a [rows, heads, channels] torch tensor; any token and head strides."""
-    if not getattr(x, "is_cuda", False) or x.get_device() != device:
-        _refuse(f"{what} must be a tensor on CUDA device {device}")
-    code = _DTYPE_CODES.get(x.dtype)
-    if code is None:
-        code = _dtype_code(x.dtype)
-    if code < 0 or x.dim() != 3:
-        _refuse(f"{what} must be [rows, heads, {channels or 'channels'}] bf16, f16 or f32")
-    rows, heads, d = x.shape
-    ts, hs, cs = x.stride()
-    if cs != 1 or (channels is not None and d != channels):
-        _refuse(f"{what} needs {channels or ''} contiguous channels")
-    if heads == 1:
-        hs = d
-    if rows <= 1:  # never stepped over
-        ts = heads * max(hs, d)
-    return _PACK_HEADS(x.data_ptr(), ts, hs, heads, code), rows, heads
+    try:
+        if x.get_device() == device:  # -1 for host tensors
+            rows, heads, d = x.shape
+            ts, hs, cs = x.stride()
+            code = _DTYPE_CODES.get(x.dtype)
+            if code is None:
+                code = _dtype_code(x.dtype)
+            if cs == 1 and code >= 0 and (channels is None or d == channels):
+                if heads == 1:
+                    hs = d
+                if rows <= 1:  # never stepped over
+                    ts = heads * max(hs, d)
+                return _PACK_HEADS(x.data_ptr(), ts, hs, heads, code), rows, heads
+    except (AttributeError, ValueError):
+        pass
+    _refuse(f"{what} must be a [rows, heads, {channels or 'channels'}] tensor (bf16, f16 or f32, channels contiguous) "
+            f"on CUDA device {device}")
 
 
 _INT32, _FLOAT32 = -2, VA_F32  # kinds of _device_array
@@ -296,11 +297,13 @@ def _device_array(x, device, what, kind, count):
     """Address of a contiguous device tensor of one dtype and element count (None passes)."""
     if x is None:
         return None
-    if not getattr(x, "is_cuda", False) or x.get_device() != device:
-        _refuse(f"{what} must be a tensor on CUDA device {device}")
-    if _dtype_code(x.dtype) != kind or x.numel() != count or not x.is_contiguous():
-        _refuse(f"{what} must be a contiguous {'int32' if kind == _INT32 else 'float32'} tensor of {count} elements")
-    return x.data_ptr()
+    try:
+        if x.get_device() == device and x.numel() == count and _dtype_code(x.dtype) == kind and x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(f"{what} must be a contiguous {'int32' if kind == _INT32 else 'float32'} tensor of {count} elements on CUDA "
+            f"device {device}")
 
 
 def default_config(**overrides) -> VaConfig:
