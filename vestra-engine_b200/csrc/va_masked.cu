@@ -301,35 +301,43 @@ __device__ __forceinline__ void hide(float* s, const int* lim, float v) {
 // least squares on Chebyshev nodes of z^2): P quadratic for |z| <= 0.3 (relative error 1.2e-6),
 // cubic for |z| <= 0.6 (2.2e-6, and scores of at most 77, so within 1.7e-4).  Else
 // cap log2(e) (1 - 2 / (1 + e^(2z))): two MUFU operations a score.
-__device__ __forceinline__ void cap_scores(float* s, const AttnTerms& t, float offset) {
+__device__ __forceinline__ float largest(const float* s) {
   float mx[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int q = 0; q < 64; q += 8)
 #pragma unroll
     for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], fabsf(s[q + 2 * i]), fabsf(s[q + 2 * i + 1]));
-  // a NaN passes: the polynomial hands it on as well
-  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-  const uint64_t off = f32x2_pack(offset, offset);
+  // a NaN passes: the polynomials hand it on as well
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+// The polynomials of one pair of scores: kCubic for the wider range.
+template <bool kCubic>
+struct CapPoly {
+  uint64_t k0, k1, k2, k3, off;
+  __device__ __forceinline__ CapPoly(const AttnTerms& t, float offset) {
+    const float* p = t.cap_poly + (kCubic ? 3 : 0);
+    k0 = f32x2_pack(p[0], p[0]), k1 = f32x2_pack(p[1], p[1]), k2 = f32x2_pack(p[2], p[2]);
+    if (kCubic) k3 = f32x2_pack(p[3], p[3]);
+    off = f32x2_pack(offset, offset);
+  }
+  __device__ __forceinline__ uint64_t operator()(uint64_t v) const {
+    const uint64_t u = f32x2_mul(v, v);
+    const uint64_t p = f32x2_fma(kCubic ? f32x2_fma(k3, u, k2) : k2, u, k1);
+    return f32x2_fma(f32x2_fma(p, u, k0), v, off);
+  }
+};
+template <bool kCubic>
+__device__ __forceinline__ void cap_poly(float* s, const AttnTerms& t, float offset) {
+  const CapPoly<kCubic> poly(t, offset);
+#pragma unroll
+  for (int q = 0; q < 32; ++q) f32x2_unpack(poly(f32x2_pack(s[2 * q], s[2 * q + 1])), s[2 * q], s[2 * q + 1]);
+}
+__device__ __forceinline__ void cap_scores(float* s, const AttnTerms& t, float offset) {
+  const float top = largest(s);
   if (__all_sync(0xffffffffu, top <= t.cap_range[0])) {
-    const uint64_t k0 = f32x2_pack(t.cap_poly[0], t.cap_poly[0]), k1 = f32x2_pack(t.cap_poly[1], t.cap_poly[1]);
-    const uint64_t k2 = f32x2_pack(t.cap_poly[2], t.cap_poly[2]);
-#pragma unroll
-    for (int q = 0; q < 32; ++q) {
-      const uint64_t v = f32x2_pack(s[2 * q], s[2 * q + 1]);
-      const uint64_t u = f32x2_mul(v, v);
-      const uint64_t p = f32x2_fma(f32x2_fma(k2, u, k1), u, k0);
-      f32x2_unpack(f32x2_fma(p, v, off), s[2 * q], s[2 * q + 1]);
-    }
+    cap_poly<false>(s, t, offset);
   } else if (__all_sync(0xffffffffu, top <= t.cap_range[1])) {
-    const uint64_t k0 = f32x2_pack(t.cap_poly[3], t.cap_poly[3]), k1 = f32x2_pack(t.cap_poly[4], t.cap_poly[4]);
-    const uint64_t k2 = f32x2_pack(t.cap_poly[5], t.cap_poly[5]), k3 = f32x2_pack(t.cap_poly[6], t.cap_poly[6]);
-#pragma unroll
-    for (int q = 0; q < 32; ++q) {
-      const uint64_t v = f32x2_pack(s[2 * q], s[2 * q + 1]);
-      const uint64_t u = f32x2_mul(v, v);
-      const uint64_t p = f32x2_fma(f32x2_fma(f32x2_fma(k3, u, k2), u, k1), u, k0);
-      f32x2_unpack(f32x2_fma(p, v, off), s[2 * q], s[2 * q + 1]);
-    }
+    cap_poly<true>(s, t, offset);
   } else {
     const float high = t.cap_out + offset, twice = -2.0f * t.cap_out;
 #pragma unroll
@@ -555,6 +563,38 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int k0 = (g.t0 + j) * kTile;
       const bool partial = __any_sync(0xffffffffu, min(limit[0], limit[1]) < k0 + kTile);
       const int lim[2] = {limit[0] - k0 - c0, limit[1] - k0 - c0};
+      uint32_t pk[32];  // 16x128b order: block k: (row 0 pair k), (row 1 pair k)
+      uint64_t acc[2];
+      auto emit = [&](int k, int i, uint64_t x) {  // the exponentials of a pair
+        float x0, x1;
+        f32x2_unpack(x, x0, x1);
+        const float p0 = ex2(x0), p1 = ex2(x1);
+        const uint64_t pp = f32x2_pack(p0, p1);
+        acc[i] = k == 0 ? pp : f32x2_add(acc[i], pp);
+        pk[2 * k + i] = kF16 ? f16x2_from_f32(p0, p1) : pack_bf16x2(p0, p1);
+      };
+      bool grow[2] = {false, false};
+      float alpha[2] = {1.0f, 1.0f};
+      // kFixed, nothing hidden: polynomial and exponential pair by pair, so that the FMA pipe and
+      // MUFU work at once.
+      bool fused = false;
+      if constexpr (kFixed) {
+        auto both = [&](auto poly) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) emit(k, i, poly(f32x2_pack(s[4 * k + 2 * i], s[4 * k + 2 * i + 1])));
+          fused = true;
+        };
+        if (!partial) {
+          const float top = largest(s);
+          if (__all_sync(0xffffffffu, top <= a.t.cap_range[0]))
+            both(CapPoly<false>(a.t, fixed));
+          else if (__all_sync(0xffffffffu, top <= a.t.cap_range[1]))
+            both(CapPoly<true>(a.t, fixed));
+        }
+      }
+      if (!fused) {
       if constexpr (kCap) {
         if (partial) hide(s, lim, 0.0f);  // hidden keys may hold anything: out of the range check
         cap_scores(s, a.t, kFixed ? fixed : 0.0f);  // kFixed: the exponent itself
@@ -566,8 +606,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       constexpr bool kScaled = kCap || kBias;  // s already in the log2 domain
       if (partial) hide(s, lim, -INFINITY);
-      bool grow[2] = {false, false};
-      float alpha[2] = {1.0f, 1.0f};
       uint64_t neg2[2] = {0, 0};
       float mx[2];
       if (!kFixed) row_maxima(s, mx);
@@ -586,19 +624,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         neg2[i] = f32x2_pack(neg, neg);
       }
       const uint64_t sc2 = f32x2_pack(sl2, sl2);
-      uint32_t pk[32];  // 16x128b order: block k: (row 0 pair k), (row 1 pair k)
-      uint64_t acc[2];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
+      for (int k = 0; k < 16; ++k)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint64_t v = f32x2_pack(s[4 * k + 2 * i], s[4 * k + 2 * i + 1]);
-          float x0, x1;
-          f32x2_unpack(kFixed ? v : kScaled ? f32x2_add(v, neg2[i]) : f32x2_fma(v, sc2, neg2[i]), x0, x1);
-          const float p0 = ex2(x0), p1 = ex2(x1);
-          const uint64_t pp = f32x2_pack(p0, p1);
-          acc[i] = k == 0 ? pp : f32x2_add(acc[i], pp);
-          pk[2 * k + i] = kF16 ? f16x2_from_f32(p0, p1) : pack_bf16x2(p0, p1);
+          emit(k, i, kFixed ? v : kScaled ? f32x2_add(v, neg2[i]) : f32x2_fma(v, sc2, neg2[i]));
         }
       }
       if (j > 0) {
