@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const bool partial = __any_sync(0xffffffffu, min(limit[0], limit[1]) < k0 + kTile);
       const int lim[2] = {limit[0] - k0 - c0, limit[1] - k0 - c0};
       uint32_t pk[32];  // 16x128b order: block k: (row 0 pair k), (row 1 pair k)
-      uint64_t acc[2];
+      uint64_t acc[2] = {0, 0};
       auto emit = [&](int k, int i, uint64_t x) {  // the exponentials of a pair
         float x0, x1;
         f32x2_unpack(x, x0, x1);
@@ -595,42 +595,42 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
       if (!fused) {
-      if constexpr (kCap) {
-        if (partial) hide(s, lim, 0.0f);  // hidden keys may hold anything: out of the range check
-        cap_scores(s, a.t, kFixed ? fixed : 0.0f);  // kFixed: the exponent itself
-      }
-      if constexpr (kBias) {
-        const bool past = k0 + kTile - 1 <= g.it.first || (a.t.causal && g.it.prefix == 0);
-        const bool ahead = k0 >= g.it.first + g.it.tokens - 1;
-        bias_scores<kCap>(s, a.t, k0, c0, frame, slope, past ? -1 : ahead ? 1 : 0);
-      }
-      constexpr bool kScaled = kCap || kBias;  // s already in the log2 domain
-      if (partial) hide(s, lim, -INFINITY);
-      uint64_t neg2[2] = {0, 0};
-      float mx[2];
-      if (!kFixed) row_maxima(s, mx);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (kFixed) break;
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        if (!kScaled) mx[i] *= sl2;
-        grow[i] = mx[i] > m[i] + kGrow;  // m = -inf: as soon as a key is seen
-        if (grow[i]) {
-          alpha[i] = ex2(m[i] - mx[i]);
-          m[i] = mx[i];
+        if constexpr (kCap) {
+          if (partial) hide(s, lim, 0.0f);  // hidden keys may hold anything: out of the range check
+          cap_scores(s, a.t, kFixed ? fixed : 0.0f);  // kFixed: the exponent itself
         }
-        const float neg = m[i] == -INFINITY ? 0.0f : kOffset - m[i];  // no key yet: every x is -inf
-        neg2[i] = f32x2_pack(neg, neg);
-      }
-      const uint64_t sc2 = f32x2_pack(sl2, sl2);
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
+        if constexpr (kBias) {
+          const bool past = k0 + kTile - 1 <= g.it.first || (a.t.causal && g.it.prefix == 0);
+          const bool ahead = k0 >= g.it.first + g.it.tokens - 1;
+          bias_scores<kCap>(s, a.t, k0, c0, frame, slope, past ? -1 : ahead ? 1 : 0);
+        }
+        constexpr bool kScaled = kCap || kBias;  // s already in the log2 domain
+        if (partial) hide(s, lim, -INFINITY);
+        uint64_t neg2[2] = {0, 0};
+        float mx[2];
+        if (!kFixed) row_maxima(s, mx);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint64_t v = f32x2_pack(s[4 * k + 2 * i], s[4 * k + 2 * i + 1]);
-          emit(k, i, kFixed ? v : kScaled ? f32x2_add(v, neg2[i]) : f32x2_fma(v, sc2, neg2[i]));
+          if (kFixed) break;
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+          if (!kScaled) mx[i] *= sl2;
+          grow[i] = mx[i] > m[i] + kGrow;  // m = -inf: as soon as a key is seen
+          if (grow[i]) {
+            alpha[i] = ex2(m[i] - mx[i]);
+            m[i] = mx[i];
+          }
+          const float neg = m[i] == -INFINITY ? 0.0f : kOffset - m[i];  // no key yet: every x is -inf
+          neg2[i] = f32x2_pack(neg, neg);
         }
+        const uint64_t sc2 = f32x2_pack(sl2, sl2);
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint64_t v = f32x2_pack(s[4 * k + 2 * i], s[4 * k + 2 * i + 1]);
+            emit(k, i, kFixed ? v : kScaled ? f32x2_add(v, neg2[i]) : f32x2_fma(v, sc2, neg2[i]));
+          }
       }
       if (j > 0) {
         // PV(j-1) has finished reading P and adding into O.
