@@ -373,16 +373,15 @@ cudaError_t launch_cache_attention(const KvCacheRef& c, const AttnTerms& t, int 
   a.out = out;
   const int64_t units = static_cast<int64_t>(c.documents) * c.kv_heads * a.row_blocks;
   // CTAs per (document, key head): the lengths are on the device, so by the capacity (at least one
-  // chunk per warp) and the number of units: the largest power of two that keeps all CTAs within 1.5
-  // times what the SMs hold at once, because documents usually differ in length; 16, which the
-  // GPU places less easily, only where everything fits at once.  Measured (S = CTAs): 16 documents of
-  // 1 to 32,000 tokens x 4 key heads 61 / 42 / 50 us for S = 4 / 8 / 16, all of 32,000 56 / 68 / 71; 4 x 9,000 x 12
-  // 19 / 17 / 25; 64 x 1,000 x 12 27 / 34 / 88 for S = 1 / 2 / 8.
+  // chunk per warp) and by what the SMs hold at once, at most 8, or 16, which the GPU places less
+  // easily, where that fits.  Measured (us; S = 4 / 6 / 8 CTAs, 16 documents x 4 key heads): lengths of 0 to 32,000
+  // 59 / 50 / 42, all 32,000 56 / 54 / 68, all 8,192 18 / 19 / 23; 128 units of mixed lengths S = 2 / 3 / 4 17.3 / 15.7 /
+  // 14.9, of 4,000 18.0 / 18.8 / 20.6.  Letting the CTAs past a document's share of the work leave at once
+  // gained nothing: a cluster still waits for all its places.
   const int64_t slots = kCtasPerSm * static_cast<int64_t>(sms), pairs = static_cast<int64_t>(c.documents) * c.kv_heads;
   const int64_t most = std::max<int64_t>(1, c.capacity / (kChunk * kWarps));
-  int splits = 1;
-  while (splits < 8 && 2 * splits <= most && pairs * 2 * splits * 2 <= 3 * slots) splits *= 2;
-  if (splits == 8 && 16 <= most && pairs * 16 <= slots) splits = 16;
+  const int64_t fit = std::max<int64_t>(1, std::min(slots / pairs, most));
+  const int splits = static_cast<int>(fit >= kMaxCluster ? kMaxCluster : std::min<int64_t>(fit, 8));
   const int64_t blocks = units * splits;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   if (c.e4m3)
