@@ -400,7 +400,7 @@ int va_rope_axes_device(va_ctx* ctx, const va_rope_axes* rope, int64_t rows, int
  * f(x) = floor(x / frame), frame = tokens per frame (1: single tokens):
  *   score(i, j) = cap * tanh(scale * q.k / cap) - slope[head] * |f(p) - f(j)|
  *   visible(i, j) = not causal, or f(j) <= f(p), or j < prefix[document]
- * score_cap 0: no cap; scale 0: 1/sqrt(64).  A row that sees no key gives zeros.
+ * score_cap 0: no cap, else 0.01..1000; scale 0: 1/sqrt(64), else at most 100.  A row that sees no key gives zeros.
  * Query head h reads key head h / (heads / kv_heads). */
 typedef struct va_attn_terms {
   int32_t heads;    /* 1..128 */

@@ -223,6 +223,18 @@ def test_masked_cap_over_its_whole_range(ctx, cap):
     run_masked(ctx, [200], [333], 2, 2, F16, cap=cap, gain=0.01, seed=4)
 
 
+@pytest.mark.parametrize("cap,scale", [(0.01, 100.0), (0.01, 0.0), (1000.0, 0.0), (1000.0, 30.0), (50.0, 1e-6)])
+def test_masked_cap_and_scale_at_their_limits(ctx, cap, scale):
+    """The ends of the ranges taken; scores up to several thousand at cap 1000."""
+    for n in (2, 150):
+        q, k, v = (randn(gen(40 + i), rows, 1, D, dtype=BF16) for i, rows in enumerate((n, 300, 300)))
+        out = torch.empty_like(q)
+        ctx.masked_attention(va.AttentionPlan(ctx, 1, 1, [0, n], [0, 300], score_cap=cap, scale=scale), q, k, v, out)
+        ref, a = attention_ref(q, k, v, False, 1, 0, None, cap, scale or 0.125)
+        # a capped score is off by up to 4e-7 of the cap, an F32 product by 64 * 2^-24 of the score
+        check_attention(out, ref, a, p_step=half_step(BF16) + 2 * 4e-7 * cap + 2.0 ** -17 * min(cap, 60 * (scale or 0.125)))
+
+
 @pytest.mark.parametrize("cap,gain", [(50.0, 1.5), (50.0, 60.0), (30.0, 8.0), (2.0, 1.5), (60.0, 30.0)])
 def test_masked_cap_with_many_keys(ctx, cap, gain):
     """Rows that all see many keys (a constant exponent reference up to cap 50), scores from
@@ -720,7 +732,8 @@ def test_refusals(ctx):
     refused(lambda: ctx.rope_axes(rope, pos, q, q.clone()[:, :1].expand(8, 4, D)))  # heads on top of each other
     refused(lambda: ctx.rope_axes(rope, pos, q, q.clone(), kv))
     for kw in (dict(heads=4, kv_heads=3), dict(heads=0), dict(heads=129, kv_heads=1), dict(frame=0),
-               dict(score_cap=-1.0), dict(score_cap=float("inf")), dict(scale=float("nan")),
+               dict(score_cap=-1.0), dict(score_cap=float("inf")), dict(scale=float("nan")), dict(score_cap=2000.0),
+               dict(score_cap=1e-3), dict(scale=-0.1), dict(scale=1e3), dict(score_cap=float("nan")),
                dict(q_offsets=[0, 9, 8]), dict(q_offsets=[-1, 8]), dict(k_offsets=[0, 2 ** 24 + 1]),
                dict(k_offsets=[0, 2 ** 31 + 9]), dict(prefix=[-1]), dict(slopes=np.array([1, 2, np.nan, 0])),
                dict(slopes=np.ones(3)), dict(q_offsets=[0])):

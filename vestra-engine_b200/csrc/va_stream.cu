@@ -93,8 +93,11 @@ const char* check_terms(const va_attn_terms* t) {
     return "heads must be 1..128 and a multiple of kv_heads";
   if (t->frame < 1) return "frame must be at least 1 token";
   if (t->causal != 0 && t->causal != 1) return "causal must be 0 or 1";
-  if (!std::isfinite(t->scale) || t->scale < 0.0f || !std::isfinite(t->score_cap) || t->score_cap < 0.0f)
-    return "scale and score_cap must be finite and not negative";
+  // The capped score's error grows with the cap (about 2e-7 of it); the tanh polynomial's factors
+  // (scale / cap)^6 have to stay inside F32.
+  if (!(t->scale >= 0.0f && t->scale <= 100.0f)) return "scale must be 0 (default) or at most 100";
+  if (!(t->score_cap == 0.0f || (t->score_cap >= 0.01f && t->score_cap <= 1000.0f)))
+    return "score_cap must be 0 (none) or 0.01..1000";
   return nullptr;
 }
 
