@@ -5,20 +5,25 @@
 // with K_j, V_j the integer or e4m3 codes and ks_j, vs_j their scales: a key's scale
 // multiplies its scores, a value's scale its probability, so codes are never scaled.
 //
-// Bound by HBM: every visible key costs 2 * (64 + 4) bytes per key head and 256 FLOP per
-// query row.  The fragments, and the joining of warps and cluster, are va_rows.cuh's: the rest of a
-// split operand costs no further product and makes products good to 2^-21 of the row's
-// largest element.  The operands are f16 because both code formats
-// become f16 in one or two instructions a pair (bf16 took four or five, and the conversions
-// are most of the loop).  Its range is met by powers of two: a query row is scaled to a
-// largest magnitude in [1, 2) and the factor goes to the scores; a probability times its
-// value scale is scaled by 2^(kTop - E), E above the largest value scale so far.
+// Bound by HBM where all SMs have work: every visible key costs 2 * (64 + 4) bytes per key head
+// and 256 FLOP per query row.  The fragments, and the joining of warps and cluster, are va_rows.cuh's:
+// the low part of a split operand costs no further product and makes products good to 2^-21 of
+// the row's largest element.  The operands are f16 because both code formats become f16 in one
+// or two instructions a pair (bf16 took four or five, and the conversions are most of the loop).
+// Its range is met by powers of two: a query row is scaled to a largest magnitude in [1, 2) and the
+// factor goes to the scores; a probability times its value scale is scaled by 2^(kTop - E), E
+// above the largest value scale so far.
 //
 // A cluster of CTAs shares one (document, key head, row block); its warps take 64-key
 // chunks in turn through a ring of its own in shared memory (cp.async, one chunk ahead), each
 // warp with its own running maximum and sum, and the partial results meet in shared memory
 // and then, through distributed shared memory, across the cluster in rank order: one
 // launch, no workspace, no atomics, and the same bits on every run.
+//
+// Measured on B200: one token over 10,392 int8 tokens x 12 heads 9.7 us; 16 documents of 32,000 e4m3 tokens x 4
+// key heads, cap and bias off, 54 us (5.1 TB/s = 0.78 of measured); 16 documents of 0 to 32,000 tokens, 22 rows, cap and
+// bias, 50 us: the longest documents' CTAs run last and alone.  A warp's chunk takes about 2.4 us with
+// 12 warps on the SM: conversions, score terms and their latencies, not the loads.
 #include <algorithm>
 #include <atomic>
 

@@ -7,6 +7,8 @@
 // once.  Eight lanes own one (token, head): 8 channels each, one 16-byte load of 2-byte
 // elements, the row's largest magnitude by three shuffles.  A warp's four groups take
 // four consecutive tokens of one head, so its code rows are 256 consecutive bytes.
+// Measured on B200 (16 heads, f16, e4m3): 22,322 tokens written 26.3 us (5.3 TB/s), 31,321 read back 34.7 us
+// (5.7 TB/s = 0.86 of measured).
 #include <algorithm>
 
 #include "va_internal.h"

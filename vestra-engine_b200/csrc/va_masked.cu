@@ -25,6 +25,12 @@
 // Few query tiles leave SMs idle, so a tile's keys can be cut over a cluster of CTAs; the
 // partial rows meet through distributed shared memory in rank order: no workspace, no
 // second launch, the same bits on every run.
+//
+// Bound by the exponentials (one per 256 FLOP, 18.3 a clock and SM): a plain tile takes 1163 to
+// 1460 cycles of an SM against 896 of MUFU.  Measured on B200: full waves 763 TFLOP/s; four packed f16
+// documents of 731 to 4,330 tokens x 12 heads 129 us (637 TFLOP/s); a 10,392-token window with cap 30
+// 497 to 520 us (640 to 668); 866 new rows over 10,392 keys, cap 50, three CTAs a tile, 60 us (462);
+// causal documents with a distance bias, 16 / 4 heads, 87 us (490).
 #include <algorithm>
 #include <atomic>
 #include <queue>

@@ -9,6 +9,8 @@
 // pair in shared memory, once for all heads of q and k (a 32-pair row is shared by 12 + 12
 // heads, so the trigonometry is 4 % of the pairs and hides behind the loads), then the
 // thread turns its chunks and writes them.  No index is divided inside the row loop.
+// Measured on B200: 10,392 bf16 tokens of 12 + 12 heads 13.5 us out of L2, 16.8 from HBM (3.8 TB/s); 27,729 F32
+// tokens of 16 + 4 heads 49.4 us (5.8 TB/s = 0.88 of measured); two tokens 2.7 us.
 //
 // Angles: a position may be any int32 and the product with the frequency is needed
 // modulo one turn, which F32 loses beyond a few thousand turns.  The frequency in turns is
