@@ -38,6 +38,15 @@ def _no_device_error(ctx):
     ctx.check_device()
 
 
+@pytest.fixture(autouse=True)
+def _float32_by_default():
+    """Other test modules make 64 bits torch's default."""
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(F32)
+    yield
+    torch.set_default_dtype(before)
+
+
 def gen(seed):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
@@ -499,6 +508,91 @@ def test_cache_attention_more_rows_than_tokens_held(ctx, fmt):
     kd = (codes[0][0, :, :4].double() * scales[0][0, :, :4, None].double()).transpose(0, 1)
     vd = (codes[1][0, :, :4].double() * scales[1][0, :, :4, None].double()).transpose(0, 1)
     check_attention(out[:7], *attention_ref(q[:7], kd, vd, True, 3, 0, None, 0.0), p_step=2.0 ** -15)
+
+
+SHARED = [(16, 4, 16), (10, 16, 16), (9, 8, 8), (150, 1, 5)]
+
+
+def shared_lengths(docs, cap, kind):
+    if kind == "equal":
+        return [cap - 1] * docs
+    if kind == "one":
+        return [0] * (docs - 1) + [cap]
+    r = np.random.default_rng(docs)
+    lens = [0, 1, cap, 63, 64, 65, cap - 1, 257] + [int(2 ** r.uniform(0, 13)) for _ in range(docs - 8)]
+    return [lens[i] for i in r.permutation(docs)]
+
+
+@pytest.mark.parametrize("kind", ["mixed", "equal", "one"])
+@pytest.mark.parametrize("docs,kvh,heads", SHARED)
+def test_cache_attention_documents_sharing_a_cluster(ctx, docs, kvh, heads, kind):
+    """Batches whose documents go two to a cluster: odd counts, empty documents, documents without rows and with more rows
+    than max_tokens (more blocks of rows than their neighbour), a bad document among good ones."""
+    fmt, dtype, cap = (torch.int8, BF16, 8192) if docs % 4 else (torch.float8_e4m3fn, F16, 8200)
+    g = gen(docs + len(kind))
+    lens = shared_lengths(docs, cap, kind)
+    new = [(1, 2, 0, 1, 1, 19, 1, 3)[b % 8] if kind == "mixed" else 1 for b in range(docs)]
+    cache, codes, scales = new_cache(g, docs, kvh, cap, fmt)
+    hist = np.cumsum([0] + lens)
+    k, v = randn(g, int(hist[-1]), kvh, D, dtype=dtype), randn(g, int(hist[-1]), kvh, D, dtype=dtype)
+    ctx.kv_cache_write(cache, k, v, i32(hist), i32(lens))
+    off = np.cumsum([1] + new)
+    q = (randn(g, int(off[-1]) + 2, heads, D) * 1.5).to(dtype)
+    slopes = torch.tensor([2.0 ** (-8 * (h + 1) / heads) for h in range(heads)], device="cuda")
+
+    def check(out, skip=()):
+        assert (out[:1] == 7).all() and (out[int(off[-1]):] == 7).all()
+        for b in range(docs):
+            rows = slice(int(off[b]), int(off[b + 1]))
+            if b in skip:
+                assert (out[rows] == 7).all()
+                continue
+            kd = (codes[0][b, :, :lens[b]].double() * scales[0][b, :, :lens[b], None].double()).transpose(0, 1)
+            vd = (codes[1][b, :, :lens[b]].double() * scales[1][b, :, :lens[b], None].double()).transpose(0, 1)
+            check_attention(out[rows], *attention_ref(q[rows], kd, vd, True, 5, 0, slopes, 40.0), p_step=2.0 ** -15)
+
+    def attend(out, offsets, held):
+        ctx.cache_attention(cache, q, out, offsets, held, max_tokens=2, frame=5, slopes=slopes, score_cap=40.0)
+
+    out = torch.full_like(q, 7.0)
+    attend(out, i32(off), i32(lens))
+    check(out)
+    again = torch.full_like(q, 7.0)
+    attend(again, i32(off), i32(lens))
+    assert torch.equal(out, again)
+    if kind == "mixed":
+        bad = new.index(19)
+        wrong = list(lens)
+        wrong[bad] = cap + 1
+        out = torch.full_like(q, 7.0)
+        attend(out, i32(off), i32(wrong))
+        torch.cuda.synchronize()
+        with pytest.raises(va.VestraError) as e:
+            ctx.check_device()
+        assert e.value.code == va.VA_ERR_DEVICE and "lengths" in str(e.value)
+        check(out, skip=(bad,))
+
+
+def test_cache_attention_sharing_follows_the_lengths_in_a_graph(ctx):
+    """A captured call whose lengths move on the device gives the eager call's bits at each of them."""
+    docs, kvh, cap = 16, 4, 8192
+    g = gen(3)
+    cache, codes, scales = new_cache(g, docs, kvh, cap, torch.int8)
+    k = randn(g, docs * cap, kvh, D, dtype=BF16)
+    ctx.kv_cache_write(cache, k, k, i32([cap * b for b in range(docs + 1)]), i32([cap] * docs))
+    q = randn(g, docs, 4 * kvh, D, dtype=BF16)
+    offsets, lens, out = i32(list(range(docs + 1))), i32([cap] * docs), torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ctx.cache_attention(cache, q, out, offsets, lens, max_tokens=1, stream=torch.cuda.current_stream().cuda_stream)
+    for kind in ("mixed", "one", "equal"):
+        lens.copy_(i32(shared_lengths(docs, cap, kind)))
+        out.fill_(7.0)
+        graph.replay()
+        eager = torch.empty_like(q)
+        ctx.cache_attention(cache, q, eager, offsets, lens, max_tokens=1)
+        assert torch.equal(out, eager)
+    graph.reset()
 
 
 def test_bad_lengths_are_reported_and_skipped(ctx):

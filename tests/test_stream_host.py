@@ -95,7 +95,7 @@ def test_the_mirror_refuses_host_tensors():
         va._device_array(torch.zeros(3, dtype=torch.int32), 0, "offsets", va._INT32, 3)
     with pytest.raises(va.VestraError):
         va.RopeAxes((16, 16, 16, 8, 8))
-    codes, scales = torch.zeros(1, 2, 8, 64, dtype=torch.int8), torch.zeros(1, 2, 8)
+    codes, scales = torch.zeros(1, 2, 8, 64, dtype=torch.int8), torch.zeros(1, 2, 8, dtype=torch.float32)
     cache = va.KvCache(codes, codes.clone(), scales, scales.clone())
     with pytest.raises(va.VestraError):
         cache.check_device(0)

@@ -14,18 +14,19 @@
 // factor goes to the scores; a probability times its value scale is scaled by 2^(kTop - E), E
 // above the largest value scale so far.
 //
-// A cluster of CTAs shares one (document, key head, row block); its warps take 64-key
-// chunks in turn through a ring of its own in shared memory (cp.async, one chunk ahead), each
+// A cluster of CTAs shares one (document, key head, row block), or two documents' that divide its
+// CTAs; a warp takes 64-key chunks in turn through a ring of its own in shared memory (cp.async, one chunk ahead), each
 // warp with its own running maximum and sum, and the partial results meet in shared memory
 // and then, through distributed shared memory, across the cluster in rank order: one
 // launch, no workspace, no atomics, and the same bits on every run.
 //
 // Measured on B200: one token over 10,392 int8 tokens x 12 heads 9.7 us; 16 documents of 32,000 e4m3 tokens x 4
-// key heads, cap and bias off, 54 us (5.1 TB/s = 0.78 of measured); 16 documents of 0 to 32,000 tokens, 22 rows, cap and
-// bias, 50 us: the longest documents' CTAs run last and alone.  A warp's chunk takes about 2.4 us with
-// 12 warps on the SM: conversions, score terms and their latencies, not the loads.
+// key heads, cap and bias off, 64 us in shared clusters (54 us = 5.1 TB/s with a cluster each); 16 documents of 0 to
+// 32,000 tokens, 22 rows, cap and bias, 37 us (48 with a cluster each).  A warp's chunk takes about 2.6 us with 12 warps on the SM and 1.1 us with
+// 4: some 950 instructions of conversions, score terms and softmax (58% of issue slots), not the loads.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "va_internal.h"
 #include "va_ptx.cuh"
@@ -43,6 +44,7 @@ constexpr int kChunk = 64;         // keys a warp takes at a time
 constexpr int kTiles = kChunk / 8;
 constexpr int kStages = 2;         // chunks of a warp in shared memory
 constexpr int kCtasPerSm = 3;
+constexpr int kMaxPaired = 256;    // documents that a CTA puts in order
 constexpr int kTop = 14;       // probabilities times value scales are brought below 2^kTop
 constexpr int kMinExp = -100;  // value scales below 2^-100 lose precision
 
@@ -118,38 +120,125 @@ __device__ __forceinline__ void load_chunk(Chunk& ch, const uint8_t* kc, const u
   }
 }
 
+// Two documents that share a cluster.  key: 0 without rows in this block of rows, else 1 + the length.
+struct Pair {
+  int doc[2], key[2], begin[2], tokens[2];
+};
+struct Documents {
+  int key[kMaxPaired];
+  Pair pair;
+};
+__device__ __forceinline__ bool good_document(const CacheAttnArgs& a, int32_t begin, int32_t end, int32_t len) {
+  return begin >= 0 && end >= begin && end <= a.rows && len >= 0 && len <= a.c.capacity;
+}
+// The documents in order of falling keys: number `index` and, from the other end, its mirror image (itself in the
+// middle of an odd count, and then key[1] is 0).  Every CTA counts for itself: at most 256 keys.
+__device__ __forceinline__ Pair find_pair(Documents& sh, const CacheAttnArgs& a, int index, int block0, bool report,
+                                          int* err) {
+  int32_t begin[kMaxPaired / kThreads], tokens[kMaxPaired / kThreads];
+  int key[kMaxPaired / kThreads];
+#pragma unroll
+  for (int i = 0; i < kMaxPaired / kThreads; ++i) {
+    const int doc = i * kThreads + static_cast<int>(threadIdx.x);
+    key[i] = -1;  // behind every document
+    if (doc < a.c.documents) {
+      begin[i] = __ldg(a.offsets + doc);
+      const int32_t end = __ldg(a.offsets + doc + 1), len = __ldg(a.lens + doc);
+      const bool ok = good_document(a, begin[i], end, len);
+      if (!ok && report) report_error(err, kDevBadLengths);
+      tokens[i] = ok ? end - begin[i] : 0;
+      key[i] = block0 * kRowsPerBlock < tokens[i] * a.group ? len + 1 : 0;
+    }
+    sh.key[doc] = key[i];
+  }
+  if (threadIdx.x == 0) sh.pair.key[1] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kMaxPaired / kThreads; ++i) {
+    const int doc = i * kThreads + static_cast<int>(threadIdx.x);
+    if (doc >= a.c.documents) break;
+    int ahead = 0;
+    for (int e = 0; e < a.c.documents; e += 4) {
+      const int4 k = *reinterpret_cast<const int4*>(&sh.key[e]);
+      ahead += (k.x > key[i] || (k.x == key[i] && e < doc)) + (k.y > key[i] || (k.y == key[i] && e + 1 < doc)) +
+               (k.z > key[i] || (k.z == key[i] && e + 2 < doc)) + (k.w > key[i] || (k.w == key[i] && e + 3 < doc));
+    }
+    const int place = ahead == index ? 0 : ahead == a.c.documents - 1 - index ? 1 : -1;
+    if (place >= 0) {
+      sh.pair.doc[place] = doc;
+      sh.pair.key[place] = key[i];
+      sh.pair.begin[place] = begin[i];
+      sh.pair.tokens[place] = tokens[i];
+    }
+  }
+  __syncthreads();
+  return sh.pair;
+}
+// CTAs of a cluster that the first of two documents gets: by their chunks, so that the slower one is soonest done.
+__device__ __forceinline__ int share(int key0, int key1, int cluster) {
+  if (key1 == 0) return cluster;
+  const float w0 = static_cast<float>((key0 - 1) / kChunk + 1), w1 = static_cast<float>((key1 - 1) / kChunk + 1);
+  const int n = min(max(static_cast<int>(cluster * w0 / (w0 + w1)), 1), cluster - 1);
+  const int up = min(n + 1, cluster - 1);
+  return fmaxf(w0 / up, w1 / (cluster - up)) < fmaxf(w0 / n, w1 / (cluster - n)) ? up : n;
+}
+
 struct Shared {
   union {
     Chunk ring[kWarps][kStages];
     Join<kWarps> join;  // once the block's last chunk is used
   };
-  Part part[kMaxCluster];  // [own row][cluster rank]
+  union {
+    Documents docs;          // read out before this CTA arrives at its first cluster barrier
+    Part part[kMaxCluster];  // [own row][number in the document's share], written after that barrier
+  };
 };
 static_assert(kCtasPerSm * (sizeof(Shared) + 1024) <= 228 * 1024, "shared memory of an SM");
 
-template <class T, bool kE4m3>
+template <class T, bool kE4m3, bool kPaired>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
-    cache_attn_kernel(const __grid_constant__ CacheAttnArgs a, int splits, int* err) {
+    cache_attn_kernel(const __grid_constant__ CacheAttnArgs a, int cluster, int* err) {
   extern __shared__ uint4 smem_raw[];
   Shared& smem = *reinterpret_cast<Shared*>(smem_raw);
   Join<kWarps>& sh = smem.join;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int rank = static_cast<int>(blockIdx.x) % splits;
-  int unit = static_cast<int>(blockIdx.x) / splits;
+  int rank = static_cast<int>(blockIdx.x) % cluster;
+  int unit = static_cast<int>(blockIdx.x) / cluster;
   const int kvh = unit % a.c.kv_heads;
   unit /= a.c.kv_heads;
   const int block0 = unit % a.row_blocks;
-  const int doc = unit / a.row_blocks;
+  int doc = unit / a.row_blocks;
 
-  const int32_t begin = __ldg(a.offsets + doc), end = __ldg(a.offsets + doc + 1);
-  const int32_t len = __ldg(a.lens + doc);
-  const bool ok = begin >= 0 && end >= begin && end <= a.rows && len >= 0 && len <= a.c.capacity;
-  if (!ok) {  // the same for every CTA of the cluster: none of them waits
-    if (threadIdx.x == 0) report_error(err, kDevBadLengths);
-    return;
+  // This CTA is number `rank` of the `splits` that share the document's keys; number 0 has rank `lead` in the
+  // cluster.  All CTAs of the cluster walk `most_rows`, so that they meet the same barriers.
+  int splits = cluster, lead = 0;
+  int32_t begin, len;
+  int tokens, most_rows;
+  if constexpr (kPaired) {
+    const Pair pair = find_pair(smem.docs, a, doc, block0, blockIdx.x == 0, err);
+    if (pair.key[0] == 0) return;  // neither document has rows here (key[0] >= key[1])
+    const int n = share(pair.key[0], pair.key[1], cluster);
+    const bool second = rank >= n;
+    splits = second ? cluster - n : n;
+    lead = second ? n : 0;
+    rank -= lead;
+    doc = second ? pair.doc[1] : pair.doc[0];
+    begin = second ? pair.begin[1] : pair.begin[0];
+    tokens = second ? pair.tokens[1] : pair.tokens[0];
+    len = (second ? pair.key[1] : pair.key[0]) - 1;
+    most_rows = (pair.key[1] == 0 ? pair.tokens[0] : max(pair.tokens[0], pair.tokens[1])) * a.group;
+  } else {
+    begin = __ldg(a.offsets + doc);
+    len = __ldg(a.lens + doc);
+    const int32_t end = __ldg(a.offsets + doc + 1);
+    if (!good_document(a, begin, end, len)) {  // the same for every CTA of the cluster: none of them waits
+      if (threadIdx.x == 0) report_error(err, kDevBadLengths);
+      return;
+    }
+    tokens = end - begin;
+    most_rows = tokens * a.group;
   }
-  const int tokens = end - begin;
   const int q_rows = tokens * a.group;
   const int prefix = a.prefix ? max(__ldg(a.prefix + doc), 0) : 0;
   const int64_t head_base = (static_cast<int64_t>(doc) * a.c.kv_heads + kvh) * a.c.capacity;
@@ -171,9 +260,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     return static_cast<int>(min(e, static_cast<int64_t>(len)));
   };
 
-  for (int rb = block0; rb * kRowsPerBlock < q_rows; rb += a.row_blocks) {
+  for (int rb = block0; rb * kRowsPerBlock < most_rows; rb += a.row_blocks) {
     // Every CTA of the cluster has started, and is done with the parts of the last block.
-    if (splits > 1) cluster_arrive();
+    if (cluster > 1) cluster_arrive();
+    if (kPaired && rb * kRowsPerBlock >= q_rows) {  // only the pair's other document has rows left: finish_block's barriers
+      cluster_wait();
+      cluster_arrive();
+      cluster_wait();
+      continue;
+    }
     const int r = rb * kRowsPerBlock + g;  // this lane's query row
     const bool valid = r < q_rows;
     const int token = valid ? r / a.group : tokens - 1;
@@ -330,30 +425,55 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     cp_wait<0>();
     __syncthreads();  // every warp is done with its ring: the join buffers may cover it
     const float back = __uint_as_float(static_cast<uint32_t>(v_exp - kTop + 127) << 23);  // 2^(E - kTop)
-    finish_block<T>(sh, smem.part, o, m, l, back, rb, q_rows, a.group, kvh, rank, splits, begin, a.out);
+    finish_block<T>(sh, smem.part, o, m, l, back, rb, q_rows, a.group, kvh, rank, splits, cluster, lead, begin,
+                   a.out);
     __syncthreads();  // before the next block's loads and parts
   }
 }
 
-template <class T, bool kE4m3>
-cudaError_t launch(const CacheAttnArgs& a, int splits, int64_t blocks, int* err, cudaStream_t st) {
-  auto kern = cache_attn_kernel<T, kE4m3>;
-  static std::atomic<uint64_t> ready{0};
-  cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), sizeof(Shared), ready);
-  if (e != cudaSuccess) return e;
+cudaLaunchConfig_t config(int64_t blocks, int cluster, cudaStream_t st, cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = cluster;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, a, splits, err);
+  return cfg;
+}
+
+// Clusters of a size that the current device holds at once.  The variants of the kernel are alike in
+// what limits them: registers and shared memory, for kCtasPerSm CTAs.
+cudaError_t clusters_held(int cluster, int* held) {
+  static std::atomic<int> known[64][kMaxCluster + 1];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (*held = known[dev][cluster].load(std::memory_order_relaxed)) > 0) return e;
+  auto kern = cache_attn_kernel<__half, true, true>;
+  static std::atomic<uint64_t> ready{0};
+  e = prepare_kernel(reinterpret_cast<const void*>(kern), sizeof(Shared), ready);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = config(cluster, cluster, nullptr, attr);
+  e = cudaOccupancyMaxActiveClusters(held, kern, &cfg);
+  if (e == cudaSuccess && dev < 64) known[dev][cluster].store(*held, std::memory_order_relaxed);
+  return e;
+}
+
+template <class T, bool kE4m3, bool kPaired>
+cudaError_t launch(const CacheAttnArgs& a, int cluster, int64_t blocks, int* err, cudaStream_t st) {
+  auto kern = cache_attn_kernel<T, kE4m3, kPaired>;
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), sizeof(Shared), ready);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = config(blocks, cluster, st, attr);
+  return cudaLaunchKernelEx(&cfg, kern, a, cluster, err);
 }
 
 }  // namespace
@@ -376,24 +496,42 @@ cudaError_t launch_cache_attention(const KvCacheRef& c, const AttnTerms& t, int 
   a.slopes = slopes;
   a.q = q;
   a.out = out;
-  const int64_t units = static_cast<int64_t>(c.documents) * c.kv_heads * a.row_blocks;
   // CTAs per (document, key head): the lengths are on the device, so by the capacity (at least one
   // chunk per warp) and by what the SMs hold at once, at most 8, or 16, which the GPU places less
-  // easily, where that fits.  Measured (us; S = 4 / 6 / 8 CTAs, 16 documents x 4 key heads): lengths of 0 to 32,000
-  // 59 / 50 / 42, all 32,000 56 / 54 / 68, all 8,192 18 / 19 / 23; 128 units of mixed lengths S = 2 / 3 / 4 17.3 / 15.7 /
-  // 14.9, of 4,000 18.0 / 18.8 / 20.6.  Letting the CTAs past a document's share of the work leave at once
+  // easily, where that fits.  Letting the CTAs past a document's share of the work leave at once
   // gained nothing: a cluster still waits for all its places.
   const int64_t slots = kCtasPerSm * static_cast<int64_t>(sms), pairs = static_cast<int64_t>(c.documents) * c.kv_heads;
   const int64_t most = std::max<int64_t>(1, c.capacity / (kChunk * kWarps));
   const int64_t fit = std::max<int64_t>(1, std::min(slots / pairs, most));
-  const int splits = static_cast<int>(fit >= kMaxCluster ? kMaxCluster : std::min<int64_t>(fit, 8));
-  const int64_t blocks = units * splits;
+  int cluster = static_cast<int>(fit >= kMaxCluster ? kMaxCluster : std::min<int64_t>(fit, 8));
+  bool paired = false;  // two documents share a cluster
+  int64_t shared_by = c.documents;  // clusters per key head and block of rows
+  // From 8 documents on, a long and a short one share a cluster and divide its CTAs by their lengths, where that
+  // is two to six each on average, the clusters all fit with hardly fewer CTAs, and a capacity of 8192 pays for the sorting.  Measured (us, own
+  // clusters / shared; lengths random / equal): 64 documents x 2 key heads of up to 32,000 84 / 68, 102 / 104; 20 x 4
+  // 58 / 48, 63 / 65; 16 x 12 of up to 9,000 36 / 30, 47 / 49; 16 x 4 of up to 32,000, where clusters of 10 are the largest
+  // that fit, 41 / 36, 56 / 65 (the mixed batch above 48 / 37).  Outside the rule: 4 x 16 of up to 32,000 46 / 51, 54 / 64;
+  // 8 x 4 27 / 29, 33 / 44; 16 x 12 of up to 2,000 11.4 / 11.7, 14.7 / 15.9.
+  if (fit >= 2 && fit <= 6 && c.documents >= 8 && c.documents <= kMaxPaired && c.capacity >= 8192) {
+    const int64_t both = (c.documents + 1) / 2;
+    for (int s = 2 * static_cast<int>(fit); 3 * s >= 5 * fit && !paired; s -= 2) {
+      int held = 0;
+      const cudaError_t e = clusters_held(s, &held);
+      if (e != cudaSuccess) return e;
+      if (held < both * c.kv_heads) continue;
+      paired = true;
+      cluster = s;
+      shared_by = both;
+    }
+  }
+  const int64_t blocks = shared_by * c.kv_heads * a.row_blocks * cluster;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-  if (c.e4m3)
-    return dtype == kF16 ? launch<__half, true>(a, splits, blocks, err, st)
-                         : launch<__nv_bfloat16, true>(a, splits, blocks, err, st);
-  return dtype == kF16 ? launch<__half, false>(a, splits, blocks, err, st)
-                       : launch<__nv_bfloat16, false>(a, splits, blocks, err, st);
+  auto go = [&](auto type, auto e4m3) {
+    return paired ? launch<decltype(type), e4m3.value, true>(a, cluster, blocks, err, st)
+                  : launch<decltype(type), e4m3.value, false>(a, cluster, blocks, err, st);
+  };
+  if (c.e4m3) return dtype == kF16 ? go(__half(), std::true_type()) : go(__nv_bfloat16(), std::true_type());
+  return dtype == kF16 ? go(__half(), std::false_type()) : go(__nv_bfloat16(), std::false_type());
 }
 
 }  // namespace va

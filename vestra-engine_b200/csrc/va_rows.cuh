@@ -169,7 +169,7 @@ struct Join {
   float o[kWarps][kRowsPerBlock][kHeadDim + 8];
   float m[kWarps][kRowsPerBlock], l[kWarps][kRowsPerBlock];
 };
-// What the cluster's CTAs send to the CTA that finishes a row: rows r, r + splits, ... go to
+// What the CTAs of a document send to the CTA that finishes a row: rows r, r + splits, ... go to
 // CTA r % splits, so a CTA receives at most 16 (splits x rows) parts.
 struct Part {
   float o[kHeadDim];
@@ -185,11 +185,13 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Joins the warps' results of a row block (o, m, l of every lane; `back` undoes a scaling of o) and
-// the cluster's, and writes the block's rows.  base: output row of the first token; rb: the block.
+// the cluster's, and writes the block's rows.  base: output row of the first token; rb: the block.  The `splits` CTAs that share the
+// document's keys stand in a cluster of `cluster` from rank `lead` on; the caller has arrived at the cluster's barrier once,
+// and every CTA of the cluster takes part in two more phases here (or stands in for them).
 template <class T, int kWarps>
 __device__ __forceinline__ void finish_block(Join<kWarps>& sh, Part* parts, const float (&o)[8][4], float m, float l,
                                              float back, int rb, int q_rows, int group, int kvh, int rank, int splits,
-                                             int64_t base, const HeadsRef& out) {
+                                             int cluster, int lead, int64_t base, const HeadsRef& out) {
   constexpr int kThreads = kWarps * 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -209,7 +211,7 @@ __device__ __forceinline__ void finish_block(Join<kWarps>& sh, Part* parts, cons
     }
   }
   __syncthreads();
-  if (splits > 1) cluster_wait();
+  if (cluster > 1) cluster_wait();
   // Join the warps and hand each row to the CTA that finishes it.
   for (int i = threadIdx.x; i < rows * kHeadDim; i += kThreads) {
     const int row = i / kHeadDim, at = i % kHeadDim;
@@ -225,13 +227,13 @@ __device__ __forceinline__ void finish_block(Join<kWarps>& sh, Part* parts, cons
     }
     const int owner = row % splits;
     Part& to = parts[row / splits * splits + rank];
-    st_cluster(&to.o[at], owner, os);
+    st_cluster(&to.o[at], lead + owner, os);
     if (at == 0) {
-      st_cluster(&to.m, owner, mt);
-      st_cluster(&to.l, owner, ls);
+      st_cluster(&to.m, lead + owner, mt);
+      st_cluster(&to.l, lead + owner, ls);
     }
   }
-  if (splits > 1) {
+  if (cluster > 1) {
     cluster_arrive();
     cluster_wait();
   } else {

@@ -213,7 +213,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) rows_attn_kernel(const _
   }
   cp_wait<0>();
   __syncthreads();  // every warp is done with its ring: the join buffers may cover it
-  finish_block<T>(smem.join, smem.part, o, m, l, 1.0f, rb, q_rows, group, kvh, rank, a.splits, it.q_row, a.m.out);
+  finish_block<T>(smem.join, smem.part, o, m, l, 1.0f, rb, q_rows, group, kvh, rank, a.splits, a.splits, 0, it.q_row,
+                  a.m.out);
 }
 
 template <class T>
