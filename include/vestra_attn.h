@@ -482,7 +482,8 @@ int va_kv_cache_read_device(va_ctx* ctx, const va_kv_cache* cache, int64_t rows,
  * strides multiples of 8 elements.  Bad offsets, or lens outside [0, capacity]: as
  * above, and the document's rows of out are left as they were.  For many new tokens
  * read the cache back and run va_masked_attention_device.  The codes of the tokens held
- * must not be e4m3's NaN (writing never makes one). */
+ * must not be e4m3's NaN (writing never makes one).  The same call gives the same bits; how
+ * a document's keys are split, and so its last bits, follows the batch's sizes and lengths. */
 int va_cache_attention_device(va_ctx* ctx, const va_kv_cache* cache, const va_attn_terms* terms, int64_t rows,
                               const int32_t* offsets, const int32_t* lens, int max_tokens, const int32_t* prefix,
                               const float* slopes, const va_heads* q, const va_heads* out, void* stream);
