@@ -595,6 +595,27 @@ def test_cache_attention_sharing_follows_the_lengths_in_a_graph(ctx):
     graph.reset()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("held", [3, 64, 130])
+def test_cache_attention_hidden_non_finite_heads(ctx, fmt, held):
+    """A token whose value (or key) head is not finite reaches the rows that see it, and no other."""
+    g = gen(held)
+    cache, codes, scales = new_cache(g, 1, 1, 256, fmt)
+    k, v = randn(g, held, 1, D, dtype=BF16), randn(g, held, 1, D, dtype=BF16)
+    v[held - 1, 0, 5] = float("nan")
+    q = randn(g, 3, 1, D, dtype=BF16)
+    for key_too in (False, True):
+        if key_too:
+            k[held - 1, 0, 7] = float("inf")
+        ctx.kv_cache_write(cache, k, v, i32([0, held]), i32([held]))
+        out = torch.empty_like(q)
+        ctx.cache_attention(cache, q, out, i32([0, 3]), i32([held]), max_tokens=3)
+        kd = (codes[0][0, :, :held - 1].double() * scales[0][0, :, :held - 1, None].double()).transpose(0, 1)
+        vd = (codes[1][0, :, :held - 1].double() * scales[1][0, :, :held - 1, None].double()).transpose(0, 1)
+        check_attention(out[:2], *attention_ref(q[:2], kd, vd, True, 1, 0, None, 0.0), p_step=2.0 ** -15)
+        assert torch.isnan(out[2]).all()
+
+
 def test_bad_lengths_are_reported_and_skipped(ctx):
     """Offsets and lengths live on the device; a bad document is skipped by bounds checks in
     the kernels and reported by check_device."""

@@ -20,10 +20,12 @@
 // and then, through distributed shared memory, across the cluster in rank order: one
 // launch, no workspace, no atomics, and the same bits on every run.
 //
-// Measured on B200: one token over 10,392 int8 tokens x 12 heads 9.7 us; 16 documents of 32,000 e4m3 tokens x 4
-// key heads, cap and bias off, 64 us in shared clusters (54 us = 5.1 TB/s with a cluster each); 16 documents of 0 to
-// 32,000 tokens, 22 rows, cap and bias, 37 us (48 with a cluster each).  A warp's chunk takes about 2.6 us with 12 warps on the SM and 1.1 us with
-// 4: some 950 instructions of conversions, score terms and softmax (58% of issue slots), not the loads.
+// Measured on B200: one token over 10,392 int8 tokens x 12 heads 9.7 us; 16 documents of 0 to 32,000 e4m3
+// tokens, 22 rows, 4 key heads, cap and bias, 36 us; 16 documents of 32,000, cap and bias off, 61 us (4.6 TB/s), and x 16
+// key heads 190 us (5.9 TB/s = 0.9 of measured).  A warp's chunk takes about 2.5 us with 12 warps on the SM and 1.1 us
+// with 4: some 900 instructions of conversions, score terms and softmax (58% of issue slots), not the loads.
+// Masks are applied to chunks that some row does not see whole only, and scales lie in the order of the
+// fragments (with one product per value scale: 37.4 -> 36.0 us, 64 -> 61, 3 to 5% elsewhere).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -87,6 +89,9 @@ struct Chunk {
   uint8_t v[kChunk][kHeadDim];
   float ks[kChunk], vs[kChunk];
 };
+// Place of a key's scales within 32: the two keys of a lane in the score fragments (tile_key's order) are
+// neighbours.  Its own inverse.
+__device__ __forceinline__ int scale_at(int key) { return key ^ ((key >> 1) & 1); }
 // Rows past `last` repeat it (they are hidden, and the codes of any row held are finite).
 __device__ __forceinline__ void load_chunk(Chunk& ch, const uint8_t* kc, const uint8_t* vc, const float* ks,
                                            const float* vs, int key0, int last, int lane) {
@@ -101,8 +106,8 @@ __device__ __forceinline__ void load_chunk(Chunk& ch, const uint8_t* kc, const u
     }
 #pragma unroll
     for (int i = 0; i < kChunk; i += 32) {
-      cp4(&ch.ks[i + lane], ks + key0 + i + lane);
-      cp4(&ch.vs[i + lane], vs + key0 + i + lane);
+      cp4(&ch.ks[i + scale_at(lane)], ks + key0 + i + lane);
+      cp4(&ch.vs[i + scale_at(lane)], vs + key0 + i + lane);
     }
   } else {
 #pragma unroll
@@ -114,8 +119,8 @@ __device__ __forceinline__ void load_chunk(Chunk& ch, const uint8_t* kc, const u
 #pragma unroll
     for (int i = 0; i < kChunk; i += 32) {
       const int64_t key = min(key0 + i + lane, last);
-      cp4(&ch.ks[i + lane], ks + key);
-      cp4(&ch.vs[i + lane], vs + key);
+      cp4(&ch.ks[i + scale_at(lane)], ks + key);
+      cp4(&ch.vs[i + scale_at(lane)], vs + key);
     }
   }
 }
@@ -273,8 +278,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const bool valid = r < q_rows;
     const int token = valid ? r / a.group : tokens - 1;
     const int head = kvh * a.group + (valid ? r % a.group : 0);
-    const int limit = valid ? limit_of(token) : 0;
     const int block_limit = limit_of(min(rb * kRowsPerBlock + kRowsPerBlock - 1, q_rows - 1) / a.group);
+    const int limit = valid ? limit_of(token) : block_limit;
     const int fp = frame_index(token + len - tokens, a.t.frame, a.frame_magic);
     const float slope = a.slopes ? __ldg(a.slopes + head) * kLog2e : 0.0f;
 
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         if (next < chunks) load_chunk(ring[to], kc, vc, ks, vs, next * kChunk, len - 1, lane);
         cp_commit();
       }
-      const Chunk& cur = ring[stage];
+      Chunk& cur = ring[stage];
       stage = stage + 1 == kStages ? 0 : stage + 1;
       const int key0 = ch * kChunk;
       // Scores of 8 rows x 32 keys: lane (g, c) gets row g, columns 2c and 2c + 1 of each tile.
@@ -355,10 +360,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         for (int t = 0; t < kTiles; ++t)
           mma(__half(), d[t], qa[s], codes_to_f16x2<kE4m3, false>(w[t][s]), codes_to_f16x2<kE4m3, true>(w[t][s]));
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
+      for (int t = 0; t < kTiles; ++t) {
+        const float2 k_scale = *reinterpret_cast<const float2*>(&cur.ks[8 * t + 2 * c]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) x[t][e] = (d[t][e] + d[t][2 + e]) * cur.ks[8 * t + ((2 * c + e) ^ (c & 1))];
-      apply_terms(x, a.t, score_scale, cap_scale, a.slopes != nullptr, slope, fp, key0, limit, c, a.frame_magic);
+        for (int e = 0; e < 2; ++e) x[t][e] = (d[t][e] + d[t][2 + e]) * (e ? k_scale.y : k_scale.x);
+      }
+      const bool cut = apply_terms(x, a.t, score_scale, cap_scale, a.slopes != nullptr, slope, fp, key0, limit, c, a.frame_magic);
       float top = x[0][0];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) top = max3f(top, x[t][0], x[t][1]);
@@ -371,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
       for (int i = 0; i < kChunk; i += 32) {
         const uint32_t vbits = __float_as_uint(cur.vs[i + lane]);
-        if (key0 + i + lane < block_limit && vbits < 0x7f800000u) vmax = max(vmax, vbits);
+        if (key0 + i + scale_at(lane) < block_limit && vbits < 0x7f800000u) vmax = max(vmax, vbits);
       }
       const uint32_t vtop = __reduce_max_sync(0xffffffffu, vmax);
       const int e_new = max(v_exp, static_cast<int>(vtop >> 23) - 126);
@@ -390,6 +397,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const float base = m == -INFINITY ? 0.0f : m;
       const float v_scale = __uint_as_float(static_cast<uint32_t>(kTop - v_exp + 127) << 23);  // 2^(kTop - E)
 #pragma unroll
+      for (int i = 0; i < kChunk; i += 32) cur.vs[i + lane] *= v_scale;
+      __syncwarp();
+#pragma unroll
       for (int u = 0; u < kTiles / 2; ++u) {
         uint32_t pa[4];
         uint2 vw[4];
@@ -397,14 +407,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         for (int half = 0; half < 2; ++half) {
           const int t = 2 * u + half;
           float w[2];
+          const float2 v_sc = *reinterpret_cast<const float2*>(&cur.vs[8 * t + 2 * c]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int kk = 8 * t + ((2 * c + e) ^ (c & 1));
             vw[2 * half + e] = *reinterpret_cast<const uint2*>(&cur.v[kk][(8 * g) ^ ((kk << 3) & 32)]);
             const float p = ex2(x[t][e] - base);
             l += p;
-            // A hidden key's value scale may be anything (stale rows): not multiplied.
-            w[e] = x[t][e] == -INFINITY ? 0.0f : p * (cur.vs[kk] * v_scale);
+            w[e] = p * (e ? v_sc.y : v_sc.x);
+          }
+          if (cut) {  // a hidden key's value scale may be anything (stale rows)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) w[e] = x[t][e] == -INFINITY ? 0.0f : w[e];
           }
           split2(__half(), w[0], w[1], pa[2 * half], pa[2 * half + 1]);
         }

@@ -94,8 +94,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) rows_attn_kernel(const _
   const bool valid = r < q_rows;
   const int token = valid ? r / group : it.tokens - 1;
   const int head = kvh * group + (valid ? r - token * group : 0);
-  const int limit = valid ? limit_of(token) : 0;
   const int block_limit = limit_of(min(rb * kRowsPerBlock + kRowsPerBlock - 1, q_rows - 1) / group);
+  const int limit = valid ? limit_of(token) : block_limit;
   const int fp = frame_index(it.first + token, t.frame, a.frame_magic);
   const float slope = a.m.slopes ? __ldg(a.m.slopes + head) : 0.0f;
 
