@@ -22,7 +22,7 @@
 //
 // Measured on B200: one token over 10,392 int8 tokens x 12 heads 9.7 us; 16 documents of 0 to 32,000 e4m3
 // tokens, 22 rows, 4 key heads, cap and bias, 36 us; 16 documents of 32,000, cap and bias off, 61 us (4.6 TB/s), and x 16
-// key heads 190 us (5.9 TB/s = 0.9 of measured).  A warp's chunk takes about 2.5 us with 12 warps on the SM and 1.1 us
+// key heads 188 us (5.9 TB/s = 0.90 of measured).  A warp's chunk takes about 2.5 us with 12 warps on the SM and 1.1 us
 // with 4: some 900 instructions of conversions, score terms and softmax (58% of issue slots), not the loads.
 // Masks are applied to chunks that some row does not see whole only, and scales lie in the order of the
 // fragments (with one product per value scale: 37.4 -> 36.0 us, 64 -> 61, 3 to 5% elsewhere).
