@@ -291,6 +291,18 @@ __device__ __forceinline__ void row_maxima(const float* s, float* mx) {
   }
 }
 
+// Scores of rows from `rows` on become 0: they belong to no row of the tile, so they may not take part in a
+// choice that the warp makes together.
+__device__ __forceinline__ void drop_rows(float* s, const int* row, int rows) {
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (row[0] >= rows) s[4 * k + e] = 0.0f;
+      if (row[1] >= rows) s[4 * k + 2 + e] = 0.0f;
+    }
+}
+
 // Scores of the thread's columns (relative to its first) from lim[i] on become v.
 __device__ __forceinline__ void hide(float* s, const int* lim, float v) {
 #pragma unroll
@@ -517,6 +529,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint32_t tS = tmem + lane_off + kColS, tP = tmem + lane_off + kColP, tO = tmem + lane_off + kColO;
     const int c0 = 2 * (lane & 3);  // first of the thread's column pair in every 8 columns
     const bool warp_live = lane_base < g.rows;
+    // The warp's last rows are past the tile's: another document's queries, or, where the heads that share a
+    // key head do not divide 128, what an earlier CTA left in shared memory.
+    const bool ragged = lane_base + 16 > g.rows;
     // The thread's two rows of the tile.
     int limit[2], row[2];
     int frame[2];
@@ -566,6 +581,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       tmem_ld_16x256b_x16(tS, s);
       tc_fence_before();
       warp_arrive(c.s_free());  // QK of the next tile may overwrite S
+      if constexpr (kCap) {
+        if (ragged) drop_rows(s, row, g.rows);  // the range of the scores chooses the form of the cap
+      }
       const int k0 = (g.t0 + j) * kTile;
       const bool partial = __any_sync(0xffffffffu, min(limit[0], limit[1]) < k0 + kTile);
       const int lim[2] = {limit[0] - k0 - c0, limit[1] - k0 - c0};
