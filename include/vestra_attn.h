@@ -417,9 +417,9 @@ typedef struct va_attn_terms {
  * the context's device.  All arrays are host arrays, read during the call:
  * q_offsets, k_offsets [documents + 1] ascending from >= 0, below 2^31 rows, at most
  * 2^24 keys per document; prefix [documents] >= 0 or NULL; slopes [heads] finite or
- * NULL.  Create allocates device memory (not during a capture); a plan serves any
- * number of calls, also at once, and is destroyed when none is running, and before
- * its context. */
+ * NULL.  Create allocates device memory (not during a capture) and returns with the plan
+ * on the device, ready for any stream; a plan serves any number of calls, also at once, and
+ * is destroyed when none is running, and before its context. */
 typedef struct va_attn_plan va_attn_plan;
 int va_attn_plan_create(va_ctx* ctx, const va_attn_terms* terms, int documents, const int64_t* q_offsets,
                         const int64_t* k_offsets, const int64_t* prefix, const float* slopes,

@@ -79,3 +79,22 @@ def test_capped_output_over_its_queries(ctx, heads, kvh, keys):
         x = q.clone()
         ctx.masked_attention(plan, x, k, v, x)
         assert torch.equal(x, want)
+
+
+# ------------------------------------------------------------------------------- plans
+def test_plans_used_at_once_on_a_stream_of_their_own(ctx):
+    """A plan's first launch goes to a stream that does not wait for the legacy stream, right after create."""
+    g = gen(11)
+    st = torch.cuda.Stream()
+    q, k, v = (randn(g, 900, 2, D, dtype=BF16) for _ in range(3))
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    ends = [[0, 900], [0, 3, 500, 900], [0, 1], [0, 130, 131]]
+    for i in range(60):
+        e = ends[i % len(ends)]
+        slopes = slopes_of(2) * (1 + i % 3)
+        torch.cuda.synchronize()
+        plan = va.AttentionPlan(ctx, 2, 2, e, e, causal=True, slopes=slopes)
+        ctx.masked_attention(plan, q, k, v, out, stream=st.cuda_stream)
+        torch.cuda.synchronize()
+        ctx.masked_attention(plan, q, k, v, want)
+        assert torch.equal(out[:e[-1]], want[:e[-1]])

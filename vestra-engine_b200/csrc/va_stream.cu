@@ -195,12 +195,16 @@ void free_plan(va_attn_plan* p) {
   delete p;
 }
 
+// On the legacy stream; from pageable memory the copy may still be under way on return (finish_uploads).
 template <class T>
 cudaError_t upload(T** dst, const T* src, size_t n) {
   cudaError_t e = cudaMalloc(reinterpret_cast<void**>(dst), n * sizeof(T));
   if (e == cudaSuccess) e = cudaMemcpy(*dst, src, n * sizeof(T), cudaMemcpyHostToDevice);
   return e;
 }
+
+// Waits for the uploads: a plan's first launch may be on a stream that does not wait for the legacy one.
+cudaError_t finish_uploads() { return cudaStreamSynchronize(cudaStreamLegacy); }
 
 const char* check_cache(const va_kv_cache* c) {
   if (!c) return "the cache is missing";
@@ -385,6 +389,7 @@ int va_attn_plan_create(va_ctx* c, const va_attn_terms* terms, int documents, co
     cudaError_t e = scope.error();
     if (e == cudaSuccess && !p->items.empty()) e = upload(&p->dev_items, p->items.data(), p->items.size());
     if (e == cudaSuccess && slopes) e = upload(&p->dev_slopes, s.data(), s.size());
+    if (e == cudaSuccess) e = finish_uploads();
     if (e != cudaSuccess) {
       free_plan(p);
       return launched(c, e, "attention plan upload");
