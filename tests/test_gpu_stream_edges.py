@@ -98,3 +98,90 @@ def test_plans_used_at_once_on_a_stream_of_their_own(ctx):
         torch.cuda.synchronize()
         ctx.masked_attention(plan, q, k, v, want)
         assert torch.equal(out[:e[-1]], want[:e[-1]])
+
+
+# ------------------------------------------------------------------ values of unlike size
+def close(got, ref, a, keys, p_step=2.0 ** -15):
+    """As check_attention, with another absolute part: outputs here may be as small as 1e-30.  The row's weights
+    p * scale are brought to a largest of 2^7 or more and held in two f16 parts, so each is off by at most 2^-25,
+    2^-32 of the largest weight.  A code is at most twice its head's largest one, and the largest weight times that
+    head's largest value is at most the largest A of the row."""
+    tol = half_step(got.dtype) * ref.abs() + (p_step + 2.0 ** -12) * a + keys * 2.0 ** -31 * a.amax(-1, keepdim=True)
+    assert ((got.double() - ref).abs() <= tol).all(), f"{((got.double() - ref).abs() / tol).max().item():.3g} of the tolerance"
+
+
+def held_values(codes, scales, n):
+    return [(c[0, :, :n].double() * s[0, :, :n, None].double()).transpose(0, 1) for c, s in zip(codes, scales)]
+
+
+FORMATS = [torch.int8, torch.float8_e4m3fn]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("power", [20, 30, 45, -45])
+@pytest.mark.parametrize("held", [2, 64, 65, 130])
+def test_hidden_token_with_values_of_another_size(ctx, fmt, held, power):
+    """The last token's values are 2^power times the others'; the earlier rows do not see it."""
+    g = gen(held)
+    cache, codes, scales = new_cache(g, 1, 1, 256, fmt)
+    k, v = randn(g, held, 1, D), randn(g, held, 1, D)
+    v[held - 1] *= 2.0 ** power
+    ctx.kv_cache_write(cache, k, v, i32([0, held]), i32([held]))
+    q = randn(g, 2, 1, D, dtype=BF16)
+    out = torch.empty_like(q)
+    ctx.cache_attention(cache, q, out, i32([0, 2]), i32([held]), max_tokens=2)
+    close(out, *attention_ref(q, *held_values(codes, scales, held), True, 1, 0, None, 0.0), held)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("at", [0, 100, 299])
+@pytest.mark.parametrize("score,power", [(-40.0, 30), (-80.0, 60), (-300.0, 100), (40.0, -60), (-8.0, 45)])
+def test_token_that_hardly_counts_with_values_of_another_size(ctx, fmt, at, score, power):
+    """Every row sees the token, but its probability makes it count little (or, at -8, all)."""
+    g = gen(at + 1)
+    held = 300
+    cache, codes, scales = new_cache(g, 1, 1, 512, fmt)
+    q = torch.full((1, 2, D), 1.0, device="cuda", dtype=BF16)
+    k, v = randn(g, held, 1, D) * 0.05, randn(g, held, 1, D)
+    k[at] = score / 8  # q . k / sqrt(64) = score
+    v[at] *= 2.0 ** power
+    ctx.kv_cache_write(cache, k, v, i32([0, held]), i32([held]))
+    out = torch.empty_like(q)
+    ctx.cache_attention(cache, q, out, i32([0, 1]), i32([held]), max_tokens=1)
+    close(out, *attention_ref(q, *held_values(codes, scales, held), True, 1, 0, None, 0.0), held)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("size", [1e-28, 1e-4, 1e6, 1e30])
+def test_values_of_one_size(ctx, fmt, size):
+    """All values tiny or huge; scores that grow from chunk to chunk, so the sums are rescaled often."""
+    g = gen(5)
+    held = 1000
+    cache, codes, scales = new_cache(g, 1, 2, 1024, fmt)
+    k, v = randn(g, held, 2, D) * 0.1, randn(g, held, 2, D) * size
+    k += torch.linspace(-2, 2, held, device="cuda")[:, None, None]
+    v *= torch.exp2(torch.linspace(10, -10, held, device="cuda"))[:, None, None]
+    ctx.kv_cache_write(cache, k, v, i32([0, held]), i32([held]))
+    q = torch.full((4, 4, D), 0.5, device="cuda", dtype=BF16)
+    out = torch.empty_like(q)
+    ctx.cache_attention(cache, q, out, i32([0, 4]), i32([held]), max_tokens=4)
+    close(out, *attention_ref(q, *held_values(codes, scales, held), True, 1, 0, None, 0.0), held)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("held", [2, 64, 65, 130, 600])
+def test_hidden_tokens_do_not_change_a_bit(ctx, fmt, held):
+    """Rows that do not see the last two tokens, whatever those hold."""
+    g = gen(held)
+    cache, codes, scales = new_cache(g, 1, 2, 640, fmt)
+    k, v = randn(g, held, 2, D), randn(g, held, 2, D) * torch.exp2(torch.randint(0, 6, (held, 1, 1), generator=g, device="cuda"))
+    q = randn(g, 3, 4, D, dtype=BF16)
+    outs = []
+    for power in (0, 5, 45, 100, -100):
+        x = v.clone()
+        x[max(0, held - 2):] *= 2.0 ** power
+        ctx.kv_cache_write(cache, k, x, i32([0, held]), i32([held]))
+        outs.append(torch.empty_like(q))
+        ctx.cache_attention(cache, q, outs[-1], i32([0, 3]), i32([held]), max_tokens=3)
+    for out in outs[1:]:
+        assert torch.equal(out[0], outs[0][0])

@@ -11,8 +11,15 @@
 // the row's largest element.  The operands are f16 because both code formats become f16 in one
 // or two instructions a pair (bf16 took four or five, and the conversions are most of the loop).
 // Its range is met by powers of two: a query row is scaled to a largest magnitude in [1, 2) and the
-// factor goes to the scores; a probability times its value scale is scaled by 2^(kTop - E), E
-// above the largest value scale so far.
+// factor goes to the scores; a weight (a probability times its value scale) is scaled by 2^(kTop - E).
+//   While every row sees the whole chunk and the warp's value scales so far lie within 2^kAlike, E is just above
+//   the largest of them, for all rows: the key of a row's maximum has probability 1, so the row's largest
+//   weight is at least 2^(E - 1 - kAlike).
+//   From the first chunk on where this does not hold, each row has its own E, above its own largest weight: a
+//   key that the row does not see, or that hardly counts in it, must not take the range from the others, whatever
+//   the values' sizes.
+// Either way a scaled weight has steps of 2^-24 and the row's largest is 2^(kTop - 1 - kAlike) or more.
+// One E per row in every chunk would cost 2 to 6 % (the weights' maximum stands between the scores and the product).
 //
 // A cluster of CTAs shares one (document, key head, row block), or two documents' that divide its
 // CTAs; a warp takes 64-key chunks in turn through a ring of its own in shared memory (cp.async, one chunk ahead), each
@@ -47,8 +54,9 @@ constexpr int kTiles = kChunk / 8;
 constexpr int kStages = 2;         // chunks of a warp in shared memory
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxPaired = 256;    // documents that a CTA puts in order
-constexpr int kTop = 14;       // probabilities times value scales are brought below 2^kTop
-constexpr int kMinExp = -100;  // value scales below 2^-100 lose precision
+constexpr int kTop = 14;       // weights are brought below 2^kTop
+constexpr int kAlike = 6;
+constexpr int kMinExp = -100;  // weights below 2^-100 lose precision
 
 struct CacheAttnArgs {
   KvCacheRef c;
@@ -79,6 +87,13 @@ __device__ __forceinline__ uint32_t codes_to_f16x2(uint32_t w) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0x64806480u));  // - (1024 + 128)
   }
   return r;
+}
+
+// 2^e: 0 below the normal range, infinity above.
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float(static_cast<uint32_t>(min(max(e + 127, 0), 255)) << 23); }
+// The least e >= kMinExp with w < 2^e (128 for what is not finite).
+__device__ __forceinline__ int exponent_above(uint32_t bits) {
+  return min(max(static_cast<int>(bits >> 23) - 126, kMinExp), 128);
 }
 
 // A warp's ring of chunks in shared memory, filled by cp.async (16 bytes of codes, 4 of
@@ -320,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       }
     }
     const float score_scale = q_scale * a.t.scale_log2, cap_scale = q_scale * a.t.cap_in;
-    int v_exp = kMinExp;  // E: every visible value scale so far is below 2^E
+    int w_exp = kMinExp;  // E: the row's weights so far are below 2^E
 
     float o[8][4];
 #pragma unroll
@@ -329,31 +344,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    int stage = 0;
-    for (int ch = first; ch < chunks; ch += stride) {
+    int stage = 0, ch = first;
+    Chunk* cur = ring;
+    auto fetch = [&] {
       cp_wait<kStages - 2>();
       __syncwarp();  // every lane's copies have landed, and the stage below is read out
-      {
-        const int next = ch + (kStages - 1) * stride;
-        const int to = stage == 0 ? kStages - 1 : stage - 1;
-        if (next < chunks) load_chunk(ring[to], kc, vc, ks, vs, next * kChunk, len - 1, lane);
-        cp_commit();
-      }
-      Chunk& cur = ring[stage];
+      const int next = ch + (kStages - 1) * stride;
+      const int to = stage == 0 ? kStages - 1 : stage - 1;
+      if (next < chunks) load_chunk(ring[to], kc, vc, ks, vs, next * kChunk, len - 1, lane);
+      cp_commit();
+      cur = ring + stage;
       stage = stage + 1 == kStages ? 0 : stage + 1;
-      const int key0 = ch * kChunk;
-      // Scores of 8 rows x 32 keys: lane (g, c) gets row g, columns 2c and 2c + 1 of each tile.
-      float x[kTiles][2], d[kTiles][4];
+    };
+    // Scores of 8 rows x 64 keys: lane (g, c) gets row g, columns 2c and 2c + 1 of each tile.
+    auto score = [&](float(&x)[kTiles][2]) {
+      float d[kTiles][4];
       uint32_t w[kTiles][4];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         const int kr = 8 * t + tile_key(g);
-        const uint4 kw = *reinterpret_cast<const uint4*>(&cur.k[kr][16 * (c ^ ((kr >> 1) & 2))]);
+        const uint4 kw = *reinterpret_cast<const uint4*>(&cur->k[kr][16 * (c ^ ((kr >> 1) & 2))]);
         w[t][0] = flip<kE4m3>(kw.x), w[t][1] = flip<kE4m3>(kw.y), w[t][2] = flip<kE4m3>(kw.z), w[t][3] = flip<kE4m3>(kw.w);
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[t][e] = 0.0f;
       }
-      // Four independent chains: a tile's four steps follow each other, the tiles do not.
+      // Eight independent chains: a tile's four steps follow each other, the tiles do not.
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -361,44 +376,35 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           mma(__half(), d[t], qa[s], codes_to_f16x2<kE4m3, false>(w[t][s]), codes_to_f16x2<kE4m3, true>(w[t][s]));
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        const float2 k_scale = *reinterpret_cast<const float2*>(&cur.ks[8 * t + 2 * c]);
+        const float2 k_scale = *reinterpret_cast<const float2*>(&cur->ks[8 * t + 2 * c]);
 #pragma unroll
         for (int e = 0; e < 2; ++e) x[t][e] = (d[t][e] + d[t][2 + e]) * (e ? k_scale.y : k_scale.x);
       }
-      const bool cut = apply_terms(x, a.t, score_scale, cap_scale, a.slopes != nullptr, slope, fp, key0, limit, c, a.frame_magic);
+    };
+    // The row's maximum with this chunk.
+    auto maximum = [&](const float(&x)[kTiles][2]) {
       float top = x[0][0];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) top = max3f(top, x[t][0], x[t][1]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float m_new = fmaxf(m, top);
-      // The largest value scale of the keys some row sees (NaN and infinity set no scale; they
-      // reach the rows that see them on their own).
-      uint32_t vmax = 0;
+      return fmaxf(m, top);
+    };
+    // A new maximum (alpha = 2^(m - m_new)) and a new E for the sums so far.
+    auto rescale = [&](float m_new, float alpha, int e_new) {
+      l *= alpha;
+      // E falls only as alpha does, so the product stays in range.
+      const float f = alpha * exp2i(max(min(w_exp - e_new, 127), -126));
+      w_exp = e_new;
+      // Accumulator rows g (elements 0, 1) and g + 8 (2, 3) are parts of query row g.
 #pragma unroll
-      for (int i = 0; i < kChunk; i += 32) {
-        const uint32_t vbits = __float_as_uint(cur.vs[i + lane]);
-        if (key0 + i + scale_at(lane) < block_limit && vbits < 0x7f800000u) vmax = max(vmax, vbits);
-      }
-      const uint32_t vtop = __reduce_max_sync(0xffffffffu, vmax);
-      const int e_new = max(v_exp, static_cast<int>(vtop >> 23) - 126);
-      if (__any_sync(0xffffffffu, m_new > m) || e_new > v_exp) {
-        float alpha = m_new > m ? ex2(m - m_new) : 1.0f;  // 0 for the first keys
-        l *= alpha;
-        alpha *= __uint_as_float(static_cast<uint32_t>(max(v_exp - e_new, -126) + 127) << 23);
-        v_exp = e_new;
-        // Accumulator rows g (elements 0, 1) and g + 8 (2, 3) are parts of query row g.
+      for (int n = 0; n < 8; ++n)
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][e] *= alpha;
-        m = m_new;
-      }
-      const float base = m == -INFINITY ? 0.0f : m;
-      const float v_scale = __uint_as_float(static_cast<uint32_t>(kTop - v_exp + 127) << 23);  // 2^(kTop - E)
-#pragma unroll
-      for (int i = 0; i < kChunk; i += 32) cur.vs[i + lane] *= v_scale;
-      __syncwarp();
+        for (int e = 0; e < 4; ++e) o[n][e] *= f;
+      m = m_new;
+    };
+    // o += weights * values; weight(t, e) of the lane's keys, in order.
+    auto add_values = [&](auto weight) {
 #pragma unroll
       for (int u = 0; u < kTiles / 2; ++u) {
         uint32_t pa[4];
@@ -406,21 +412,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int t = 2 * u + half;
-          float w[2];
-          const float2 v_sc = *reinterpret_cast<const float2*>(&cur.vs[8 * t + 2 * c]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int kk = 8 * t + ((2 * c + e) ^ (c & 1));
-            vw[2 * half + e] = *reinterpret_cast<const uint2*>(&cur.v[kk][(8 * g) ^ ((kk << 3) & 32)]);
-            const float p = ex2(x[t][e] - base);
-            l += p;
-            w[e] = p * (e ? v_sc.y : v_sc.x);
+            vw[2 * half + e] = *reinterpret_cast<const uint2*>(&cur->v[kk][(8 * g) ^ ((kk << 3) & 32)]);
           }
-          if (cut) {  // a hidden key's value scale may be anything (stale rows)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) w[e] = x[t][e] == -INFINITY ? 0.0f : w[e];
-          }
-          split2(__half(), w[0], w[1], pa[2 * half], pa[2 * half + 1]);
+          const float2 w = weight(t);
+          split2(__half(), w.x, w.y, pa[2 * half], pa[2 * half + 1]);
         }
 #pragma unroll
         for (int word = 0; word < 2; ++word) {
@@ -435,10 +433,85 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           mma(__half(), o[4 * word + 3], pa, codes_to_f16x2<kE4m3, true>(hi0), codes_to_f16x2<kE4m3, true>(hi1));
         }
       }
+    };
+
+    // Chunks that every row sees whole, while the value scales are alike: one E for all rows.
+    const int whole = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(limit))) / kChunk;
+    uint32_t v_most = 0, v_least = 0x7f800000u;  // bits of the largest and the smallest value scale so far
+    bool fetched = false;
+    for (; ch < whole; ch += stride) {
+      fetch();
+      float x[kTiles][2];
+      score(x);
+      apply_terms<false>(x, a.t, score_scale, cap_scale, a.slopes != nullptr, slope, fp, ch * kChunk, limit, c, a.frame_magic);
+      const float m_new = maximum(x);
+      // NaN and infinity set no range; they reach the rows on their own.
+      uint32_t most = 0, least = 0x7f800000u;
+#pragma unroll
+      for (int i = 0; i < kChunk; i += 32) {
+        const uint32_t bits = __float_as_uint(cur->vs[i + lane]);
+        if (bits < 0x7f800000u) most = max(most, bits), least = min(least, bits);
+      }
+      v_most = max(v_most, __reduce_max_sync(0xffffffffu, most));
+      v_least = min(v_least, __reduce_min_sync(0xffffffffu, least));
+      if (v_most > v_least + (static_cast<uint32_t>(kAlike) << 23)) {
+        fetched = true;
+        break;
+      }
+      const int e_new = exponent_above(v_most);
+      if (__any_sync(0xffffffffu, m_new > m) || e_new != w_exp) rescale(m_new, m_new > m ? ex2(m - m_new) : 1.0f, e_new);
+      const float base = m == -INFINITY ? 0.0f : m;
+      const float v_scale = exp2i(kTop - w_exp);
+#pragma unroll
+      for (int i = 0; i < kChunk; i += 32) cur->vs[i + lane] *= v_scale;
+      __syncwarp();
+      add_values([&](int t) {
+        const float2 v_sc = *reinterpret_cast<const float2*>(&cur->vs[8 * t + 2 * c]);
+        const float p0 = ex2(x[t][0] - base), p1 = ex2(x[t][1] - base);
+        l += p0;
+        l += p1;
+        return make_float2(p0 * v_sc.x, p1 * v_sc.y);
+      });
+    }
+    // The others (one break of the above, the chunks with a mask): E by row.  In the units of m, the largest weight
+    // so far is 2^(E - 1) or somewhat less.
+    float w_run = exp2i(w_exp - 1);  // the lane's
+    for (; ch < chunks; ch += stride) {
+      if (!fetched) fetch();
+      fetched = false;
+      const int key0 = ch * kChunk;
+      float x[kTiles][2];
+      score(x);
+      apply_terms<true>(x, a.t, score_scale, cap_scale, a.slopes != nullptr, slope, fp, key0, limit, c, a.frame_magic);
+      const float m_new = maximum(x);
+      const float base = m_new == -INFINITY ? 0.0f : m_new;
+      const float alpha = m_new > m ? ex2(m - m_new) : 1.0f;  // 0 for the first keys
+      // x becomes the weights, before E is known.
+      float sum = 0.0f, w_top = 0.0f;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const float2 v_sc = *reinterpret_cast<const float2*>(&cur->vs[8 * t + 2 * c]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p = ex2(x[t][e] - base);
+          sum += p;
+          // a hidden key's value scale may be anything (stale rows)
+          x[t][e] = key0 + 8 * t + ((2 * c + e) ^ (c & 1)) < limit ? p * (e ? v_sc.y : v_sc.x) : 0.0f;
+        }
+        w_top = max3f(w_top, fabsf(x[t][0]), fabsf(x[t][1]));  // NaN is no maximum
+      }
+      w_run = fmaxf(w_run * alpha, w_top);
+      w_top = fmaxf(w_run, __shfl_xor_sync(0xffffffffu, w_run, 1));
+      w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, 2));
+      const int e_new = exponent_above(__float_as_uint(w_top));
+      if (__any_sync(0xffffffffu, m_new > m || e_new != w_exp)) rescale(m_new, alpha, e_new);
+      l += sum;
+      const float w_scale = exp2i(kTop - w_exp);
+      add_values([&](int t) { return make_float2(x[t][0] * w_scale, x[t][1] * w_scale); });
     }
     cp_wait<0>();
     __syncthreads();  // every warp is done with its ring: the join buffers may cover it
-    const float back = __uint_as_float(static_cast<uint32_t>(v_exp - kTop + 127) << 23);  // 2^(E - kTop)
+    const float back = exp2i(w_exp - kTop);
     finish_block<T>(sh, smem.part, o, m, l, back, rb, q_rows, a.group, kvh, rank, splits, cluster, lead, begin,
                    a.out);
     __syncthreads();  // before the next block's loads and parts

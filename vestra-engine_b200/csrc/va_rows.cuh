@@ -131,9 +131,9 @@ __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x
 // Scores of the lane's keys from their products (x, times the key's scale): scale or cap, distance
 // bias, mask.  Each term over all scores of the lane under one branch, so that they overlap.
 // score_scale = scale log2(e), cap_scale = 2 log2(e) scale / cap, both times what x lacks.
-// Returns whether the chunk has keys that some row of the warp does not see.
-template <int kTiles>
-__device__ __forceinline__ bool apply_terms(float (&x)[kTiles][2], const AttnTerms& t, float score_scale, float cap_scale,
+// kMask false: every row sees the whole chunk.
+template <bool kMask, int kTiles>
+__device__ __forceinline__ void apply_terms(float (&x)[kTiles][2], const AttnTerms& t, float score_scale, float cap_scale,
                                             bool biased, float slope, int frame_at, int key0, int limit, int c,
                                             uint32_t frame_magic) {
 #define VA_EACH_SCORE(...)                                 \
@@ -158,11 +158,9 @@ __device__ __forceinline__ bool apply_terms(float (&x)[kTiles][2], const AttnTer
                     x[i][e] = fmaf(-slope, fabsf(dist), x[i][e]);)
     }
   }
-  const bool cut = __any_sync(0xffffffffu, key0 + 8 * kTiles > limit);
-  if (cut) {
+  if (kMask && __any_sync(0xffffffffu, key0 + 8 * kTiles > limit)) {
     VA_EACH_SCORE(x[i][e] = key0 + kk < limit ? x[i][e] : -INFINITY;)
   }
-  return cut;
 #undef VA_EACH_SCORE
 }
 

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) rows_attn_kernel(const _
     for (int i = 0; i < kTiles; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) x[i][e] = d[i][e];
-    apply_terms(x, t, t.scale_log2, t.cap_in, a.m.slopes != nullptr, slope, fp, key0, limit, c, a.frame_magic);
+    apply_terms<true>(x, t, t.scale_log2, t.cap_in, a.m.slopes != nullptr, slope, fp, key0, limit, c, a.frame_magic);
     float top = x[0][0];
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) top = max3f(top, x[i][0], x[i][1]);
