@@ -185,3 +185,39 @@ def test_hidden_tokens_do_not_change_a_bit(ctx, fmt, held):
         ctx.cache_attention(cache, q, outs[-1], i32([0, 3]), i32([held]), max_tokens=3)
     for out in outs[1:]:
         assert torch.equal(out[0], outs[0][0])
+
+
+# ------------------------------------------------------------------ few rows over long documents
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("depth", [8.0, 14.0, 17.5, 20.0])
+@pytest.mark.parametrize("docs", [1, 40])  # 40: a key head's keys stay with one CTA
+def test_single_row_with_a_long_flat_tail(ctx, dtype, depth, docs):
+    """One key `depth` nats above many equal ones whose values share a sign: every one of them is small, their
+    sum is not.  The values of the equal keys are 1, the other key's 0, so the result is the tail's share.
+
+    Tolerance: the output's rounding; two parts of a probability (2^-16 of it in bf16, 2^-22 or 2^-40 of the largest
+    in f16); F32 sums in order: a lane adds n / lanes probabilities, each addition off by at most 2^-24 of the lane's
+    sum, which for the lane with the largest key is at most its share of the tail, 1 / lanes; the products' sums
+    likewise (16 keys an addition, truncated: 2^-23)."""
+    n = 1 << 20 if docs == 1 else 1 << 18
+    heads = 1 if docs == 1 else 12
+    ends = [64 * i for i in range(docs)] + [64 * docs + n]  # the last document is long, the others short
+    rows = list(range(docs + 1))
+    splits = va.attention_plan_shape(heads, heads, rows, ends)["splits"]
+    assert splits == (16 if docs == 1 else 1)
+    long = ends[-2]
+    n = ends[-1] - long
+    k = torch.zeros(ends[-1], heads, D, device="cuda", dtype=dtype)
+    v = torch.ones_like(k)
+    k[long, :, 0] = depth
+    v[long] = 0
+    q = torch.zeros(docs, heads, D, device="cuda", dtype=dtype)
+    q[..., 0] = 8.0
+    out = torch.empty_like(q)
+    ctx.masked_attention(va.AttentionPlan(ctx, heads, heads, rows, ends), q, k, v, out)
+    score = float(k[long, 0, 0])  # as rounded to the type
+    tail = (n - 1) * np.exp(-score)
+    ref, lanes = tail / (1 + tail), 16 * splits
+    parts = 2.0 ** -16 * ref if dtype == BF16 else 2.0 ** -22 * ref + n * 2.0 ** -40
+    sums = ref * (tail / (1 + tail) / lanes + n / lanes * 2.0 ** -24 + n / (lanes / 4) / 16 * 2.0 ** -23)
+    assert (out[-1].double() - ref).abs().max() <= half_step(dtype) * ref + parts + sums

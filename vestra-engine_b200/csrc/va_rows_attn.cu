@@ -5,7 +5,9 @@
 // rows.  Bound by HBM: every visible key costs 256 bytes per key head and is used by at most 16
 // rows.  Layout, score terms and joins as in va_rows.cuh; keys and values are the operands as they
 // are (no conversion), the query row too (its low half rows are zero), and a probability keeps a
-// high and a low part, so the result is closer to F32 than the tile kernel's.
+// high and a low part, so the result is closer to F32 than the tile kernel's.  f16's steps end at
+// 2^-24, so there probabilities are lifted by 2^kLift, and the sums with them (it cancels in the quotient): each is
+// off by at most 2^-22 of itself or 2^-40 of the row's largest.
 //
 // A cluster of CTAs shares one (tile, key head, 8-row block); its warps take 32-key chunks in turn
 // through a ring of their own in shared memory (cp.async, one chunk ahead).  Measured on B200: one token
@@ -13,6 +15,7 @@
 // keys is 4: three chunks a warp and the cluster's join are the rest.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "va_internal.h"
 #include "va_ptx.cuh"
@@ -68,6 +71,7 @@ __device__ __forceinline__ void load_chunk(Chunk& ch, const char* k, const char*
 
 template <class T>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) rows_attn_kernel(const __grid_constant__ RowsArgs a) {
+  constexpr float kLift = std::is_same<T, __half>::value ? 15.0f : 0.0f;  // so a probability is at most 2^15
   extern __shared__ uint4 smem_raw[];
   Shared& smem = *reinterpret_cast<Shared*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -184,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) rows_attn_kernel(const _
         for (int e = 0; e < 4; ++e) o[n][e] *= alpha;
       m = m_new;
     }
-    const float base = m == -INFINITY ? 0.0f : m;
+    const float base = (m == -INFINITY ? 0.0f : m) - kLift;
 #pragma unroll
     for (int u = 0; u < kTiles / 2; ++u) {
       uint32_t pa[4];
