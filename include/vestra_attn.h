@@ -434,8 +434,12 @@ int va_attn_plan_shape(const va_attn_terms* terms, int documents, const int64_t*
 /* q, out: [.., heads]; k, v: [.., kv_heads]; all BF16 or all F16; data 16-byte
  * aligned, strides multiples of 8 elements, heads not overlapping.  Only rows of the
  * plan's documents are read or written, but a document's own key and value rows must be
- * finite: a NaN or infinity in one may reach rows that do not see it; with BF16 and a
- * score_cap up to 50 values stay below 2^79 (larger ones may overflow).  out may be q. */
+ * finite: a NaN or infinity in one may reach rows that do not see it.  With BF16, a
+ * score_cap up to 50, no slopes and rows that all see 1024 keys or more, values stay below
+ * 2^79 (larger ones may overflow), and in rows whose keys all score near -score_cap values
+ * below n * 2^-44 lose precision, n = the most keys a row sees (2^-30 for 2^14).  F16:
+ * probabilities below 2^-25 of a row's largest lose precision, those below 2^-36 count as 0
+ * (tiles of 16 rows or fewer: 2^-30 and 2^-40).  out may be q. */
 int va_masked_attention_device(va_ctx* ctx, const va_attn_plan* plan, const va_heads* q, const va_heads* k,
                                const va_heads* v, const va_heads* out, void* stream);
 

@@ -221,3 +221,21 @@ def test_single_row_with_a_long_flat_tail(ctx, dtype, depth, docs):
     parts = 2.0 ** -16 * ref if dtype == BF16 else 2.0 ** -22 * ref + n * 2.0 ** -40
     sums = ref * (tail / (1 + tail) / lanes + n / lanes * 2.0 ** -24 + n / (lanes / 4) / 16 * 2.0 ** -23)
     assert (out[-1].double() - ref).abs().max() <= half_step(dtype) * ref + parts + sums
+
+
+# ------------------------------------------------------------------ constant exponent reference
+@pytest.mark.parametrize("keys", [1100, 5000])
+@pytest.mark.parametrize("power", [0, -20, -28, -30, 60, 78])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_saturated_scores_with_small_and_large_values(ctx, keys, power, sign):
+    """Every score at one end of the cap: the probabilities are the largest or the smallest the reference allows."""
+    g = gen(keys)
+    q = torch.full((20, 1, D), 30.0, device="cuda", dtype=BF16)
+    k = torch.full((keys, 1, D), 30.0 * sign, device="cuda", dtype=BF16)
+    v = (randn(g, keys, 1, D).double() * 2.0 ** power / 4).to(BF16)
+    out = torch.empty_like(q)
+    ctx.masked_attention(va.AttentionPlan(ctx, 1, 1, [0, 20], [0, keys], score_cap=50.0), q, k, v, out)
+    ref, a = attention_ref(q, k, v, False, 1, 0, None, 50.0)
+    u = half_step(BF16)
+    # equal probabilities: one rounding of each, and the output's
+    assert ((out.double() - ref).abs() <= u * ref.abs() + (u + 2.0 ** -12) * a).all()

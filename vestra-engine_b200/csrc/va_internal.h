@@ -372,6 +372,8 @@ struct MaskedArgs {
   AttnTerms t;
   int group, tile_tokens, items, splits;
   int fewest_keys;          // keys the row that sees fewest sees
+  int most_keys;            // and the one that sees most
+  float fixed;              // the constant exponent reference's negative (set by launch_masked)
   const MaskedItem* item;
   const float* slopes;      // [heads] device, times log2(e); nullptr: no bias
   HeadsRef out;

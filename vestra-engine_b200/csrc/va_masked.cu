@@ -55,9 +55,10 @@ constexpr uint32_t kTileBytes = kTile * kHeadDim * 2;
 constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 192;
 constexpr int kMaxSplits = 16;
-// See masked_attn_kernel: caps up to 50 (72.13 in the log2 domain), probabilities from 2^-120 up.
-constexpr float kFixedCap = 72.2f, kFixedTop = 2.0f * kFixedCap - 120.0f;
+// See masked_attn_kernel: caps up to 50 (72.13 in the log2 domain), for values up to 2^kFixedValues.
+constexpr float kFixedCap = 72.2f;
 constexpr int kFixedKeys = 1024;
+constexpr int kFixedValues = 79;
 
 struct Smem {
   static constexpr uint32_t kQ = 0;
@@ -455,9 +456,12 @@ __device__ __forceinline__ void bias_scores(float* s, const AttnTerms& t, int k0
 }
 
 // kFixed (capped scores without a bias, bf16, cap log2(e) <= kFixedCap): every score lies in
-// [-cap, cap], so the exponent's reference is the constant cap log2(e) - kFixedTop instead
-// of the row's maximum: probabilities lie in [2^(kFixedTop - 2 kFixedCap), 2^kFixedTop], inside
-// bf16's and F32's normal range, and no maximum, exchange or rescaling is needed (a 10,392-token
+// [-cap, cap], so the exponent's reference is the constant cap log2(e) - top instead
+// of the row's maximum: probabilities lie in [2^(top - 2 kFixedCap), 2^top].  top is as high as values up to 2^79
+// allow, 127 - 79 - log2(keys of the longest document): 24 for the 2^24 keys a document may have (probabilities
+// from 2^-120 up, inside bf16's and F32's normal range), 34 for a 10,392-token window, so that rows whose keys all
+// score near -cap keep small values (down to about 2^(4 - top); below they meet F32's smallest numbers).
+// No maximum, exchange or rescaling is needed (a 10,392-token
 // window 611 us against 684).  Where the row's maximum is the reference, the largest probability
 // is exactly 1; here it is rounded like the others, which shows in rows that see few keys (error
 // up to 1.6 times that of an F32 softmax rounded to bf16, against 1.1), so every row of the
@@ -555,7 +559,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       slope[i] = kBias ? a.slopes[head] : 0.0f;
     }
     const float sl2 = a.t.scale_log2;
-    const float fixed = kFixedTop - a.t.cap_out;
     // Running maxima, log2 domain, may lag by kGrow (kFixed: the constant reference).
     float m[2] = {kFixed ? 0.0f : -INFINITY, kFixed ? 0.0f : -INFINITY};
     float l[2] = {0.0f, 0.0f};            // partial sums over the thread's columns
@@ -613,15 +616,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (!partial) {
           const float top = largest(s);
           if (__all_sync(0xffffffffu, top <= a.t.cap_range[0]))
-            both(CapPoly<false>(a.t, fixed));
+            both(CapPoly<false>(a.t, a.fixed));
           else if (__all_sync(0xffffffffu, top <= a.t.cap_range[1]))
-            both(CapPoly<true>(a.t, fixed));
+            both(CapPoly<true>(a.t, a.fixed));
         }
       }
       if (!fused) {
         if constexpr (kCap) {
           if (partial) hide(s, lim, 0.0f);  // hidden keys may hold anything: out of the range check
-          cap_scores(s, a.t, kFixed ? fixed : 0.0f);  // kFixed: the exponent itself
+          cap_scores(s, a.t, kFixed ? a.fixed : 0.0f);  // kFixed: the exponent itself
         }
         if constexpr (kBias) {
           const bool past = k0 + kTile - 1 <= g.it.first || (a.t.causal && g.it.prefix == 0);
@@ -911,7 +914,13 @@ cudaError_t launch_masked(const HeadsRef& q, const HeadsRef& k, const HeadsRef& 
   static const Fn fn[2][2][2] = {
       {{launch<false, false, false>, launch<false, false, true>}, {launch<false, true, false>, launch<false, true, true>}},
       {{launch<true, false, false>, launch<true, false, true>}, {launch<true, true, false>, launch<true, true, true>}}};
-  if (!f16 && cap && !bias && a.t.cap_out <= kFixedCap && a.fewest_keys >= kFixedKeys) return launch<false, true, false, true>(mq, mk, mv, a, blocks, err, st);
+  if (!f16 && cap && !bias && a.t.cap_out <= kFixedCap && a.fewest_keys >= kFixedKeys) {
+    MaskedArgs fixed = a;
+    int log2_keys = 10;
+    while ((int64_t(1) << log2_keys) < a.most_keys) ++log2_keys;
+    fixed.fixed = static_cast<float>(127 - kFixedValues - log2_keys) - a.t.cap_out;
+    return launch<false, true, false, true>(mq, mk, mv, fixed, blocks, err, st);
+  }
   return fn[f16][cap][bias](mq, mk, mv, a, blocks, err, st);
 }
 

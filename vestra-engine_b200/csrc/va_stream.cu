@@ -435,6 +435,7 @@ int va_masked_attention_device(va_ctx* c, const va_attn_plan* p, const va_heads*
   a.items = static_cast<int>(p->items.size());
   a.splits = p->splits;
   a.fewest_keys = p->fewest_keys;
+  a.most_keys = p->items[0].keys;
   a.item = p->dev_items;
   a.slopes = p->dev_slopes;
   a.out = ref(out);
