@@ -213,7 +213,7 @@ __device__ __forceinline__ void run_producer(const Ctl& c, const Geom& g, const 
 }
 
 // UMMA issuer (the whole warp waits, lane 0 issues): QK(0), QK(1), then per key tile PV(j), QK(j+2).
-template <bool kF16>
+template <bool kF16, bool kCap>
 __device__ __forceinline__ void run_mma(const Ctl& c, const Geom& g, uint32_t tmem, int* err) {
   constexpr uint32_t idesc_qk = kF16 ? idesc_f16_f32(kTile, kTile, false, false)
                                      : idesc_bf16_f32(kTile, kTile, false, false);
@@ -245,6 +245,14 @@ __device__ __forceinline__ void run_mma(const Ctl& c, const Geom& g, uint32_t tm
     return r;
   };
   bool ok = g.n > 0 && wait(c.q_full(), 0);
+  // A warp of softmax chooses the form of the cap by the range of its scores, and rows past the tile's last may not
+  // take part: they hold another document's queries (which another CTA may be overwriting, out may be q), or, where
+  // the heads that share a key head do not divide 128, what an earlier CTA left.  Zeros score 0.
+  if (kCap && ok && g.rows < kTile) {
+    for (int i = g.rows * 8 + lane; i < kTile * 8; i += 32) st_shared_v4(c.sQ() + i * 16, make_uint4(0, 0, 0, 0));
+    fence_proxy_async_smem();
+    __syncwarp();
+  }
   if (ok) ok = qk(0);
   if (ok && g.n > 1) ok = qk(1);
   for (int j = 0; ok && j < g.n; ++j) {
@@ -290,18 +298,6 @@ __device__ __forceinline__ void row_maxima(const float* s, float* mx) {
     }
     mx[i] = max3f(a, b, fmaxf(v[60], v[61]));
   }
-}
-
-// Scores of rows from `rows` on become 0: they belong to no row of the tile, so they may not take part in a
-// choice that the warp makes together.
-__device__ __forceinline__ void drop_rows(float* s, const int* row, int rows) {
-#pragma unroll
-  for (int k = 0; k < 16; ++k)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (row[0] >= rows) s[4 * k + e] = 0.0f;
-      if (row[1] >= rows) s[4 * k + 2 + e] = 0.0f;
-    }
 }
 
 // Scores of the thread's columns (relative to its first) from lim[i] on become v.
@@ -520,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (lane == 0) run_producer(c, g, &map_k, &map_v, err);
       __syncwarp();
     } else {
-      run_mma<kF16>(c, g, tmem, err);
+      run_mma<kF16, kCap>(c, g, tmem, err);
     }
     if (a.splits > 1) {
       cluster_sync();  // partial rows written
@@ -533,9 +529,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint32_t tS = tmem + lane_off + kColS, tP = tmem + lane_off + kColP, tO = tmem + lane_off + kColO;
     const int c0 = 2 * (lane & 3);  // first of the thread's column pair in every 8 columns
     const bool warp_live = lane_base < g.rows;
-    // The warp's last rows are past the tile's: another document's queries, or, where the heads that share a
-    // key head do not divide 128, what an earlier CTA left in shared memory.
-    const bool ragged = lane_base + 16 > g.rows;
     // The thread's two rows of the tile.
     int limit[2], row[2];
     int frame[2];
@@ -584,9 +577,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       tmem_ld_16x256b_x16(tS, s);
       tc_fence_before();
       warp_arrive(c.s_free());  // QK of the next tile may overwrite S
-      if constexpr (kCap) {
-        if (ragged) drop_rows(s, row, g.rows);  // the range of the scores chooses the form of the cap
-      }
       const int k0 = (g.t0 + j) * kTile;
       const bool partial = __any_sync(0xffffffffu, min(limit[0], limit[1]) < k0 + kTile);
       const int lim[2] = {limit[0] - k0 - c0, limit[1] - k0 - c0};
