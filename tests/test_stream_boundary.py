@@ -3,6 +3,7 @@ for the CUDA runtime and the launchers (fake_stream_runtime.cpp), which records 
 import ctypes
 import os
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -79,3 +80,24 @@ def test_a_plan_is_on_the_device_when_create_returns(lib, slopes, q_lens, k_lens
     for h, s in enumerate(slopes or []):
         assert seen.slope[h] == pytest.approx(s * np.log2(np.e), rel=1e-6)
     lib.va_attn_plan_destroy(plan)
+
+
+def test_a_layout_of_too_many_tiles_is_refused_before_it_is_built():
+    """2^31 tiles of one token would be 60 GB of work list: refused by their number, in a process that may
+    not allocate 2 GB more than it has."""
+    code = """
+import resource, sys
+sys.path.insert(0, %r)
+import numpy as np, vestra_attn as va
+va.load_library()
+with open('/proc/self/statm') as f:
+    used = int(f.read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + 2 ** 31, used + 2 ** 31))
+ends = np.minimum(np.arange(129, dtype=np.int64) * 2 ** 24, 2 ** 31 - 1)
+try:
+    va.attention_plan_shape(128, 1, ends, np.zeros(129, np.int64))
+except va.VestraError as e:
+    sys.exit(0 if e.code == va.VA_ERR_INVALID else 3)
+sys.exit(4)
+""" % os.path.dirname(va.__file__)
+    assert subprocess.run([sys.executable, "-c", code], timeout=300).returncode == 0

@@ -141,13 +141,20 @@ const char* build_plan(const va_attn_terms* t, int documents, const int64_t* qo,
   p->q_rows = qo[documents];
   p->k_rows = ko[documents];
   if (p->q_rows > kMaxRows || p->k_rows > kMaxRows) return "offsets reach past 2^31 rows";
+  // Everything is checked, the number of tiles too, before the list is built.
+  int64_t tiles = 0;
+  for (int b = 0; b < documents; ++b) {
+    if (qo[b + 1] < qo[b] || ko[b + 1] < ko[b] || qo[b + 1] > kMaxRows || ko[b + 1] > kMaxRows) return "offsets must ascend";
+    if (ko[b + 1] - ko[b] > kMaxDocKeys) return "a document has more than 2^24 keys";
+    if (qo[b + 1] - qo[b] > kMaxDocKeys) return "a document has more than 2^24 query rows";
+    if (prefix && prefix[b] < 0) return "prefix must not be negative";
+    tiles += (qo[b + 1] - qo[b] + p->tile_tokens - 1) / p->tile_tokens;
+  }
+  if (tiles > kMaxRows / t->kv_heads / 16) return "too many query tiles";
+  p->items.reserve(static_cast<size_t>(tiles));
   for (int b = 0; b < documents; ++b) {
     const int64_t lq = qo[b + 1] - qo[b], lk = ko[b + 1] - ko[b];
-    if (lq < 0 || lk < 0 || qo[b + 1] > kMaxRows || ko[b + 1] > kMaxRows) return "offsets must ascend";
-    if (lk > kMaxDocKeys) return "a document has more than 2^24 keys";
-    if (lq > kMaxDocKeys) return "a document has more than 2^24 query rows";
     const int64_t pre = prefix ? prefix[b] : 0;
-    if (pre < 0) return "prefix must not be negative";
     for (int64_t i = 0; i < lq; i += p->tile_tokens) {
       va::MaskedItem it{};
       it.q_row = static_cast<int>(qo[b] + i);
@@ -168,7 +175,6 @@ const char* build_plan(const va_attn_terms* t, int documents, const int64_t* qo,
       p->items.push_back(it);
     }
   }
-  if (p->items.size() > static_cast<size_t>(kMaxRows) / t->kv_heads / 16) return "too many query tiles";
   // Longest first, so the last CTAs to start are the short ones; equal ones in row order, so
   // the tiles that read the same keys run together.
   std::stable_sort(p->items.begin(), p->items.end(),
@@ -179,9 +185,9 @@ const char* build_plan(const va_attn_terms* t, int documents, const int64_t* qo,
                                 p->items[0].keys, sms);
     return nullptr;
   }
-  std::vector<int> tiles(p->items.size());
-  for (size_t i = 0; i < tiles.size(); ++i) tiles[i] = (p->items[i].keys + 127) / 128;
-  p->splits = va::masked_splits(tiles.data(), static_cast<int64_t>(tiles.size()), t->kv_heads, sms);
+  std::vector<int> key_tiles(p->items.size());
+  for (size_t i = 0; i < key_tiles.size(); ++i) key_tiles[i] = (p->items[i].keys + 127) / 128;
+  p->splits = va::masked_splits(key_tiles.data(), tiles, t->kv_heads, sms);
   return nullptr;
 }
 
