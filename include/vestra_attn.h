@@ -416,10 +416,11 @@ typedef struct va_attn_terms {
  * document sees another's keys.  The plan holds the work list of one such layout on
  * the context's device.  All arrays are host arrays, read during the call:
  * q_offsets, k_offsets [documents + 1] ascending from >= 0, below 2^31 rows, at most
- * 2^24 keys per document; prefix [documents] >= 0 or NULL; slopes [heads] finite or
- * NULL.  Create allocates device memory (not during a capture) and returns with the plan
- * on the device, ready for any stream; a plan serves any number of calls, also at once, and
- * is destroyed when none is running, and before its context. */
+ * 2^24 keys and query rows per document; prefix [documents] >= 0 or NULL; slopes [heads],
+ * magnitudes at most 2^96, or NULL (score and bias are summed in F32).  Create allocates
+ * device memory (not during a capture) and returns with the plan on the device, ready for
+ * any stream; a plan serves any number of calls, also at once, and is destroyed when none is
+ * running, and before its context. */
 typedef struct va_attn_plan va_attn_plan;
 int va_attn_plan_create(va_ctx* ctx, const va_attn_terms* terms, int documents, const int64_t* q_offsets,
                         const int64_t* k_offsets, const int64_t* prefix, const float* slopes,
@@ -480,8 +481,8 @@ int va_kv_cache_read_device(va_ctx* ctx, const va_kv_cache* cache, int64_t rows,
                             const int32_t* first, const va_heads* k, const va_heads* v, void* stream);
 /* Attention of a few new tokens per document over the cache (terms as above): rows
  * [offsets[b], offsets[b+1]) of q are the last tokens of the lens[b] held, normally
- * just written.  prefix int32 [documents] and slopes F32 [heads] on the device, or
- * NULL.  max_tokens: the most rows a document usually has (sizes the launch; more rows
+ * just written.  prefix int32 [documents] and slopes F32 [heads] (magnitudes at
+ * most 2^96, not checked) on the device, or NULL.  max_tokens: the most rows a document usually has (sizes the launch; more rows
  * are served too, more slowly).  q, out [rows, heads] BF16 or F16, 16-byte aligned,
  * strides multiples of 8 elements.  Bad offsets, or lens outside [0, capacity]: as
  * above, and the document's rows of out are left as they were.  For many new tokens

@@ -239,3 +239,24 @@ def test_saturated_scores_with_small_and_large_values(ctx, keys, power, sign):
     u = half_step(BF16)
     # equal probabilities: one rounding of each, and the output's
     assert ((out.double() - ref).abs() <= u * ref.abs() + (u + 2.0 ** -12) * a).all()
+
+
+# ------------------------------------------------------------------ slopes
+@pytest.mark.parametrize("slope", [2.0 ** 96, -2.0 ** 96, 1e6])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("n,m", [(2, 40), (150, 300), (300, 150)])
+def test_steep_slopes(ctx, slope, cap, n, m):
+    """A bias that leaves every row one frame: the nearest, or with a negative slope the farthest.  Score and bias
+    are one F32 sum, so a score beside a bias of 1e6 and more is lost (half an ulp of 1e6 is 2^-5); rows whose own
+    frame holds keys have distance 0 there, and their scores count."""
+    g = gen(n)
+    q, k, v = (randn(g, r, 1, D, dtype=BF16) for r in (n, m, m))
+    slopes = np.array([slope], np.float32)
+    plan = va.AttentionPlan(ctx, 1, 1, [0, n], [0, m], causal=True, frame=5, prefix=[3], slopes=slopes, score_cap=cap)
+    out = torch.empty_like(q)
+    ctx.masked_attention(plan, q, k, v, out)
+    assert torch.isfinite(out.float()).all()
+    if slope > 0:
+        ref, a = attention_ref(q, k, v, True, 5, 3, np.array([1e6]), cap)
+        rows = torch.arange(n, device="cuda") + m - n >= 0
+        check_attention(out[rows], ref[rows], a[rows])

@@ -101,3 +101,18 @@ except va.VestraError as e:
 sys.exit(4)
 """ % os.path.dirname(va.__file__)
     assert subprocess.run([sys.executable, "-c", code], timeout=300).returncode == 0
+
+
+# ------------------------------------------------------------------------------ slopes
+@pytest.mark.parametrize("slope,ok", [(2.0 ** 96, True), (-2.0 ** 96, True), (2.0 ** 96 * 1.001, False), (3e38, False),
+                                      (-3e38, False), (float("inf"), False), (float("nan"), False), (0.0, True)])
+def test_slopes_whose_bias_would_leave_f32_are_refused(lib, slope, ok):
+    """slope log2(e) times the largest distance has to stay finite: an infinite one times distance 0 is NaN."""
+    rc, plan = create_plan(lib, [0, 3], [0, 3], slopes=[0.5, 0.5, slope, 0.5])
+    assert rc == (va.VA_OK if ok else va.VA_ERR_INVALID)
+    if ok:
+        assert lib.va_masked_attention_device(lib.ctx, plan, *[heads_of(4 * 64, 64, 4)] * 4, 0) == va.VA_OK
+        assert np.isfinite(np.float32(lib.fake_seen().contents.slope[2]) * np.float32(2.0 ** 30))
+        lib.va_attn_plan_destroy(plan)
+    else:
+        assert b"slopes" in lib.fake_error(lib.ctx)

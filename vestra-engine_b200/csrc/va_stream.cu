@@ -28,6 +28,7 @@ constexpr double kLog2e = 1.4426950408889634;
 constexpr int64_t kMaxRows = 0x7fffffff;
 constexpr int64_t kMaxCapacity = int64_t(1) << 30;  // chunk arithmetic stays in 32 bits
 constexpr int64_t kMaxDocKeys = int64_t(1) << 24;  // frame indices stay exact in F32
+constexpr float kMaxSlope = 0x1p96f;  // times log2(e) and 2^30 tokens: inside F32
 
 // Makes the context's device current for one call and puts the caller's back.
 class DeviceScope {
@@ -383,7 +384,7 @@ int va_attn_plan_create(va_ctx* c, const va_attn_terms* terms, int documents, co
     std::vector<float> s;
     if (!m && slopes) {
       for (int h = 0; h < terms->heads && !m; ++h) {
-        if (!std::isfinite(slopes[h])) m = "slopes must be finite";
+        if (!(std::fabs(slopes[h]) <= kMaxSlope)) m = "slopes must be finite, at most 2^96";
         s.push_back(static_cast<float>(slopes[h] * kLog2e));
       }
     }
