@@ -358,7 +358,8 @@ int va_linear_bf16(va_ctx* ctx, const void* a, const void* w_t, const float* bia
 
 /* A token-major tensor of heads: element (token, head, c) of `data` is at token *
  * token_stride + head * head_stride + c (strides in elements, the head's channels
- * contiguous), so q, k and v may be views of one packed projection. */
+ * contiguous), so q, k and v may be views of one packed projection.  The token stride of a
+ * tensor of one row or none, and the head stride of one head, may be anything. */
 typedef struct va_heads {
   void* data;
   int64_t token_stride;

@@ -260,3 +260,39 @@ def test_steep_slopes(ctx, slope, cap, n, m):
         ref, a = attention_ref(q, k, v, True, 5, 3, np.array([1e6]), cap)
         rows = torch.arange(n, device="cuda") + m - n >= 0
         check_attention(out[rows], ref[rows], a[rows])
+
+
+# ------------------------------------------------------------------ strides that are never stepped over
+@pytest.mark.parametrize("token_stride", [64, 1, 0, 2 ** 40])
+def test_one_row_of_any_token_stride(ctx, token_stride):
+    """A view of one row keeps whatever stride its rows had."""
+    g = gen(3)
+    heads = 4
+    wide = randn(g, heads, 7, D, dtype=BF16)  # head-major
+    row = wide[:, 5:6].transpose(0, 1)
+    x = row.as_strided((1, heads, D), (token_stride, 7 * D, 1), row.storage_offset())
+    clean = row.contiguous()
+    kv = randn(g, 300, heads, D, dtype=BF16)
+    out, want = torch.empty_like(clean), torch.empty_like(clean)
+    for n in (1, 300):  # one key row, too
+        plan = va.AttentionPlan(ctx, heads, heads, [0, 1], [0, n])
+        ctx.masked_attention(plan, x, x if n == 1 else kv, x if n == 1 else kv, out)
+        ctx.masked_attention(plan, clean, clean if n == 1 else kv, clean if n == 1 else kv, want)
+        assert torch.equal(out, want)
+    one_key = va.AttentionPlan(ctx, heads, heads, [0, 300], [0, 1])  # the tensor maps' form
+    o2, w2 = torch.empty_like(kv), torch.empty_like(kv)
+    ctx.masked_attention(one_key, kv, x, x, o2)
+    ctx.masked_attention(one_key, kv, clean, clean, w2)
+    assert torch.equal(o2, w2) and torch.equal(o2, clean.expand_as(o2))
+    pos = i32([[7]])
+    ctx.rope_axes(va.RopeAxes((64,)), pos, x, out)
+    ctx.rope_axes(va.RopeAxes((64,)), pos, clean, want)
+    assert torch.equal(out, want)
+    results = []
+    for y in (x, clean):
+        cache, codes, scales = new_cache(gen(1), 1, heads, 8, torch.int8)
+        ctx.kv_cache_write(cache, y, y, i32([0, 1]), i32([1]))
+        o = torch.empty_like(clean)
+        ctx.cache_attention(cache, y, o, i32([0, 1]), i32([1]), max_tokens=1)
+        results.append((codes[0][:, :, 0].clone(), o))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])

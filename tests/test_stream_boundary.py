@@ -116,3 +116,70 @@ def test_slopes_whose_bias_would_leave_f32_are_refused(lib, slope, ok):
         lib.va_attn_plan_destroy(plan)
     else:
         assert b"slopes" in lib.fake_error(lib.ctx)
+
+
+# ------------------------------------------------------------------------------ strides
+PTR = 1 << 20
+
+
+def cache_of(kv_heads, documents=1, capacity=64):
+    return va.VaKvCache(documents, kv_heads, capacity, va.KV_INT8, 0, PTR, PTR, PTR, PTR)
+
+
+def every_call(lib, h, rows, heads):
+    """Return codes of the calls with all operands of these heads and rows."""
+    cache, terms = cache_of(heads), va.VaAttnTerms(heads, heads, 1, 1, 0.0, 0.0)
+    rope = va.VaRopeAxes(1, (ctypes.c_int32 * 4)(64), 0, 0, 100.0)
+    out = [lib.va_rope_axes_device(lib.ctx, ctypes.byref(rope), rows, 64, PTR, h, h, h, h, 0),
+           lib.va_kv_cache_write_device(lib.ctx, ctypes.byref(cache), rows, PTR, PTR, h, h, 0),
+           lib.va_kv_cache_read_device(lib.ctx, ctypes.byref(cache), rows, PTR, PTR, h, h, 0),
+           lib.va_cache_attention_device(lib.ctx, ctypes.byref(cache), ctypes.byref(terms), rows, PTR, PTR, 1, None,
+                                         None, h, h, 0)]
+    rc, plan = create_plan(lib, [0, rows], [0, rows], heads, heads)
+    out += [rc, lib.va_masked_attention_device(lib.ctx, plan, h, h, h, h, 0)]
+    lib.va_attn_plan_destroy(plan)
+    return out
+
+
+@pytest.mark.parametrize("rows,token_stride,head_stride", [
+    (0, 64, 64), (0, 0, 0), (0, 256, 64),                                   # head-major and empty
+    (1, 64, 64), (1, 0, 64), (1, 1, 64), (1, -8, 64), (1, 2 ** 40, 64),     # a stride that is never stepped over
+    (1, 64, 2 ** 27), (1, 4 * 2 ** 27, 2 ** 27),                            # one row of a long head-major buffer
+    (2, 256, 64), (2, 64, 128), (5, 64, 320), (5, 2 ** 30, 64)])
+def test_strides_that_no_element_shares_are_taken(lib, rows, token_stride, head_stride):
+    h = heads_of(token_stride, head_stride, 4)
+    assert every_call(lib, h, rows, 4) == [va.VA_OK] * 6
+    seen = lib.fake_seen().contents
+    if seen.launches and rows == 1:
+        assert seen.token_stride[0] % 8 == 0 and 0 < seen.token_stride[0] <= 2 ** 30
+    if rows > 1:
+        assert seen.token_stride[0] == token_stride and seen.head_stride[0] == head_stride
+
+
+@pytest.mark.parametrize("rows,token_stride,head_stride", [
+    (1, 64, 0), (1, 64, 63), (1, 64, -64), (1, 64, 2 ** 39), (2, 64, 64), (2, 0, 64), (2, -256, 64), (5, 64, 319),
+    (5, 2 ** 30 + 8, 64), (5, 192, 64)])
+def test_strides_that_overlap_are_refused(lib, rows, token_stride, head_stride):
+    h = heads_of(token_stride, head_stride, 4)
+    codes = every_call(lib, h, rows, 4)
+    assert codes[4] == va.VA_OK and codes[:4] + codes[5:] == [va.VA_ERR_INVALID] * 5
+    assert lib.fake_seen().contents.launches == 0
+
+
+def view_on_device(x):
+    """A meta tensor's numbers, as of a CUDA tensor."""
+    class View:
+        shape, dtype = x.shape, x.dtype
+        get_device = staticmethod(lambda: 0)
+        stride = staticmethod(x.stride)
+        data_ptr = staticmethod(lambda: PTR)
+    return View()
+
+
+@pytest.mark.parametrize("rows", [0, 1, 2])
+def test_a_few_rows_of_a_long_head_major_buffer(lib, rows):
+    torch = pytest.importorskip("torch")
+    x = torch.empty(16, 2 ** 22, 64, dtype=torch.bfloat16, device="meta")  # 2^28 elements a head
+    packed, n, heads = va._heads(view_on_device(x[:, 5:5 + rows].transpose(0, 1)), 0, "q", 64)
+    assert (n, heads) == (rows, 16)
+    assert every_call(lib, packed, rows, 16) == [va.VA_OK] * 6

@@ -63,29 +63,31 @@ int bad(va_ctx* c, const char* msg) { return va::ctx_fail(c, VA_ERR_INVALID, msg
 int elem_size(int dtype) { return dtype == VA_F32 ? 4 : 2; }
 
 // No two elements of [rows][heads][head_dim] share an address: either the heads lie inside a
-// token's stride or the tokens inside a head's.
+// token's stride or the tokens inside a head's.  A stride that is never stepped over may be anything.
 bool strides_ok(const va_heads* h, int head_dim, int64_t rows) {
-  constexpr int64_t kMost = int64_t(1) << 30;
-  if (h->heads < 1 || h->token_stride < 0 || h->head_stride < 0 || h->token_stride > kMost) return false;
-  if (h->heads == 1) return h->token_stride >= head_dim;
-  if (h->head_stride > (int64_t(1) << 38)) return false;
-  const bool token_major = h->head_stride >= head_dim && h->head_stride <= kMost &&
-                           h->token_stride >= (h->heads - 1) * h->head_stride + head_dim;
-  const bool head_major = h->token_stride >= head_dim && rows > 0 &&
-                          h->head_stride >= (rows - 1) * h->token_stride + head_dim;
+  constexpr int64_t kMost = int64_t(1) << 30, kMostHead = int64_t(1) << 38;
+  if (h->heads < 1) return false;
+  if (rows == 0) return true;
+  if (rows == 1) return h->heads == 1 || (h->head_stride >= head_dim && h->head_stride <= kMostHead);
+  if (h->token_stride < head_dim || h->token_stride > kMost) return false;
+  if (h->heads == 1) return true;
+  if (h->head_stride < head_dim || h->head_stride > kMostHead) return false;
+  const bool token_major = h->head_stride <= kMost && h->token_stride >= (h->heads - 1) * h->head_stride + head_dim;
+  const bool head_major = h->head_stride >= (rows - 1) * h->token_stride + head_dim;
   return token_major || head_major;
 }
 
 // 16-byte vectors: aligned data, strides in whole vectors.
-bool vector_ok(const va_heads* h) {
+bool vector_ok(const va_heads* h, int64_t rows) {
   const int per = 16 / elem_size(h->dtype);
-  return reinterpret_cast<uintptr_t>(h->data) % 16 == 0 && h->token_stride % per == 0 &&
-         (h->heads == 1 || h->head_stride % per == 0);
+  return reinterpret_cast<uintptr_t>(h->data) % 16 == 0 && (rows <= 1 || h->token_stride % per == 0) &&
+         (rows == 0 || h->heads == 1 || h->head_stride % per == 0);
 }
 
-va::HeadsRef ref(const va_heads* h) {
+va::HeadsRef ref(const va_heads* h, int64_t rows) {
   if (!h) return va::HeadsRef{nullptr, 0, 0, 0};
-  return va::HeadsRef{h->data, h->token_stride, h->heads > 1 ? h->head_stride : 0, h->heads};
+  constexpr int64_t kNoStep = 64;  // for kernels and tensor maps: a legal stride
+  return va::HeadsRef{h->data, rows > 1 ? h->token_stride : kNoStep, h->heads > 1 ? h->head_stride : 0, h->heads};
 }
 
 const char* check_terms(const va_attn_terms* t) {
@@ -248,7 +250,7 @@ int cache_rows_call(va_ctx* c, const va_kv_cache* cache, int64_t rows, const int
     if (h->heads != cache->kv_heads) return bad(c, "k and v need the cache's kv_heads");
     if (rows > 0 && !h->data) return bad(c, "k and v data must be given");
     if (!strides_ok(h, 64, rows)) return bad(c, "k or v strides overlap");
-    if (!vector_ok(h)) return bad(c, "k and v need 16-byte aligned data and strides");
+    if (!vector_ok(h, rows)) return bad(c, "k and v need 16-byte aligned data and strides");
   }
   return VA_OK;
 }
@@ -304,10 +306,10 @@ int va_rope_axes_device(va_ctx* c, const va_rope_axes* rope, int64_t rows, int h
     for (const va_heads* h : {in[w], out[w]})
       if (reinterpret_cast<uintptr_t>(h->data) % elem_size(h->dtype)) return bad(c, "rope data is not aligned to its type");
     if (in[w]->data == out[w]->data &&
-        (in[w]->token_stride != out[w]->token_stride || (in[w]->heads > 1 && in[w]->head_stride != out[w]->head_stride)))
+        ((rows > 1 && in[w]->token_stride != out[w]->token_stride) || (in[w]->heads > 1 && in[w]->head_stride != out[w]->head_stride)))
       return bad(c, "an output on its input needs the same strides");
-    a.in[w] = ref(in[w]);
-    a.out[w] = ref(out[w]);
+    a.in[w] = ref(in[w], rows);
+    a.out[w] = ref(out[w], rows);
   }
   if (rows == 0) return VA_OK;
   if (!positions) return bad(c, "positions must be given");
@@ -433,7 +435,7 @@ int va_masked_attention_device(va_ctx* c, const va_attn_plan* p, const va_heads*
     if (o.h->heads != o.heads) return bad(c, "q and out need the plan's heads, k and v its kv_heads");
     if (!o.h->data) return bad(c, "q, k, v and out data must be given");
     if (!strides_ok(o.h, 64, o.rows)) return bad(c, "strides overlap");
-    if (!vector_ok(o.h)) return bad(c, "data must be 16-byte aligned, strides multiples of 8 elements");
+    if (!vector_ok(o.h, o.rows)) return bad(c, "data must be 16-byte aligned, strides multiples of 8 elements");
   }
   va::MaskedArgs a{};
   a.t = p->terms;
@@ -445,13 +447,13 @@ int va_masked_attention_device(va_ctx* c, const va_attn_plan* p, const va_heads*
   a.most_keys = p->items[0].keys;
   a.item = p->dev_items;
   a.slopes = p->dev_slopes;
-  a.out = ref(out);
+  a.out = ref(out, p->q_rows);
   DeviceScope scope(core.device);
   if (scope.error() != cudaSuccess) return launched(c, scope.error(), "attention device");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (va::rows_form(p->most_rows))
-    return launched(c, va::launch_rows(ref(q), ref(k), ref(v), a, p->most_rows, q->dtype, st), "masked attention launch");
-  return launched(c, va::launch_masked(ref(q), ref(p->k_rows ? k : q), ref(p->k_rows ? v : q), p->q_rows,
+    return launched(c, va::launch_rows(ref(q, p->q_rows), ref(k, p->k_rows), ref(v, p->k_rows), a, p->most_rows, q->dtype, st), "masked attention launch");
+  return launched(c, va::launch_masked(ref(q, p->q_rows), ref(p->k_rows ? k : q, p->k_rows), ref(p->k_rows ? v : q, p->k_rows), p->q_rows,
                                        p->k_rows, a, q->dtype, core.err, st),
                   "masked attention launch");
 }
@@ -465,7 +467,7 @@ int va_kv_cache_write_device(va_ctx* c, const va_kv_cache* cache, int64_t rows, 
   const va::CtxCore core = va::ctx_core(c);
   DeviceScope scope(core.device);
   if (scope.error() != cudaSuccess) return launched(c, scope.error(), "cache device");
-  return launched(c, va::launch_kv_write(cache_ref(cache), k->dtype, rows, offsets, lens, ref(k), ref(v), core.sms, core.err,
+  return launched(c, va::launch_kv_write(cache_ref(cache), k->dtype, rows, offsets, lens, ref(k, rows), ref(v, rows), core.sms, core.err,
                                          static_cast<cudaStream_t>(stream)),
                   "cache write launch");
 }
@@ -478,7 +480,7 @@ int va_kv_cache_read_device(va_ctx* c, const va_kv_cache* cache, int64_t rows, c
   const va::CtxCore core = va::ctx_core(c);
   DeviceScope scope(core.device);
   if (scope.error() != cudaSuccess) return launched(c, scope.error(), "cache device");
-  return launched(c, va::launch_kv_read(cache_ref(cache), k->dtype, rows, offsets, first, ref(k), ref(v), core.sms, core.err,
+  return launched(c, va::launch_kv_read(cache_ref(cache), k->dtype, rows, offsets, first, ref(k, rows), ref(v, rows), core.sms, core.err,
                                         static_cast<cudaStream_t>(stream)),
                   "cache read launch");
 }
@@ -499,7 +501,7 @@ int va_cache_attention_device(va_ctx* c, const va_kv_cache* cache, const va_attn
     if (h->heads != terms->heads) return bad(c, "q and out need the terms' heads");
     if (rows > 0 && !h->data) return bad(c, "q and out data must be given");
     if (!strides_ok(h, 64, rows)) return bad(c, "strides overlap");
-    if (!vector_ok(h)) return bad(c, "data must be 16-byte aligned, strides multiples of 8 elements");
+    if (!vector_ok(h, rows)) return bad(c, "data must be 16-byte aligned, strides multiples of 8 elements");
   }
   if (rows == 0) return VA_OK;
   const va::CtxCore core = va::ctx_core(c);
@@ -507,7 +509,7 @@ int va_cache_attention_device(va_ctx* c, const va_kv_cache* cache, const va_attn
   if (scope.error() != cudaSuccess) return launched(c, scope.error(), "cache attention device");
   const int most = static_cast<int>(std::min<int64_t>(max_tokens, rows));
   return launched(c, va::launch_cache_attention(cache_ref(cache), make_terms(terms), q->dtype, rows, offsets, lens,
-                                                most, prefix, slopes, ref(q), ref(out), core.sms, core.err,
+                                                most, prefix, slopes, ref(q, rows), ref(out, rows), core.sms, core.err,
                                                 static_cast<cudaStream_t>(stream)),
                   "cache attention launch");
 }

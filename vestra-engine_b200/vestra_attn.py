@@ -281,8 +281,6 @@ def _heads(x, device, what, channels=None):
             if cs == 1 and code >= 0 and (channels is None or d == channels):
                 if heads == 1:
                     hs = d
-                if rows <= 1:  # never stepped over
-                    ts = heads * max(hs, d)
                 return _PACK_HEADS(x.data_ptr(), ts, hs, heads, code), rows, heads
     except (AttributeError, ValueError):
         pass
