@@ -296,3 +296,23 @@ def test_one_row_of_any_token_stride(ctx, token_stride):
         ctx.cache_attention(cache, y, o, i32([0, 1]), i32([1]), max_tokens=1)
         results.append((codes[0][:, :, 0].clone(), o))
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+
+
+# ------------------------------------------------------------------ many documents
+def test_max_tokens_of_the_whole_batch_over_many_documents(ctx):
+    """max_tokens is an estimate: taken as all rows of the batch it may not size a launch past the grid's limit."""
+    docs, heads = 70000, 8
+    g = gen(17)
+    cache, codes, scales = new_cache(g, docs, 1, 2, torch.int8)
+    k, v = randn(g, docs, 1, D, dtype=BF16), randn(g, docs, 1, D, dtype=BF16)
+    ends = torch.arange(docs + 1, device="cuda", dtype=torch.int32)
+    ctx.kv_cache_write(cache, k, v, ends, torch.ones(docs, device="cuda", dtype=torch.int32))
+    q = randn(g, docs, heads, D, dtype=BF16)
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    lens = torch.ones(docs, device="cuda", dtype=torch.int32)
+    ctx.cache_attention(cache, q, out, ends, lens, max_tokens=docs)
+    ctx.cache_attention(cache, q, want, ends, lens, max_tokens=1)
+    assert torch.equal(out, want)
+    # one token held: its value, from the codes
+    value = codes[1][:, 0, 0].double() * scales[1][:, 0, :1].double()
+    assert ((out.double() - value[:, None]).abs() <= (half_step(BF16) + 2.0 ** -18) * value[:, None].abs()).all()

@@ -53,6 +53,7 @@ constexpr int kChunk = 64;         // keys a warp takes at a time
 constexpr int kTiles = kChunk / 8;
 constexpr int kStages = 2;         // chunks of a warp in shared memory
 constexpr int kCtasPerSm = 3;
+constexpr int64_t kMostBlocks = 1 << 20;
 constexpr int kMaxPaired = 256;    // documents that a CTA puts in order
 constexpr int kTop = 14;       // weights are brought below 2^kTop
 constexpr int kAlike = 6;
@@ -611,7 +612,10 @@ cudaError_t launch_cache_attention(const KvCacheRef& c, const AttnTerms& t, int 
       shared_by = both;
     }
   }
-  const int64_t blocks = shared_by * c.kv_heads * a.row_blocks * cluster;
+  // A generous max_tokens over many documents: CTAs past a thousand rounds take several blocks of rows instead.
+  const int64_t units = shared_by * c.kv_heads * cluster;
+  a.row_blocks = static_cast<int>(std::min<int64_t>(a.row_blocks, std::max<int64_t>(1, kMostBlocks / units)));
+  const int64_t blocks = units * a.row_blocks;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   auto go = [&](auto type, auto e4m3) {
     return paired ? launch<decltype(type), e4m3.value, true>(a, cluster, blocks, err, st)
