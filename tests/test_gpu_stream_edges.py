@@ -316,3 +316,62 @@ def test_max_tokens_of_the_whole_batch_over_many_documents(ctx):
     # one token held: its value, from the codes
     value = codes[1][:, 0, 0].double() * scales[1][:, 0, :1].double()
     assert ((out.double() - value[:, None]).abs() <= (half_step(BF16) + 2.0 ** -18) * value[:, None].abs()).all()
+
+
+# ------------------------------------------------------------------ what the tolerances tell apart
+def weight_steps(w, dropped):
+    """w [keys] as the kernel holds weights: two f16 parts of w * 2^k, the largest in [2^13, 2^14), or one (dropped)."""
+    k = 14 - torch.floor(torch.log2(w.max())) - 1
+    x = (w * torch.exp2(k)).float().double()
+    hi = x.half().double()
+    return (hi if dropped else hi + (x - hi).half().double()) * torch.exp2(-k)
+
+
+@pytest.mark.parametrize("held", [1, 2, 40, 64, 200])
+def test_both_parts_of_a_weight_count(ctx, held):
+    """Queries of zeros: every probability is 1 exactly, so a weight is its int8 value scale and the result is off by
+    half a step of f16 at its size, a weight's 2^-22 (two parts; 2^-38 of the largest at least), and F32 products and sums:
+    held + 4 roundings of 2^-24.  A weight of one part, 2^-11, is told apart."""
+    g = gen(held)
+    heads = 16
+    cache, codes, scales = new_cache(g, 1, heads, 256, torch.int8)
+    v = (randn(g, held, heads, D).abs() * 30 + 20).clamp(max=120)
+    v[..., 0] = 127 * (1 + 0.98 * 2.0 ** -11)  # every scale: 0.98 half steps of f16 past 1, and none cancels another
+    ctx.kv_cache_write(cache, torch.zeros_like(v), v, i32([0, held]), i32([held]))
+    q = torch.zeros(1, heads, D, device="cuda", dtype=F16)
+    out = torch.empty_like(q)
+    ctx.cache_attention(cache, q, out, i32([0, 1]), i32([held]), max_tokens=1)
+    c, s = codes[1][0, :, :held].double(), scales[1][0, :, :held].double()
+    ref = (c * s[..., None]).sum(1) / held
+    tol = torch.exp2(torch.floor(torch.log2(ref.abs())) - 11) + (2.0 ** -22 + (held + 4) * 2.0 ** -24) * ref.abs()
+    assert ((out[0].double() - ref).abs() <= tol).all()
+    one = torch.stack([(c[h] * weight_steps(s[h], True)[:, None]).sum(0) / held for h in range(heads)])
+    assert ((one.half().double() - ref).abs() > tol).any()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kind", ["one channel", "wide"])
+def test_scores_of_a_few_units_to_f32(ctx, fmt, kind):
+    """Keys of one channel, so that a score is one product: probabilities are as good as F32's.  A score s is off by
+    4 roundings of 2^-24 of s, the exponential by 2^-22 (and its argument by 2^-24 of s log2(e)), a weight by 2^-22,
+    F32 sums by keys * 2^-24: with s up to 8 below 2^-18 a key, 2^-16 for numerator and denominator of 300 keys.
+    wide: the channel that scores holds 2^-12 of the row's largest element, still exact."""
+    g = gen(9)
+    held, heads = 300, 16
+    cache, codes, scales = new_cache(g, 1, heads, 512, fmt)
+    s = torch.rand(held, heads, generator=g, device="cuda") * 8
+    k = torch.zeros(held, heads, D, device="cuda")
+    v = randn(g, held, heads, D).abs() + 0.5
+    q = torch.zeros(1, heads, D, device="cuda", dtype=F16)
+    at = 2.0 ** -12 * 1.1875 if kind == "wide" else 1.1875
+    q[..., 7] = at
+    if kind == "wide":
+        q[..., 50] = 1.0
+    k[..., 7] = s * 8 / at
+    ctx.kv_cache_write(cache, k, v, i32([0, held]), i32([held]))
+    out = torch.empty_like(q)
+    ctx.cache_attention(cache, q, out, i32([0, 1]), i32([held]), max_tokens=1)
+    kd, vd = held_values(codes, scales, held)
+    ref, a = attention_ref(q, kd, vd, True, 1, 0, None, 0.0)
+    tol = torch.exp2(torch.floor(torch.log2(ref.abs())) - 11) + 2.0 ** -16 * a
+    assert ((out.double() - ref).abs() <= tol).all()

@@ -6,12 +6,12 @@
 // multiplies its scores, a value's scale its probability, so codes are never scaled.
 //
 // Bound by HBM where all SMs have work: every visible key costs 2 * (64 + 4) bytes per key head
-// and 256 FLOP per query row.  The fragments, and the joining of warps and cluster, are va_rows.cuh's:
-// the low part of a split operand costs no further product and makes products good to 2^-21 of
-// the row's largest element.  The operands are f16 because both code formats become f16 in one
-// or two instructions a pair (bf16 took four or five, and the conversions are most of the loop).
-// Its range is met by powers of two: a query row is scaled to a largest magnitude in [1, 2) and the
-// factor goes to the scores; a weight (a probability times its value scale) is scaled by 2^(kTop - E).
+// and 256 FLOP per query row.  The fragments, and the joining of warps and cluster, are va_rows.cuh's.  The operands
+// are f16 because both code formats become f16 in one or two instructions a pair (bf16 took four or five, and the
+// conversions are most of the loop).  Its range is met by powers of two.  A query row is scaled to a largest magnitude
+// in [1, 2) and the factor goes to the scores: 16-bit elements stay exact down to 2^-14 of the largest, and to 2^-25
+// of it below.  A weight (a probability times its value scale) is scaled by 2^(kTop - E) and split in two f16 parts,
+// the second in the product's rows 8..15 at no further cost.
 //   While every row sees the whole chunk and the warp's value scales so far lie within 2^kAlike, E is just above
 //   the largest of them, for all rows: the key of a row's maximum has probability 1, so the row's largest
 //   weight is at least 2^(E - 1 - kAlike).
@@ -331,8 +331,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const float inv = __uint_as_float((254u - ex) << 23);
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        split2(__half(), x[4 * s] * inv, x[4 * s + 1] * inv, qa[s][0], qa[s][1]);
-        split2(__half(), x[4 * s + 2] * inv, x[4 * s + 3] * inv, qa[s][2], qa[s][3]);
+        qa[s][0] = f16x2_from_f32(x[4 * s] * inv, x[4 * s + 1] * inv);
+        qa[s][2] = f16x2_from_f32(x[4 * s + 2] * inv, x[4 * s + 3] * inv);
+        qa[s][1] = qa[s][3] = 0u;
       }
     }
     const float score_scale = q_scale * a.t.scale_log2, cap_scale = q_scale * a.t.cap_in;
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       for (int t = 0; t < kTiles; ++t) {
         const float2 k_scale = *reinterpret_cast<const float2*>(&cur->ks[8 * t + 2 * c]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) x[t][e] = (d[t][e] + d[t][2 + e]) * (e ? k_scale.y : k_scale.x);
+        for (int e = 0; e < 2; ++e) x[t][e] = d[t][e] * (e ? k_scale.y : k_scale.x);
       }
     };
     // The row's maximum with this chunk.
