@@ -375,3 +375,105 @@ def test_scores_of_a_few_units_to_f32(ctx, fmt, kind):
     ref, a = attention_ref(q, kd, vd, True, 1, 0, None, 0.0)
     tol = torch.exp2(torch.floor(torch.log2(ref.abs())) - 11) + 2.0 ** -16 * a
     assert ((out.double() - ref).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------ rows that are not finite, operands head by head
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+@pytest.mark.parametrize("n,m,splits", [(2, 5000, 16), (200, 5000, 2), (40000, 300, 1)])
+def test_a_query_that_is_not_finite_reaches_its_own_row_only(ctx, dtype, cap, n, m, splits):
+    """Its row is NaN in every form of the launch (few rows, keys cut over a cluster, one CTA a tile)."""
+    g = gen(n)
+    q, k, v = (randn(g, r, 1, D, dtype=dtype) for r in (n, m, m))
+    shape = va.attention_plan_shape(1, 1, [0, n], [0, m])
+    assert (shape["splits"] == 1) == (splits == 1)
+    plan = va.AttentionPlan(ctx, 1, 1, [0, n], [0, m], score_cap=cap)
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    ctx.masked_attention(plan, q, k, v, clean)
+    q[1] = float("nan")
+    ctx.masked_attention(plan, q, k, v, out)
+    assert torch.isnan(out[1]).all()
+    others = torch.arange(n, device="cuda") != 1
+    if cap == 0:
+        assert torch.equal(out[others], clean[others])
+    assert torch.isfinite(out[others].float()).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_cached_query_that_is_not_finite_reaches_its_own_row_only(ctx, fmt):
+    g = gen(2)
+    for held in (3, 3000):
+        cache, codes, scales = new_cache(g, 1, 2, 3000, fmt)
+        k, v = randn(g, held, 2, D), randn(g, held, 2, D)
+        ctx.kv_cache_write(cache, k, v, i32([0, held]), i32([held]))
+        q = randn(g, 3, 4, D, dtype=BF16)
+        clean, out = torch.empty_like(q), torch.empty_like(q)
+        ctx.cache_attention(cache, q, clean, i32([0, 3]), i32([held]), max_tokens=3)
+        q[1, 2] = float("nan")
+        ctx.cache_attention(cache, q, out, i32([0, 3]), i32([held]), max_tokens=3)
+        assert torch.isnan(out[1, 2]).all()
+        out[1, 2] = clean[1, 2]
+        assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("n,m,heads,kvh", [(1, 3000, 4, 2), (300, 700, 6, 2), (3, 40, 3, 3)])
+def test_head_major_operands(ctx, n, m, heads, kvh):
+    g = gen(m)
+    q, k, v = (randn(g, h, r, D, dtype=BF16) for h, r in ((heads, n), (kvh, m), (kvh, m)))
+    plan = va.AttentionPlan(ctx, heads, kvh, [0, n], [0, m], causal=True)
+    want = torch.empty(n, heads, D, device="cuda", dtype=BF16)
+    ctx.masked_attention(plan, *(x.transpose(0, 1).contiguous() for x in (q, k, v)), want)
+    out = torch.empty(heads, n, D, device="cuda", dtype=BF16)
+    ctx.masked_attention(plan, *(x.transpose(0, 1) for x in (q, k, v)), out.transpose(0, 1))
+    assert torch.equal(out.transpose(0, 1), want)
+    results = []
+    for a, b, c in ((k, v, q), tuple(x.transpose(0, 1).contiguous().transpose(0, 1) for x in (k, v, q))):
+        cache, codes, scales = new_cache(gen(1), 1, kvh, m, torch.int8)
+        ctx.kv_cache_write(cache, a.transpose(0, 1), b.transpose(0, 1), i32([0, m]), i32([m]))
+        o = torch.empty_like(c)
+        ctx.cache_attention(cache, c.transpose(0, 1), o.transpose(0, 1), i32([0, n]), i32([m]), max_tokens=n)
+        back = torch.empty_like(k)
+        ctx.kv_cache_read(cache, i32([0, m]), back.transpose(0, 1), torch.empty_like(v).transpose(0, 1))
+        results.append((o.clone(), back, codes[1].clone()))
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    """No call needs one before it: everything that a launch sets up can be set up during a capture."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch, vestra_attn as va
+from test_gpu_stream import gen, i32, new_cache, randn
+ctx, g, bf = va.Context(va.default_config(max_rows=64), 0), gen(0), torch.bfloat16
+docs, cap = 16, 8192
+cache, codes, scales = new_cache(g, docs, 4, cap, torch.int8)
+q, k, v = randn(g, 64, 4, 64, dtype=bf), randn(g, 64, 4, 64, dtype=bf), randn(g, 64, 4, 64, dtype=bf)
+plans = [va.AttentionPlan(ctx, 4, 4, [0, n], [0, 64]) for n in (64, 1)]
+ends, lens, pos = i32([4 * b for b in range(docs + 1)]), i32([4] * docs), i32([[i] for i in range(64)])
+outs = [torch.zeros_like(q) for _ in range(6)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+def calls(outs, s):
+    ctx.rope_axes(va.RopeAxes((64,)), pos, q, outs[0], stream=s)
+    ctx.kv_cache_write(cache, k, v, ends, lens, stream=s)
+    ctx.masked_attention(plans[0], q, k, v, outs[1], stream=s)
+    ctx.masked_attention(plans[1], q, k, v, outs[2], stream=s)
+    ctx.cache_attention(cache, q, outs[3], ends, lens, max_tokens=4, stream=s)
+    ctx.kv_cache_read(cache, ends, outs[4], outs[5], stream=s)
+with torch.cuda.graph(graph):
+    calls(outs, torch.cuda.current_stream().cuda_stream)
+graph.replay()
+torch.cuda.synchronize()
+again = [torch.zeros_like(q) for _ in range(6)]
+calls(again, 0)
+torch.cuda.synchronize()
+ctx.check_device()
+assert all(torch.equal(a, b) and b.any() for a, b in zip(outs, again))
+graph.reset()
+""" % (os.path.dirname(os.path.abspath(__file__)), os.path.dirname(va.__file__))
+    assert subprocess.run([sys.executable, "-c", code], timeout=300).returncode == 0

@@ -753,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           lt *= old;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (q[e].x != -INFINITY) {
+            if (q[e].y != 0.0f) {  // keys seen (a row of NaN scores has a NaN sum and no maximum)
               const float f = ex2(q[e].x - m_new);
               sum.x += f * v[e].x, sum.y += f * v[e].y, sum.z += f * v[e].z, sum.w += f * v[e].w;
               lt += f * q[e].y;
