@@ -29,6 +29,8 @@ struct Seen {
   int64_t items, most_keys;      // masked: work items, keys of the longest
   int64_t token_stride[2], head_stride[2];
   float slope[4];
+  int64_t rope_chunk, rope_pairs;
+  uint8_t rope_first[128], rope_second[128];
 } seen;
 
 void launched(const va::HeadsRef& a, const va::HeadsRef& b) {
@@ -94,6 +96,10 @@ int rows_splits(int64_t, int, int) { return 1; }
 int masked_splits(const int*, int64_t, int, int) { return 1; }
 cudaError_t launch_rope_axes(const RopeAxesArgs& a, int, cudaStream_t) {
   launched(a.in[0], a.out[0]);
+  seen.rope_chunk = a.chunk;
+  seen.rope_pairs = a.pairs;
+  std::memcpy(seen.rope_first, a.first, sizeof(a.first));
+  std::memcpy(seen.rope_second, a.second, sizeof(a.second));
   return cudaSuccess;
 }
 cudaError_t launch_kv_write(const KvCacheRef&, int, int64_t, const int32_t*, const int32_t*, const HeadsRef& k,

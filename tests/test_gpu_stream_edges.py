@@ -477,3 +477,28 @@ assert all(torch.equal(a, b) and b.any() for a, b in zip(outs, again))
 graph.reset()
 """ % (os.path.dirname(os.path.abspath(__file__)), os.path.dirname(va.__file__))
     assert subprocess.run([sys.executable, "-c", code], timeout=300).returncode == 0
+
+
+# ------------------------------------------------------------------ rotary operands off every vector boundary
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("pairing", [0, 1])
+@pytest.mark.parametrize("offset,pad,gap", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (3, 2, 5), (2, 0, 4), (4, 4, 0), (8, 8, 8)])
+@pytest.mark.parametrize("sections,layout", [((2,), "per_axis"), ((20, 22, 22), "per_axis"), ((20, 22, 20), "shared"),
+                                             ((16, 24, 24), "per_axis"), ((64,), "shared")])
+def test_rope_at_any_offset_and_stride(ctx, dtype, pairing, offset, pad, gap, sections, layout):
+    from test_gpu_stream import rope_ref, rope_tol
+    g = gen(offset + 10 * pad)
+    rows, heads, d = 9, 3, sum(sections) + 2
+    flat = randn(g, offset + rows * (heads * (d + pad) + gap), dtype=dtype)
+    x = flat.as_strided((rows, heads, d), (heads * (d + pad) + gap, d + pad, 1), offset)
+    pos = torch.randint(-100, 100, (rows, len(sections)), generator=g, device="cuda", dtype=torch.int32)
+    rope = va.RopeAxes(sections, 100.0, layout, pairing)
+    ref = rope_ref(x, pos, sections, 100.0, layout, pairing)
+    out = torch.full_like(flat, 7.0).as_strided(x.shape, x.stride(), offset)
+    ctx.rope_axes(rope, pos, x, out)
+    assert (out.double() - ref).abs().max() <= rope_tol(x, dtype)
+    outside = torch.ones_like(flat, dtype=torch.bool)
+    outside.as_strided(x.shape, x.stride(), offset).fill_(False)
+    keep = flat.clone()
+    ctx.rope_axes(rope, pos, x, x)
+    assert torch.equal(x, out) and torch.equal(flat[outside], keep[outside])

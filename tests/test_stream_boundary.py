@@ -17,7 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 class Seen(ctypes.Structure):
     _fields_ = [("launches", ctypes.c_int64), ("unfinished", ctypes.c_int64), ("items", ctypes.c_int64),
                 ("most_keys", ctypes.c_int64), ("token_stride", ctypes.c_int64 * 2), ("head_stride", ctypes.c_int64 * 2),
-                ("slope", ctypes.c_float * 4)]
+                ("slope", ctypes.c_float * 4), ("rope_chunk", ctypes.c_int64), ("rope_pairs", ctypes.c_int64),
+                ("rope_first", ctypes.c_uint8 * 128), ("rope_second", ctypes.c_uint8 * 128)]
 
 
 @pytest.fixture(scope="module")
@@ -183,3 +184,57 @@ def test_a_few_rows_of_a_long_head_major_buffer(lib, rows):
     packed, n, heads = va._heads(view_on_device(x[:, 5:5 + rows].transpose(0, 1)), 0, "q", 64)
     assert (n, heads) == (rows, 16)
     assert every_call(lib, packed, rows, 16) == [va.VA_OK] * 6
+
+
+# ------------------------------------------------------------------------------ rotary vectors
+@pytest.mark.parametrize("dtype,size", [(va.VA_BF16, 2), (va.VA_F16, 2), (va.VA_F32, 4)])
+@pytest.mark.parametrize("pairing", [0, 1])
+@pytest.mark.parametrize("layout", ["per_axis", "shared"])
+def test_every_rotary_vector_is_aligned(lib, dtype, size, pairing, layout):
+    """Random offsets, strides and sections: each vector that the chosen chunk loads or stores starts at a multiple
+    of its size, and the chunk is as wide as that allows."""
+    rng = np.random.default_rng(10 * pairing + size + len(layout))
+    chunks = set()
+    for _ in range(400):
+        sections = [2 * int(rng.choice([1, 3, 4, 5, 8, 12, 16, 32])) for _ in range(int(rng.integers(1, 4)))]
+        d, heads, rows = sum(sections) + 2 * int(rng.integers(0, 3)), int(rng.integers(1, 4)), int(rng.integers(1, 4))
+        if d > 256:
+            continue
+        tensors = []
+        for at in (PTR, 2 * PTR):  # input and output
+            head = d + int(rng.choice([0, 0, 1, 2, 6, 8]))
+            token = heads * head + int(rng.choice([0, 0, 0, 1, 4, 8]))
+            tensors.append((at + size * int(rng.choice([0, 0, 0, 1, 2, 3, 4, 8])), token, head))
+        rope = va.VaRopeAxes(len(sections), (ctypes.c_int32 * 4)(*sections), va.ROPE_LAYOUTS[layout], pairing, 100.0)
+        packed = [heads_of(t, h, heads, dtype, p) for p, t, h in tensors]
+        assert lib.va_rope_axes_device(lib.ctx, ctypes.byref(rope), rows, d, PTR, packed[0], packed[1], None, None, 0) == va.VA_OK
+        seen = lib.fake_seen().contents
+        v, pairs = seen.rope_chunk, seen.rope_pairs
+
+        def aligned(v):
+            if pairs % v:
+                return False
+            n = v * (2 if pairing else 1)
+            starts = {0}
+            for p, t, h in tensors:
+                for r in range(rows):
+                    for k in range(heads):
+                        for at in range(0, pairs, v):
+                            first, second = seen.rope_first[at], seen.rope_second[at]
+                            # the chunk's pairs lie in a row
+                            for e in range(v):
+                                step = 2 * e if pairing else e
+                                if (seen.rope_first[at + e], seen.rope_second[at + e]) != (first + step, second + step):
+                                    return False
+                            base = p + size * (r * t + k * h)
+                            starts |= {(base + size * c) % (size * n) for c in ((first,) if pairing else (first, second))}
+            return starts == {0}
+
+        chunks.add(v)
+        if v == 0:
+            assert pairing == 1 and not aligned(1)  # element by element
+            continue
+        assert aligned(v)
+        if 2 * v * (2 if pairing else 1) * size <= 16 and len(sections) == 1 and rows > 1 and heads > 1:
+            assert not aligned(2 * v)
+    assert chunks == ({0, 1, 2, 4} if pairing and size == 2 else {0, 1, 2} if pairing else {1, 2, 4, 8} if size == 2 else {1, 2, 4})

@@ -322,11 +322,14 @@ struct RopeAxesArgs {
   uint8_t axis[kRopeMaxPairs];
   int pairs, axes, head_dim, rotated;  // rotated = sum of the sections
   int pairing;
-  int min_half;                       // gcd of the halves of all blocks and sections
+  int chunk;                          // pairs a thread takes as vectors (rope_chunk)
   int64_t rows;
   const int32_t* positions;
   HeadsRef in[2], out[2];             // q and k; heads 0: absent
 };
+// Pairs per chunk: 8, 4, 2 or 1, loaded as one vector of 2 chunk elements (pairing 1) or two of chunk elements
+// (pairing 0); 0: pairs whose elements are loaded one by one.
+int rope_chunk(const RopeAxesArgs& a, int min_half, int elem_bytes);
 cudaError_t launch_rope_axes(const RopeAxesArgs& a, int dtype, cudaStream_t st);
 
 struct KvCacheRef {

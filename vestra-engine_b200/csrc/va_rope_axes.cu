@@ -48,8 +48,8 @@ __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bflo
 template <>
 __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
 
-template <class T, int N>
-struct alignas(sizeof(T) * N) Vec {
+template <class T, int N, bool kAligned = true>
+struct alignas(kAligned ? sizeof(T) * N : sizeof(T)) Vec {
   T v[N];
 };
 
@@ -72,15 +72,15 @@ __device__ __forceinline__ float2 turn_cos_sin(int position, uint64_t turns) {
   }
 }
 
-// V pairs per chunk; kInter: pairs are neighbours (2i, 2i+1), one vector of 2V elements;
-// otherwise two vectors of V elements, min_half a multiple of V.
-template <class T, int V, bool kInter>
+// V pairs per chunk; kInter: pairs are neighbours (2i, 2i+1), one vector of 2V elements, or, where that is not
+// aligned (kAligned false, V = 1), two loads of an element; otherwise two vectors of V elements.
+template <class T, int V, bool kInter, bool kAligned>
 __global__ void __launch_bounds__(kMaxThreads) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a) {
   constexpr int kRows = rows_per_block<T, V, kInter>();
   extern __shared__ float4 table[];  // cosines [kRows][pairs], then sines: a chunk's are one vector each
   float* cosines = reinterpret_cast<float*>(table);
   float* sines = cosines + kRows * a.pairs;
-  using Part = Vec<T, kInter ? 2 * V : V>;
+  using Part = Vec<T, kInter ? 2 * V : V, kAligned>;
   constexpr int kVecs = kInter ? 1 : 2;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
   const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), a.rows - row0));
@@ -156,9 +156,9 @@ __global__ void __launch_bounds__(kMaxThreads) rope_axes_kernel(const __grid_con
   }
 }
 
-template <class T, int V>
-cudaError_t launch_v(const RopeAxesArgs& a, cudaStream_t st) {
-  const int rows = a.pairing ? rows_per_block<T, V, true>() : rows_per_block<T, V, false>();
+template <class T, int V, bool kInter, bool kAligned = true>
+cudaError_t launch(const RopeAxesArgs& a, cudaStream_t st) {
+  constexpr int rows = rows_per_block<T, V, kInter>();
   const int64_t blocks = (a.rows + rows - 1) / rows;
   const int items = (a.in[0].heads + a.in[1].heads) * (a.pairs / V);
   // As few threads past the items as the warp size allows.
@@ -167,41 +167,38 @@ cudaError_t launch_v(const RopeAxesArgs& a, cudaStream_t st) {
   if (blocks > 0x7fffffff || parts > 65535) return cudaErrorInvalidValue;
   const size_t smem = 2 * sizeof(float) * rows * a.pairs;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
-  if (a.pairing)
-    rope_axes_kernel<T, V, true><<<grid, threads, smem, st>>>(a);
-  else
-    rope_axes_kernel<T, V, false><<<grid, threads, smem, st>>>(a);
+  rope_axes_kernel<T, V, kInter, kAligned><<<grid, threads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
-// The widest chunk (in pairs) that every block, pointer and stride allows, at most
-// 16 bytes a vector.
 template <class T>
 cudaError_t launch_t(const RopeAxesArgs& a, cudaStream_t st) {
-  const int per_pair = a.pairing ? 2 : 1;  // elements of one vector per pair
-  int v = 16 / static_cast<int>(sizeof(T)) / per_pair;
-  for (; v > 1; v >>= 1) {
-    bool ok = a.min_half % v == 0;
-    for (int w = 0; w < 2; ++w) {
-      if (a.in[w].heads == 0) continue;
-      for (const HeadsRef* h : {&a.in[w], &a.out[w]}) {
-        const int e = v * per_pair;
-        ok = ok && reinterpret_cast<uintptr_t>(h->data) % (sizeof(T) * e) == 0 && h->token_stride % e == 0 &&
-             h->head_stride % e == 0;
-      }
+  if (a.pairing) {
+    switch (a.chunk) {
+      case 4:
+        if constexpr (sizeof(T) == 2) return launch<T, 4, true>(a, st);
+        break;
+      case 2:
+        return launch<T, 2, true>(a, st);
+      case 1:
+        return launch<T, 1, true>(a, st);
+      case 0:
+        return launch<T, 1, true, false>(a, st);
     }
-    if (ok) break;
+  } else {
+    switch (a.chunk) {
+      case 8:
+        if constexpr (sizeof(T) == 2) return launch<T, 8, false>(a, st);
+        break;
+      case 4:
+        return launch<T, 4, false>(a, st);
+      case 2:
+        return launch<T, 2, false>(a, st);
+      case 1:
+        return launch<T, 1, false>(a, st);
+    }
   }
-  switch (v) {
-    case 8:
-      if constexpr (sizeof(T) == 2) return launch_v<T, 8>(a, st);
-    case 4:
-      return launch_v<T, 4>(a, st);
-    case 2:
-      return launch_v<T, 2>(a, st);
-    default:
-      return launch_v<T, 1>(a, st);
-  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace

@@ -258,6 +258,25 @@ int cache_rows_call(va_ctx* c, const va_kv_cache* cache, int64_t rows, const int
 }  // namespace
 
 namespace va {
+// The widest vectors that every block (min_half: the gcd of their halves), pointer and stride allows, at most 16
+// bytes.
+int rope_chunk(const RopeAxesArgs& a, int min_half, int elem_bytes) {
+  const int per_pair = a.pairing ? 2 : 1;  // elements of one vector per pair
+  for (int v = 16 / elem_bytes / per_pair; v >= 1; v >>= 1) {
+    bool ok = min_half % v == 0;
+    for (int w = 0; w < 2; ++w) {
+      if (a.in[w].heads == 0) continue;
+      for (const HeadsRef* h : {&a.in[w], &a.out[w]}) {
+        const int e = v * per_pair;
+        ok = ok && reinterpret_cast<uintptr_t>(h->data) % (elem_bytes * e) == 0 && h->token_stride % e == 0 &&
+             h->head_stride % e == 0;
+      }
+    }
+    if (ok) return v;
+  }
+  return 0;  // pairing 1 only: there one pair is a vector of two elements already
+}
+
 cudaError_t prepare_kernel(const void* kernel, int smem_bytes, std::atomic<uint64_t>& ready) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -344,7 +363,7 @@ int va_rope_axes_device(va_ctx* c, const va_rope_axes* rope, int64_t rows, int h
   a.head_dim = head_dim;
   a.rotated = total;
   a.pairing = rope->pairing;
-  a.min_half = g;
+  a.chunk = va::rope_chunk(a, g, elem_size(q->dtype));
   a.rows = rows;
   a.positions = positions;
   const va::CtxCore core = va::ctx_core(c);
