@@ -238,3 +238,24 @@ def test_every_rotary_vector_is_aligned(lib, dtype, size, pairing, layout):
         if 2 * v * (2 if pairing else 1) * size <= 16 and len(sections) == 1 and rows > 1 and heads > 1:
             assert not aligned(2 * v)
     assert chunks == ({0, 1, 2, 4} if pairing and size == 2 else {0, 1, 2} if pairing else {1, 2, 4, 8} if size == 2 else {1, 2, 4})
+
+
+# ------------------------------------------------------------------------------ arrays read on the device
+@pytest.mark.parametrize("which", ["positions", "offsets", "lens", "first", "prefix", "slopes"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_arrays_off_their_types_alignment_are_refused(lib, which, off):
+    """An int32 or F32 array at an odd address would be a misaligned access in the kernel."""
+    h = heads_of(256, 64, 4)
+    cache, terms = cache_of(4), va.VaAttnTerms(4, 4, 1, 1, 0.0, 0.0)
+    rope = va.VaRopeAxes(1, (ctypes.c_int32 * 4)(64), 0, 0, 100.0)
+    at = {k: PTR + (off if k == which else 0) for k in ("positions", "offsets", "lens", "first", "prefix", "slopes")}
+    calls = {
+        "rope": lambda: lib.va_rope_axes_device(lib.ctx, ctypes.byref(rope), 3, 64, at["positions"], h, h, None, None, 0),
+        "write": lambda: lib.va_kv_cache_write_device(lib.ctx, ctypes.byref(cache), 3, at["offsets"], at["lens"], h, h, 0),
+        "read": lambda: lib.va_kv_cache_read_device(lib.ctx, ctypes.byref(cache), 3, at["offsets"], at["first"], h, h, 0),
+        "attend": lambda: lib.va_cache_attention_device(lib.ctx, ctypes.byref(cache), ctypes.byref(terms), 3, at["offsets"],
+                                                        at["lens"], 1, at["prefix"], at["slopes"], h, h, 0)}
+    uses = {"positions": ["rope"], "offsets": ["write", "read", "attend"], "lens": ["write", "attend"], "first": ["read"],
+            "prefix": ["attend"], "slopes": ["attend"]}[which]
+    for name, call in calls.items():
+        assert call() == (va.VA_ERR_INVALID if name in uses else va.VA_OK), name

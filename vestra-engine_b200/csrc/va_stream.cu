@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
 #include <new>
 #include <vector>
 
@@ -61,6 +62,13 @@ int launched(va_ctx* c, cudaError_t e, const char* what) {
 int bad(va_ctx* c, const char* msg) { return va::ctx_fail(c, VA_ERR_INVALID, msg); }
 
 int elem_size(int dtype) { return dtype == VA_F32 ? 4 : 2; }
+
+// int32 and F32 arrays that kernels read (nullptr passes).
+bool words_ok(std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if (reinterpret_cast<uintptr_t>(p) % 4) return false;
+  return true;
+}
 
 // No two elements of [rows][heads][head_dim] share an address: either the heads lie inside a
 // token's stride or the tokens inside a head's.  A stride that is never stepped over may be anything.
@@ -240,10 +248,11 @@ va::KvCacheRef cache_ref(const va_kv_cache* c) {
   return r;
 }
 
-int cache_rows_call(va_ctx* c, const va_kv_cache* cache, int64_t rows, const int32_t* offsets, const va_heads* k,
-                    const va_heads* v) {
+int cache_rows_call(va_ctx* c, const va_kv_cache* cache, int64_t rows, const int32_t* offsets, const int32_t* edge,
+                    const va_heads* k, const va_heads* v) {
   if (const char* m = check_cache(cache)) return bad(c, m);
   if (!offsets || !k || !v) return bad(c, "offsets, k and v must be given");
+  if (!words_ok({offsets, edge})) return bad(c, "offsets, lens and first must be 4-byte aligned");
   if (rows < 0 || rows > kMaxRows) return bad(c, "rows must be 0..2^31 - 1");
   if (k->dtype < VA_BF16 || k->dtype > VA_F32 || v->dtype != k->dtype) return bad(c, "k and v must have one type");
   for (const va_heads* h : {k, v}) {
@@ -332,6 +341,7 @@ int va_rope_axes_device(va_ctx* c, const va_rope_axes* rope, int64_t rows, int h
   }
   if (rows == 0) return VA_OK;
   if (!positions) return bad(c, "positions must be given");
+  if (!words_ok({positions})) return bad(c, "positions must be 4-byte aligned");
   const bool shared = rope->layout == VA_ROPE_SHARED;
   int start = 0, n = 0, g = 0;
   auto gcd = [](int x, int y) {
@@ -480,7 +490,7 @@ int va_masked_attention_device(va_ctx* c, const va_attn_plan* p, const va_heads*
 int va_kv_cache_write_device(va_ctx* c, const va_kv_cache* cache, int64_t rows, const int32_t* offsets,
                              const int32_t* lens, const va_heads* k, const va_heads* v, void* stream) {
   if (!c) return VA_ERR_INVALID;
-  const int rc = cache_rows_call(c, cache, rows, offsets, k, v);
+  const int rc = cache_rows_call(c, cache, rows, offsets, lens, k, v);
   if (rc) return rc;
   if (!lens) return bad(c, "lens must be given");
   const va::CtxCore core = va::ctx_core(c);
@@ -494,7 +504,7 @@ int va_kv_cache_write_device(va_ctx* c, const va_kv_cache* cache, int64_t rows, 
 int va_kv_cache_read_device(va_ctx* c, const va_kv_cache* cache, int64_t rows, const int32_t* offsets,
                             const int32_t* first, const va_heads* k, const va_heads* v, void* stream) {
   if (!c) return VA_ERR_INVALID;
-  const int rc = cache_rows_call(c, cache, rows, offsets, k, v);
+  const int rc = cache_rows_call(c, cache, rows, offsets, first, k, v);
   if (rc) return rc;
   const va::CtxCore core = va::ctx_core(c);
   DeviceScope scope(core.device);
@@ -512,6 +522,7 @@ int va_cache_attention_device(va_ctx* c, const va_kv_cache* cache, const va_attn
   if (const char* m = check_terms(terms)) return bad(c, m);
   if (terms->kv_heads != cache->kv_heads) return bad(c, "terms and cache differ in kv_heads");
   if (!offsets || !lens || !q || !out) return bad(c, "offsets, lens, q and out must be given");
+  if (!words_ok({offsets, lens, prefix, slopes})) return bad(c, "offsets, lens, prefix and slopes must be 4-byte aligned");
   if (rows < 0 || rows > kMaxRows / terms->heads) return bad(c, "rows * heads must be below 2^31");
   if (max_tokens < 1) return bad(c, "max_tokens must be at least 1");
   if (q->dtype != VA_BF16 && q->dtype != VA_F16) return bad(c, "cache attention takes BF16 or F16");
