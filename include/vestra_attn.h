@@ -421,7 +421,9 @@ typedef struct va_attn_terms {
  * magnitudes at most 2^96, or NULL (score and bias are summed in F32).  Create allocates
  * device memory (not during a capture) and returns with the plan on the device, ready for
  * any stream; a plan serves any number of calls, also at once, and is destroyed when none is
- * running, and before its context. */
+ * running, and before its context.  All query tiles of a plan are cut alike over their keys:
+ * single tokens over documents much longer than the others want a plan of their own.  Create
+ * and destroy take 35 to 50 us together; destroy waits for the device. */
 typedef struct va_attn_plan va_attn_plan;
 int va_attn_plan_create(va_ctx* ctx, const va_attn_terms* terms, int documents, const int64_t* q_offsets,
                         const int64_t* k_offsets, const int64_t* prefix, const float* slopes,

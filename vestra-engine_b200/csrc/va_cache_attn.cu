@@ -27,12 +27,12 @@
 // and then, through distributed shared memory, across the cluster in rank order: one
 // launch, no workspace, no atomics, and the same bits on every run.
 //
-// Measured on B200: one token over 10,392 int8 tokens x 12 heads 9.7 us; 16 documents of 0 to 32,000 e4m3
-// tokens, 22 rows, 4 key heads, cap and bias, 36 us; 16 documents of 32,000, cap and bias off, 61 us (4.6 TB/s), and x 16
-// key heads 188 us (5.9 TB/s = 0.90 of measured).  A warp's chunk takes about 2.5 us with 12 warps on the SM and 1.1 us
-// with 4: some 900 instructions of conversions, score terms and softmax (58% of issue slots), not the loads.
+// Measured on B200: one token over 10,392 int8 tokens x 12 heads 9.5 us; 16 documents of 0 to 32,000 e4m3
+// tokens, 22 rows, 4 key heads, cap and bias, 35 us; 16 documents of 32,000, cap and bias off, caches in turn, 51 us
+// (5.4 TB/s), and x 16 key heads 179 us (6.2 TB/s = 0.95 of measured).  A warp's chunk takes about 2.5 us with 12 warps
+// on the SM and 1.1 us with 4: some 900 instructions of conversions, score terms and softmax (58% of issue slots), not the loads.
 // Masks are applied to chunks that some row does not see whole only, and scales lie in the order of the
-// fragments (with one product per value scale: 37.4 -> 36.0 us, 64 -> 61, 3 to 5% elsewhere).
+// fragments.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -596,11 +596,13 @@ cudaError_t launch_cache_attention(const KvCacheRef& c, const AttnTerms& t, int 
   bool paired = false;  // two documents share a cluster
   int64_t shared_by = c.documents;  // clusters per key head and block of rows
   // From 8 documents on, a long and a short one share a cluster and divide its CTAs by their lengths, where that
-  // is two to six each on average, the clusters all fit with hardly fewer CTAs, and a capacity of 8192 pays for the sorting.  Measured (us, own
-  // clusters / shared; lengths random / equal): 64 documents x 2 key heads of up to 32,000 84 / 68, 102 / 104; 20 x 4
-  // 58 / 48, 63 / 65; 16 x 12 of up to 9,000 36 / 30, 47 / 49; 16 x 4 of up to 32,000, where clusters of 10 are the largest
-  // that fit, 41 / 36, 56 / 65 (the mixed batch above 48 / 37).  Outside the rule: 4 x 16 of up to 32,000 46 / 51, 54 / 64;
-  // 8 x 4 27 / 29, 33 / 44; 16 x 12 of up to 2,000 11.4 / 11.7, 14.7 / 15.9.
+  // is two to six each on average, the clusters all fit with hardly fewer CTAs, and a capacity of 8192 pays for the
+  // sorting.  Measured (us, own clusters / shared, e4m3, 4 query heads a key head, caches in turn; lengths random /
+  // equal): 64 documents x 2 key heads of up to 32,000 68 / 51, 88 / 90; 20 x 4 43 / 35, 58 / 59; 16 x 12 of up to
+  // 9,000 32 / 28, 42 / 42; 16 x 4 of up to 32,000, where clusters of 10 are the largest that fit, 38 / 32, 47 / 51:
+  // the lengths are on the device, so equal ones pay up to 8 % for what unequal ones gain.  Outside the rule
+  // (sharing forced): 4 x 16 of up to 32,000 46 / 51, 54 / 64; 8 x 4 27 / 29, 33 / 44; 16 x 12 of up to 2,000 11.4 / 11.7,
+  // 14.7 / 15.9.
   if (fit >= 2 && fit <= 6 && c.documents >= 8 && c.documents <= kMaxPaired && c.capacity >= 8192) {
     const int64_t both = (c.documents + 1) / 2;
     for (int s = 2 * static_cast<int>(fit); 3 * s >= 5 * fit && !paired; s -= 2) {

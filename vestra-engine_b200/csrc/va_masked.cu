@@ -26,11 +26,15 @@
 // partial rows meet through distributed shared memory in rank order: no workspace, no
 // second launch, the same bits on every run.
 //
-// Bound by the exponentials (one per 256 FLOP, 18.3 a clock and SM): a plain tile takes 1163 to
-// 1460 cycles of an SM against 896 of MUFU.  Measured on B200: full waves 763 TFLOP/s; four packed f16
-// documents of 731 to 4,330 tokens x 12 heads 129 us (637 TFLOP/s); a 10,392-token window with cap 30
-// 497 to 520 us (640 to 668); 866 new rows over 10,392 keys, cap 50, three CTAs a tile, 60 us (462);
-// causal documents with a distance bias, 16 / 4 heads, 87 us (490).
+// What bounds it: this form runs all exponentials on MUFU (one per 256 FLOP, 18.3 a clock and SM: 0.46 us of a
+// 128 x 128 tile at 1.965 GHz); in full waves a tile takes 0.81 us of an SM, the rest being what two CTAs do not hide
+// of its chain.  MUFU is no floor of the operator: the layer path's key-split kernel gives part of the exponentials to
+// FMA warps and runs the plain 10,392-token window at 811 TFLOP/s with a row maximum, this one at 724.
+// Measured on B200: full waves 763 TFLOP/s; four packed f16 documents of 731 to 4,330 tokens x 12 heads 129 us
+// (637 TFLOP/s); a 10,392-token window x 12 heads without a cap 458 us, with cap 30 490 to 525 (632 to 677 TFLOP/s),
+// with cap 60 633, in f16 with cap 30 656, and 1084 where scores pass 0.6 of the cap (an exponential and a reciprocal
+// more each); 866 new rows over 10,392 keys, cap 50, three CTAs a tile, 58 us (476), without a cap 56; causal documents
+// with a distance bias, 16 / 4 heads, 87 us (490).
 #include <algorithm>
 #include <atomic>
 #include <queue>
@@ -38,6 +42,7 @@
 
 #include "va_internal.h"
 #include "va_ptx.cuh"
+#include "va_stream.cuh"
 #include "va_tmem16.cuh"
 
 namespace va {
@@ -106,18 +111,6 @@ struct Ctl {
   __device__ uint32_t sV(int s) const { return base + Smem::kV + s * kTileBytes; }
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
   const unsigned long long t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity)) {
@@ -131,15 +124,6 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  return a;
-}
 __device__ __forceinline__ float4 ld_cluster_v4(uint32_t a) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -582,7 +566,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int lim[2] = {limit[0] - k0 - c0, limit[1] - k0 - c0};
       uint32_t pk[32];  // 16x128b order: block k: (row 0 pair k), (row 1 pair k)
       uint64_t acc[2] = {0, 0};
-      auto emit = [&](int k, int i, uint64_t x) {  // the exponentials of a pair
+      // The exponentials of a pair.  They enter the second product in the operands' type (a tensor-core product has
+      // operands of one type), the sum in F32: against 64 bits the result is 1 to 9 % further off than an F32
+      // softmax rounded once (the 9 where a bias leaves few keys).
+      auto emit = [&](int k, int i, uint64_t x) {
         float x0, x1;
         f32x2_unpack(x, x0, x1);
         const float p0 = ex2(x0), p1 = ex2(x1);
@@ -866,7 +853,10 @@ double masked_time(const int* key_tiles, int64_t items, int kv_heads, int sms, i
 
 int masked_splits(const int* key_tiles, int64_t items, int kv_heads, int sms) {
   // Two rounds of CTAs and more: a cut gains nothing that the order does not give (816 and 984 tiles
-  // in 1 / 2 / 3 CTAs each: 129 / 152 / 180 and 508 / 530 / 561 us).
+  // in 1 / 2 / 3 CTAs each: 129 / 152 / 180 and 508 / 530 / 561 us).  That holds where the longest tile is short beside
+  // the whole; one count for all tiles does not suit a plan that mixes a prompt with single tokens over much
+  // longer documents (a causal prompt of 6,400 tokens x 12 heads 103 us, with one token over 32,000 keys 273, that token
+  // in a plan of its own 20): the header advises a plan for each kind.
   if (items == 0 || items * kv_heads >= 4 * static_cast<int64_t>(sms)) return 1;
   int best = 1;
   double best_time = masked_time(key_tiles, items, kv_heads, sms, 1);

@@ -18,6 +18,7 @@
 
 #include "va_internal.h"
 #include "va_ptx.cuh"
+#include "va_stream.cuh"
 
 namespace va {
 namespace rows {
@@ -26,18 +27,6 @@ constexpr int kHeadDim = 64;
 constexpr int kRowsPerBlock = 8;
 constexpr int kMaxCluster = 16;
 constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ void mma(__half /*type*/, float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm(
@@ -180,12 +169,8 @@ struct Part {
 };
 // Stores v at this address of CTA `rank` of the cluster.
 __device__ __forceinline__ void st_cluster(float* p, int rank, float v) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr(smem_u32(p), rank)), "f"(v) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Joins the warps' results of a row block (o, m, l of every lane; `back` undoes a scaling of o) and
 // the cluster's, and writes the block's rows.  base: output row of the first token; rb: the block.  The `splits` CTAs that share the

@@ -11,8 +11,8 @@
 //
 // A cluster of CTAs shares one (tile, key head, 8-row block); its warps take 32-key chunks in turn
 // through a ring of their own in shared memory (cp.async, one chunk ahead).  Measured on B200: one token
-// over 10,392 keys x 12 heads 9.9 us (16.8 in the tile kernel; 3.2 TB/s), of which a launch without
-// keys is 4: three chunks a warp and the cluster's join are the rest.
+// over 10,392 keys x 12 heads 9.4 us (16.8 in the tile kernel; 3.4 TB/s), of which a launch without
+// keys is 4: five or six chunks a warp, one after the other, and the cluster's join are the rest.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

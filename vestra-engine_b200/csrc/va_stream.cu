@@ -1,6 +1,6 @@
 // C-ABI layer of the streaming-attention operators: argument checks, the plan of the masked
 // attention (host work list), and the launches.  The kernels are in va_rope_axes.cu,
-// va_masked.cu, va_kv_cache.cu and va_cache_attn.cu.
+// va_masked.cu, va_rows_attn.cu, va_kv_cache.cu and va_cache_attn.cu.
 #include <algorithm>
 #include <cmath>
 #include <cstdio>

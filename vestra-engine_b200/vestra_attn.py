@@ -101,10 +101,6 @@ class VaModelConfig(ctypes.Structure):
     ]
 
 
-_lib = None
-_vp = ctypes.c_void_p
-_f32p = ctypes.POINTER(ctypes.c_float)
-
 class VaRopeAxes(ctypes.Structure):
     _fields_ = [("axes", ctypes.c_int32), ("section", ctypes.c_int32 * 4), ("layout", ctypes.c_int32),
                 ("pairing", ctypes.c_int32), ("base", ctypes.c_float)]
@@ -121,6 +117,9 @@ class VaKvCache(ctypes.Structure):
                 ("v_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p)]
 
 
+_lib = None
+_vp = ctypes.c_void_p
+_f32p = ctypes.POINTER(ctypes.c_float)
 _i32p = ctypes.POINTER(ctypes.c_int)
 
 
