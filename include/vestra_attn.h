@@ -443,7 +443,7 @@ int va_attn_plan_shape(const va_attn_terms* terms, int documents, const int64_t*
  * 2^79 (larger ones may overflow), and in rows whose keys all score near -score_cap values
  * below n * 2^-44 lose precision, n = the most keys a row sees (2^-30 for 2^14).  F16:
  * probabilities below 2^-25 of a row's largest lose precision, those below 2^-36 count as 0
- * (tiles of 16 rows or fewer: 2^-30 and 2^-40).  out may be q. */
+ * (tiles of 16 rows or fewer: 2^-29 and 2^-40).  out may be q. */
 int va_masked_attention_device(va_ctx* ctx, const va_attn_plan* plan, const va_heads* q, const va_heads* k,
                                const va_heads* v, const va_heads* out, void* stream);
 
@@ -469,11 +469,13 @@ typedef struct va_kv_cache {
 } va_kv_cache;
 /* Appends: rows [offsets[b], offsets[b+1]) of k and v become tokens [lens[b] - n,
  * lens[b]) of document b, n = offsets[b+1] - offsets[b]; lens = tokens held after the
- * call (a document without rows is left alone, its lens not looked at beyond the check).  offsets int32 [documents + 1] and lens int32 [documents] are device arrays,
- * read when the kernel runs (a captured call follows their contents).  rows = rows of
+ * call (a document without rows is left alone, its lens not looked at beyond the check).
+ * offsets int32 [documents + 1] and lens int32 [documents] are device arrays, read when the
+ * kernel runs (a captured call follows their contents).  rows = rows of
  * k and v; rows outside every document are not read.  A document with lens[b] - n < 0, lens[b] >
  * capacity, or offsets out of [0, rows] or descending is skipped and reported by
- * va_check_device (VA_ERR_DEVICE); where offsets descend, others may be skipped too.  k, v [rows, kv_heads] of one type. */
+ * va_check_device (VA_ERR_DEVICE); where offsets descend, others may be skipped too.  k, v
+ * [rows, kv_heads] of one type. */
 int va_kv_cache_write_device(va_ctx* ctx, const va_kv_cache* cache, int64_t rows, const int32_t* offsets,
                              const int32_t* lens, const va_heads* k, const va_heads* v, void* stream);
 /* Reads back: rows [offsets[b], offsets[b+1]) of k and v receive tokens first[b].. of
@@ -484,10 +486,11 @@ int va_kv_cache_read_device(va_ctx* ctx, const va_kv_cache* cache, int64_t rows,
                             const int32_t* first, const va_heads* k, const va_heads* v, void* stream);
 /* Attention of a few new tokens per document over the cache (terms as above): rows
  * [offsets[b], offsets[b+1]) of q are the last tokens of the lens[b] held, normally
- * just written.  prefix int32 [documents] and slopes F32 [heads] (magnitudes at
- * most 2^96, not checked) on the device, or NULL.  max_tokens: the most rows a document usually has (sizes the launch; more rows
- * are served too, more slowly).  q, out [rows, heads] BF16 or F16, 16-byte aligned,
- * strides multiples of 8 elements.  Bad offsets, or lens outside [0, capacity]: as
+ * just written.  prefix int32 [documents] and slopes F32 [heads] (magnitudes at most 2^96,
+ * not checked) on the device, or NULL.  max_tokens: the most rows a document usually has
+ * (sizes the launch; more rows are served too, more slowly).  q, out [rows, heads] BF16 or
+ * F16, 16-byte aligned, strides multiples of 8 elements; out may be q.  Probabilities below
+ * 2^-126 count as 0, and value scales below 2^-100 lose precision.  Bad offsets, or lens outside [0, capacity]: as
  * above, and the document's rows of out are left as they were.  For many new tokens
  * read the cache back and run va_masked_attention_device.  The codes of the tokens held
  * must not be e4m3's NaN (writing never makes one).  The same call gives the same bits; how

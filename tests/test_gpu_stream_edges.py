@@ -502,3 +502,22 @@ def test_rope_at_any_offset_and_stride(ctx, dtype, pairing, offset, pad, gap, se
     keep = flat.clone()
     ctx.rope_axes(rope, pos, x, x)
     assert torch.equal(x, out) and torch.equal(flat[outside], keep[outside])
+
+
+@pytest.mark.parametrize("docs,heads,kvh", [(3, 4, 2), (12, 4, 4), (40, 5, 1)])
+def test_cache_attention_over_its_queries(ctx, docs, heads, kvh):
+    """out may be q: every CTA of a cluster has read its rows before one is written."""
+    g = gen(docs)
+    cap = 8192 if docs >= 8 else 900
+    new = [1 + (5 * b) % 9 for b in range(docs)]
+    lens = [n + (997 * b) % (cap - 20) for b, n in enumerate(new)]
+    cache, codes, scales = new_cache(g, docs, kvh, cap, torch.int8)
+    k, v = randn(g, sum(lens), kvh, D), randn(g, sum(lens), kvh, D) * 40
+    ctx.kv_cache_write(cache, k, v, i32(np.cumsum([0] + lens)), i32(lens))
+    q = randn(g, sum(new), heads, D, dtype=BF16)
+    off, held, want = i32(np.cumsum([0] + new)), i32(lens), torch.empty_like(q)
+    ctx.cache_attention(cache, q, want, off, held, max_tokens=4)
+    for _ in range(10):
+        x = q.clone()
+        ctx.cache_attention(cache, x, x, off, held, max_tokens=4)
+        assert torch.equal(x, want)

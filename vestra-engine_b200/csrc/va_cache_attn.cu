@@ -17,9 +17,10 @@
 //   weight is at least 2^(E - 1 - kAlike).
 //   From the first chunk on where this does not hold, each row has its own E, above its own largest weight: a
 //   key that the row does not see, or that hardly counts in it, must not take the range from the others, whatever
-//   the values' sizes.
+//   the values' sizes (probabilities below 2^-126 are 0).
 // Either way a scaled weight has steps of 2^-24 and the row's largest is 2^(kTop - 1 - kAlike) or more.
-// One E per row in every chunk would cost 2 to 6 % (the weights' maximum stands between the scores and the product).
+// The weights' maximum then stands between the scores and the product: scales that span 2^6 and more make the mixed
+// batch below 38.5 us instead of 35, 16 x 32,000 x 16 key heads 224 instead of 202, one token 11.4 instead of 10.2.
 //
 // A cluster of CTAs shares one (document, key head, row block), or two documents' that divide its
 // CTAs; a warp takes 64-key chunks in turn through a ring of its own in shared memory (cp.async, one chunk ahead), each
