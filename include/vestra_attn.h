@@ -443,7 +443,9 @@ int va_attn_plan_shape(const va_attn_terms* terms, int documents, const int64_t*
  * 2^79 (larger ones may overflow), and in rows whose keys all score near -score_cap values
  * below n * 2^-44 lose precision, n = the most keys a row sees (2^-30 for 2^14).  F16:
  * probabilities below 2^-25 of a row's largest lose precision, those below 2^-36 count as 0
- * (tiles of 16 rows or fewer: 2^-29 and 2^-40).  out may be q. */
+ * (tiles of 16 rows or fewer: 2^-29 and 2^-40).  out may be q.  The same call gives the
+ * same bits; a document's last bits may follow the plan's other documents (form and cut of
+ * the launch), not their contents. */
 int va_masked_attention_device(va_ctx* ctx, const va_attn_plan* plan, const va_heads* q, const va_heads* k,
                                const va_heads* v, const va_heads* out, void* stream);
 
